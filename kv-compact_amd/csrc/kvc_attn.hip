@@ -1,0 +1,853 @@
+// Attention kernels on MI355X (include/kvc-cache.h): new or drafted tokens
+// over a paged cache, and whole prompts.
+//
+// One pass over the keys with a running maximum and sum per row:
+//   s = scale q.k + bias, m' = max(m, max s), a = exp(m - m'),
+//   p = exp(s - m'), l' = a l + sum p, o' = a o + p V; result o / l, lse m + log l.
+// The products run on matrix instructions in the transposed form
+//   S^T[key][row] = K Q^T,  O^T[column][row] = V^T P^T,
+// because a lane then holds one row in both: the scores it gets from the first
+// product are, as they lie in its registers, its part of the second one's
+// operand, and the row's maximum, sum and rescale need no transposition.
+//
+// Rows of a KV head are its tokens times the group's query heads, so that a
+// key is read once for all of them.
+#include "kvc_launch.h"
+
+#include <math.h>
+#include <stdint.h>
+
+namespace kvc {
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kF32 = KV_TYPE_F32, kF16 = KV_TYPE_F16, kBF16 = KV_TYPE_BF16, kQ8 = KV_TYPE_Q8_0;
+
+// Where rows of K or V stand: pages of a pool (table set), or one array.
+struct RowsAt {
+    const char * base;
+    long long ld_tok, ld_head;   // bytes
+};
+
+struct AttnArgs {
+    RowsAt k, v;
+    const char * q;
+    char * o;
+    long long q_tok, q_head, o_tok, o_head;   // elements
+    float * lse;
+    const int * cu;
+    const int * seqs;
+    const int * len;       // cells of each sequence, or nullptr: its tokens
+    const int * table;     // pages, or nullptr: contiguous tokens
+    const float * bias;    // this layer's [page][H][page_size], or nullptr
+    const unsigned long long * mask;
+    int mask_words, n_seq, n_tok, H, G, dk, dv;
+    int shift, n_pages, max_seqs, max_pages;
+    int splits, tiles;     // key ranges; row tiles the grid has for each sequence (0: flat over all sequences)
+    float scale;
+    float * part_o;        // [splits][n_tok * n_head][dv]
+    float * part_ml;       // [splits][n_tok * n_head][2]
+};
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// Exchange between lane groups 16 and 32 apart: the larger (sum) of the four
+// lanes that hold one row.
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+__device__ __forceinline__ float f16_value(unsigned short u) { return (float)__builtin_bit_cast(_Float16, u); }
+__device__ __forceinline__ float bf16_value(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
+
+template <int TYPE> __device__ __forceinline__ float value_of(const char * p, long long i) {
+    if constexpr (TYPE == kF32) return reinterpret_cast<const float *>(p)[i];
+    const unsigned short u = reinterpret_cast<const unsigned short *>(p)[i];
+    if constexpr (TYPE == kBF16) return bf16_value(u);
+    return f16_value(u);
+}
+
+// two fp32 values rounded (to nearest even) into one register of the 16-bit type
+template <int TYPE> __device__ __forceinline__ unsigned pack2(float a, float b) {
+    if constexpr (TYPE == kF16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        h2 r = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(unsigned, r);
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        b2 r = {(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(unsigned, r);
+    }
+}
+
+template <int TYPE> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
+    if constexpr (TYPE == kF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// N elements (16 bytes, or 8) from column `col` of a row of d: whole vectors
+// where rows are aligned and d is a multiple of the vector, one by one
+// otherwise. Nothing is read at or past column d.
+template <int N, int BYTES, bool CAREFUL> __device__ __forceinline__ void load_cols(const char * row, int col, int d,
+                                                                                     unsigned * out) {
+    constexpr int W = N * BYTES / 4;
+    if constexpr (!CAREFUL) {
+        if (col < d) {
+            if constexpr (W == 4)
+                *reinterpret_cast<u4 *>(out) = *reinterpret_cast<const u4 *>(row + (long long)col * BYTES);
+            else
+                *reinterpret_cast<u2 *>(out) = *reinterpret_cast<const u2 *>(row + (long long)col * BYTES);
+        } else {
+            for (int i = 0; i < W; i++) out[i] = 0;
+        }
+    } else {
+        for (int i = 0; i < W; i++) {
+            if constexpr (BYTES == 4) {
+                out[i] = col + i < d ? reinterpret_cast<const unsigned *>(row)[col + i] : 0;
+            } else {
+                const unsigned short * r = reinterpret_cast<const unsigned short *>(row);
+                const unsigned a = col + 2 * i < d ? r[col + 2 * i] : 0, b = col + 2 * i + 1 < d ? r[col + 2 * i + 1] : 0;
+                out[i] = a | b << 16;
+            }
+        }
+    }
+}
+
+typedef u2 u2_any __attribute__((aligned(2)));
+typedef unsigned u1_any __attribute__((aligned(2)));
+
+// signed byte i of a register pair, as fp32
+__device__ __forceinline__ float byte_value(const unsigned * w, int i) {
+    return (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)));
+}
+
+// Attention of RT tiles of 16 rows (of one KV head of one sequence) over a
+// range of keys; four waves of a block take alternate tiles of 32 keys and
+// join in LDS. TYPE: the type of the cache rows (kQ8: q and o are QT).
+// D: 64, 128 or 256, the head widths rounded up.
+//
+// Fragments (16x16x32, lane l, m = l % 16, g = l / 16): an operand's lane
+// holds row m and elements 8g .. 8g+7 of the summed axis, a result's lane
+// column m and rows 4g .. 4g+3. Keys of a 32-key tile are numbered on the
+// summed axis of the second product so that a lane's elements are the scores
+// it holds: 4g+i of the first 16 keys, then of the second. V's lane m holds
+// VW neighbouring columns of those keys, which makes VW fragments after a
+// 2 x 2 exchange of halves (v_perm), without LDS.
+// F32 sums 4 elements an instruction (16x16x4), one of them a lane's.
+// Q8_0: K's codes are exact in bf16, a block of 32 is one instruction, and its
+// scale multiplies the block's sums in fp32; V is the fp32 product of scale
+// and code as a sum of two bf16.
+template <int TYPE, int QT, int D, int RT, bool CAREFUL>
+struct RowKernel {
+    static constexpr int ES = TYPE == kF32 ? 4 : 2;          // bytes of a q element
+    static constexpr int KV = 16 / ES;                       // q / k elements a 16-byte load holds
+    static constexpr int NK = D / (4 * KV);                  // loads of a q or k row
+    static constexpr int VW = TYPE == kF32 ? 4 : (D / 16 < 8 ? D / 16 : 8);
+    static constexpr int NU = D / 16 / VW;                   // V loads of a row
+    static constexpr int NC = D / 16;                        // column fragments
+    static constexpr int NB = D / 32;                        // Q8_0 blocks
+    static constexpr bool Q8 = TYPE == kQ8;
+    static constexpr int WV = Q8 ? (VW + 3) / 4 : VW * ES / 4;    // registers of a V load
+    static constexpr int WK = Q8 ? 2 : 4;
+    static constexpr int NKL = Q8 ? NB : NK;
+    static constexpr int MT = Q8 ? kBF16 : TYPE;             // type on the matrix units
+    static constexpr bool SPLIT = Q8 && QT == kF16;          // q and p as two bf16 each
+
+    // fp16 weights are 2^10 times exp(s - m): those under 2^-24 of the largest, not 2^-14, lose bits
+    static constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f;
+    static constexpr float log_lift = TYPE == kF16 ? 6.93147180559945309417f : 0.0f;
+
+    // column of fragment c's lane m
+    static __device__ __forceinline__ int column(int m, int c) { return (c / VW) * 16 * VW + VW * m + c % VW; }
+};
+
+template <int TYPE, int QT, int D, int RT, bool CAREFUL>
+__global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
+    using C = RowKernel<TYPE, QT, D, RT, CAREFUL>;
+    constexpr int ROWS = 16 * RT, LD = D + 4;
+    constexpr bool Q8 = C::Q8;
+    __shared__ __align__(16) float join[4][ROWS][LD];
+    __shared__ float join_m[4][ROWS], join_l[4][ROWS];
+    __shared__ __align__(16) float scales[Q8 ? 4 : 1][2][32][Q8 ? C::NB : 1];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, g = lane >> 4;
+
+    // which rows: KV head h fastest, then the key range, the row tile, the sequence
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    const int split = u % a.splits;
+    u /= a.splits;
+    int s = 0, tile = 0, tile_step;
+    if (a.tiles) {
+        tile = u % a.tiles;
+        s = u / a.tiles;
+        tile_step = a.tiles;
+    } else {
+        // flat: the u-th row tile of all sequences together, longest keys first
+        // (the order inside a sequence is turned round)
+        int before = 0, found = -1;
+        for (int s0 = 0; s0 < a.n_seq && found < 0; s0 += 64) {
+            int tiles = 0;
+            if (s0 + lane < a.n_seq) {
+                const int n = a.cu[s0 + lane + 1] - a.cu[s0 + lane];
+                tiles = n > 0 ? (int)(((long long)n * a.G + ROWS - 1) / ROWS) : 0;
+            }
+            int incl = tiles;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned long long hit = __ballot(before + incl > u);
+            if (hit) {
+                const int w = __ffsll((long long)hit) - 1;
+                found = s0 + w;
+                tile = __shfl(tiles, w) - 1 - (u - before - (__shfl(incl, w) - __shfl(tiles, w)));
+            }
+            before += __shfl(incl, 63);
+        }
+        if (found < 0) return;
+        s = found;
+        tile_step = 1 << 30;
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    int tok0 = a.cu[s], tok1 = a.cu[s + 1];
+    tok0 = tok0 < 0 ? 0 : tok0;
+    tok1 = tok1 > a.n_tok ? a.n_tok : tok1;
+    const int n_new = tok1 - tok0;
+    if (n_new <= 0) return;
+    const int seq = a.table ? (a.seqs ? a.seqs[s] : s) : 0;
+    int held = n_new;   // keys of the sequence
+    const int * table = nullptr;
+    if (a.table) {
+        const bool there = seq >= 0 && seq < a.max_seqs;
+        held = there ? a.len[seq] : 0;
+        if (held < n_new || held > (long long)a.max_pages << a.shift) held = 0;
+        table = a.table + (long long)(there ? seq : 0) * a.max_pages;
+    }
+    const int base = held ? held - n_new : 0;   // keys that every token sees
+    const int rows = n_new * a.G;
+    const int page_mask = a.table ? (1 << a.shift) - 1 : 0;
+
+    for (; (long long)tile * ROWS < rows; tile += tile_step) {
+        const int row0 = tile * ROWS;
+        // keys this tile can see, and this block's range of them
+        int last_tok = (row0 + ROWS - 1) / a.G;
+        if (last_tok >= n_new) last_tok = n_new - 1;
+        const int end_all = held == 0 ? 0 : (a.mask ? held : base + last_tok + 1);
+        const int first_tok = row0 / a.G;
+        const int clear = a.mask ? base : base + first_tok + 1;   // keys before it are seen by every row
+        const int n_tiles = (end_all + 31) >> 5;
+        const int per = (n_tiles + a.splits - 1) / a.splits;
+        const int t_lo = split * per, t_hi = t_lo + per < n_tiles ? t_lo + per : n_tiles;
+
+        // rows of this lane
+        int tok[RT], head[RT];
+        bool on[RT];
+        u4 q[RT][C::NK], q_lo[C::SPLIT ? RT : 1][C::SPLIT ? C::NK : 1];
+        for (int r = 0; r < RT; r++) {
+            const int row = row0 + 16 * r + m;
+            on[r] = row < rows;
+            tok[r] = on[r] ? row / a.G : 0;
+            head[r] = on[r] ? row % a.G : 0;
+            const char * p = a.q + ((long long)(tok0 + tok[r]) * a.q_tok + (long long)(h * a.G + head[r]) * a.q_head) * C::ES;
+            for (int j = 0; j < C::NK; j++) {
+                unsigned w[4];
+                load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, w);
+                if constexpr (C::SPLIT) {
+                    // an fp16 value is the sum of two bf16
+                    unsigned hi[4], lo[4];
+                    for (int i = 0; i < 4; i++) {
+                        const float x = f16_value((unsigned short)w[i]), y = f16_value((unsigned short)(w[i] >> 16));
+                        const unsigned xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+                        hi[i] = xh >> 16 | yh;
+                        lo[i] = pack2<kBF16>(x - __uint_as_float(xh), y - __uint_as_float(yh));
+                    }
+                    q[r][j] = u4{hi[0], hi[1], hi[2], hi[3]};
+                    q_lo[r][j] = u4{lo[0], lo[1], lo[2], lo[3]};
+                } else {
+                    q[r][j] = u4{w[0], w[1], w[2], w[3]};
+                }
+            }
+        }
+        f4 acc[RT][C::NC];
+        float mx[RT], sum[RT];
+        for (int r = 0; r < RT; r++) {
+            mx[r] = -INFINITY;
+            sum[r] = 0.0f;
+            for (int c = 0; c < C::NC; c++) acc[r][c] = f4{0, 0, 0, 0};
+        }
+
+        // address of the first row of 16 keys, and whether they are on a good page
+        auto rows16 = [&](const RowsAt & x, int key, bool & ok, int & page) -> const char * {
+            ok = true;
+            page = 0;
+            if (!table) return x.base + (long long)(tok0 + key) * x.ld_tok + h * x.ld_head;
+            const int col = key >> a.shift;
+            page = key < held ? table[col] : -1;
+            ok = page >= 0 && page < a.n_pages;
+            if (!ok) page = 0;
+            return x.base + (((long long)page << a.shift) + (key & page_mask)) * x.ld_tok + h * x.ld_head;
+        };
+
+        unsigned kr[2][C::NKL][C::WK];
+        unsigned vr[8][C::NU][C::WV];
+        for (int t = t_lo + wave; t < t_hi; t += 4) {
+            const int key0 = t << 5;
+            bool ok[2];
+            int page[2];
+            // (contiguous rows end with the sequence: those past it repeat the last)
+            auto row_of = [&](int key) { return table ? key & 15 : (key < held ? key : held - 1) - (key & ~15); };
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const char * p = rows16(a.k, key0 + 16 * x, ok[x], page[x]) + (long long)row_of(key0 + 16 * x + m) * a.k.ld_tok;
+#pragma unroll
+                for (int j = 0; j < C::NKL; j++) {
+                    if constexpr (Q8) {
+                        *reinterpret_cast<u2 *>(kr[x][j]) = 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + 34 * j + 2 + 8 * g) : u2{0, 0};
+                    } else {
+                        load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                bool o2;
+                int p2;
+                const char * p0 = rows16(a.v, key0 + 16 * x, o2, p2);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const char * p = p0 + (long long)row_of(key0 + 16 * x + 4 * g + i) * a.v.ld_tok;
+#pragma unroll
+                    for (int w = 0; w < C::NU; w++) {
+                        const int col = C::column(m, w * C::VW);
+                        if constexpr (Q8) {
+                            const char * b = p + col / 32 * 34 + 2 + col % 32;
+                            if constexpr (C::WV == 2)
+                                *reinterpret_cast<u2 *>(vr[4 * x + i][w]) = col < a.dv ? *reinterpret_cast<const u2_any *>(b) : u2{0, 0};
+                            else
+                                vr[4 * x + i][w][0] = col < a.dv ? *reinterpret_cast<const u1_any *>(b) : 0;
+                        } else {
+                            load_cols<C::VW, C::ES, CAREFUL>(p, col, a.dv, vr[4 * x + i][w]);
+                        }
+                    }
+                }
+            }
+            if constexpr (Q8) {
+                // scales of K and V: lane pair per key, through LDS for the lanes that hold them elsewhere
+                const int key = lane >> 1, half = lane & 1;
+                bool o2;
+                int p2;
+                const char * pk = rows16(a.k, key0 + (key & 16), o2, p2) + (long long)(key & 15) * a.k.ld_tok;
+                const char * pv = rows16(a.v, key0 + (key & 16), o2, p2) + (long long)(key & 15) * a.v.ld_tok;
+                for (int b = half; b < C::NB; b += 2) {
+                    scales[wave][0][key][b] = 32 * b < a.dk ? f16_value(*reinterpret_cast<const unsigned short *>(pk + 34 * b)) : 0.0f;
+                    scales[wave][1][key][b] = 32 * b < a.dv ? f16_value(*reinterpret_cast<const unsigned short *>(pv + 34 * b)) : 0.0f;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            }
+
+            // S^T of both halves
+            f4 sc[RT][2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int r = 0; r < RT; r++) sc[r][x] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < C::NKL; j++) {
+                    if constexpr (TYPE == kF32) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int r = 0; r < RT; r++)
+                                sc[r][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    __uint_as_float(kr[x][j][e]), __uint_as_float(q[r][j][e]), sc[r][x], 0, 0, 0);
+                    } else if constexpr (Q8) {
+                        unsigned w[4];
+                        for (int e = 0; e < 4; e++)
+                            w[e] = __float_as_uint(byte_value(kr[x][j], 2 * e)) >> 16 |
+                                   (__float_as_uint(byte_value(kr[x][j], 2 * e + 1)) & 0xffff0000u);
+                        const u4 kf = {w[0], w[1], w[2], w[3]};
+#pragma unroll
+                        for (int r = 0; r < RT; r++) {
+                            f4 part = mfma16<kBF16>(kf, q[r][j], f4{0, 0, 0, 0});
+                            if constexpr (C::SPLIT) part = mfma16<kBF16>(kf, q_lo[r][j], part);
+                            for (int i = 0; i < 4; i++) sc[r][x][i] += scales[wave][0][16 * x + 4 * g + i][j] * part[i];
+                        }
+                    } else {
+                        const u4 kf = {kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]};
+#pragma unroll
+                        for (int r = 0; r < RT; r++) sc[r][x] = mfma16<C::MT>(kf, q[r][j], sc[r][x]);
+                    }
+                }
+            }
+            // scale, bias, masks: a key that a row does not see has -inf
+            const bool masked = key0 + 32 > clear || !ok[0] || !ok[1];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                float b[4] = {0, 0, 0, 0};
+                if (a.bias) {
+                    const int k = (key0 + 16 * x + 4 * g) & page_mask;   // four cells of one page
+                    const float * p = a.bias + (((long long)page[x] * a.H + h) << a.shift) + k;
+                    for (int i = 0; i < 4; i++) b[i] = p[i];
+                }
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+                    for (int i = 0; i < 4; i++) {
+                        float v = sc[r][x][i] * a.scale;
+                        if (a.bias) v = b[i] == -INFINITY ? -INFINITY : v + b[i];
+                        if (masked) {
+                            const int key = key0 + 16 * x + 4 * g + i, rel = key - base;
+                            bool see = key < held && ok[x];
+                            if (rel >= 0 && see) {
+                                if (a.mask)
+                                    see = rel < 64 * a.mask_words &&
+                                          (a.mask[(long long)(tok0 + tok[r]) * a.mask_words + (rel >> 6)] >> (rel & 63) & 1);
+                                else
+                                    see = rel <= tok[r];
+                            }
+                            if (!see) v = -INFINITY;
+                        }
+                        sc[r][x][i] = v;
+                    }
+            }
+            // running maximum and sum
+            float ref[RT];
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                float t0 = fmaxf(fmaxf(sc[r][0][0], sc[r][0][1]), fmaxf(sc[r][0][2], sc[r][0][3]));
+                float t1 = fmaxf(fmaxf(sc[r][1][0], sc[r][1][1]), fmaxf(sc[r][1][2], sc[r][1][3]));
+                const float now = fmaxf(mx[r], row_max(fmaxf(t0, t1)));
+                const float top = now == -INFINITY ? 0.0f : now;
+                ref[r] = top - C::log_lift;
+                if (__ballot(now != mx[r])) {
+                    const float f = exp_of(mx[r] - top);
+                    sum[r] *= f;
+                    for (int c = 0; c < C::NC; c++) acc[r][c] *= f;
+                }
+                mx[r] = now;
+            }
+            // V of keys that no row may see is not to be multiplied, whatever it holds; and where some
+            // rows see a key and others do not, a value that is not finite reaches only those that do
+            bool odd = false;   // (uniform) such values are in this tile
+            if (masked || a.bias) {
+                bool hidden = false;
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+                    for (int x = 0; x < 2; x++)
+                        for (int i = 0; i < 4; i++) hidden |= sc[r][x][i] == -INFINITY;
+                if (__ballot(hidden)) {
+                    bool bad = false;
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int kk = 4 * x + i;
+                            const bool there = key0 + 16 * x + 4 * g + i < held && ok[x];
+                            for (int w = 0; w < C::NU; w++)
+                                for (int y = 0; y < C::WV; y++) {
+                                    unsigned & z = vr[kk][w][y];
+                                    if (!there) z = 0;
+                                    if constexpr (TYPE == kF32) {
+                                        if ((z & 0x7f800000u) == 0x7f800000u) {
+                                            bad = true;
+                                            z = 0;
+                                        }
+                                    } else if constexpr (!Q8) {
+                                        constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
+                                        if ((z & e) == e || (z >> 16 & e) == e) bad = true;
+                                        if ((z & e) == e) z &= 0xffff0000u;
+                                        if ((z >> 16 & e) == e) z &= 0xffffu;
+                                    }
+                                }
+                            if constexpr (Q8)
+                                for (int w = 0; w < C::NU; w++) {
+                                    const int blk = C::column(m, w * C::VW) / 32;
+                                    const float f = scales[wave][1][16 * x + 4 * g + i][blk];
+                                    if (!(fabsf(f) < INFINITY)) {
+                                        bad |= there;
+                                        scales[wave][1][16 * x + 4 * g + i][blk] = 0.0f;
+                                    }
+                                }
+                        }
+                    odd = __ballot(bad) != 0;
+                }
+            }
+            if constexpr (Q8) __builtin_amdgcn_wave_barrier();
+            // weights, as the second product's operand
+            float p[RT][8];
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                float t = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    p[r][i] = exp_of(sc[r][i >> 2][i & 3] - ref[r]);
+                    t += p[r][i];
+                }
+                sum[r] += t;
+            }
+            // O^T += V^T P^T
+            if constexpr (TYPE == kF32) {
+#pragma unroll
+                for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+                    for (int c = 0; c < C::NC; c++)
+#pragma unroll
+                        for (int r = 0; r < RT; r++)
+                            acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(vr[kk][c / C::VW][c % C::VW]), p[r][kk], acc[r][c], 0, 0, 0);
+            } else {
+                u4 pf[RT], pl[C::SPLIT ? RT : 1];
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    unsigned w[4], lo[4];
+                    for (int e = 0; e < 4; e++) {
+                        w[e] = pack2<C::MT>(p[r][2 * e], p[r][2 * e + 1]);
+                        if constexpr (C::SPLIT)
+                            lo[e] = pack2<kBF16>(p[r][2 * e] - bf16_value((unsigned short)w[e]),
+                                                 p[r][2 * e + 1] - bf16_value((unsigned short)(w[e] >> 16)));
+                    }
+                    pf[r] = u4{w[0], w[1], w[2], w[3]};
+                    if constexpr (C::SPLIT) pl[r] = u4{lo[0], lo[1], lo[2], lo[3]};
+                }
+                float vs[8];
+#pragma unroll
+                for (int c = 0; c < C::NC; c++) {
+                    const int w = c / C::VW, y = c % C::VW;
+                    if constexpr (Q8) {
+                        if (y == 0)
+                            for (int kk = 0; kk < 8; kk++)
+                                vs[kk] = scales[wave][1][16 * (kk >> 2) + 4 * g + (kk & 3)][C::column(m, c) / 32];
+                        unsigned hi[4], lo[4];
+                        for (int e = 0; e < 4; e++) {
+                            const float v0 = vs[2 * e] * byte_value(vr[2 * e][w], y);
+                            const float v1 = vs[2 * e + 1] * byte_value(vr[2 * e + 1][w], y);
+                            const unsigned h0 = __float_as_uint(v0) & 0xffff0000u, h1 = __float_as_uint(v1) & 0xffff0000u;
+                            hi[e] = h0 >> 16 | h1;
+                            lo[e] = pack2<kBF16>(v0 - __uint_as_float(h0), v1 - __uint_as_float(h1));
+                        }
+                        const u4 vh = {hi[0], hi[1], hi[2], hi[3]}, vl = {lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+                        for (int r = 0; r < RT; r++) {
+                            acc[r][c] = mfma16<kBF16>(vh, pf[r], acc[r][c]);
+                            acc[r][c] = mfma16<kBF16>(vl, pf[r], acc[r][c]);
+                            if constexpr (C::SPLIT) acc[r][c] = mfma16<kBF16>(vh, pl[r], acc[r][c]);
+                        }
+                    } else {
+                        unsigned f[4];
+                        for (int e = 0; e < 4; e++)   // halves y of keys 2e, 2e+1
+                            f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][w][y >> 1], vr[2 * e][w][y >> 1],
+                                                         y & 1 ? 0x07060302u : 0x05040100u);
+                        const u4 vf = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+                        for (int r = 0; r < RT; r++) acc[r][c] = mfma16<C::MT>(vf, pf[r], acc[r][c]);
+                    }
+                }
+            }
+            if (odd) {
+                for (int kk = 0; kk < 32; kk++) {
+                    if (key0 + kk >= held || !ok[kk >> 4]) continue;
+                    bool o2;
+                    int p2;
+                    const char * row = rows16(a.v, key0 + (kk & 16), o2, p2) + (long long)(kk & 15) * a.v.ld_tok;
+                    const int from = ((kk & 15) >> 2) * 16 + m;
+                    for (int r = 0; r < RT; r++) {
+                        const int e = kk >> 4, i = kk & 3;
+                        const float s0 = i == 0 ? sc[r][e][0] : i == 1 ? sc[r][e][1] : i == 2 ? sc[r][e][2] : sc[r][e][3];
+                        const float sv = __shfl(s0, from);
+                        const float w = exp_of(sv - ref[r]);
+                        for (int c = 0; c < C::NC && sv != -INFINITY; c++)
+                            for (int y = 0; y < 4; y++) {
+                                const int col = C::column(4 * g + y, c);
+                                if (col >= a.dv) continue;
+                                float v;
+                                if constexpr (Q8)
+                                    v = f16_value(*reinterpret_cast<const unsigned short *>(row + col / 32 * 34)) *
+                                        (float)*reinterpret_cast<const signed char *>(row + col / 32 * 34 + 2 + col % 32);
+                                else
+                                    v = value_of<TYPE>(row, col);
+                                if (!(fabsf(v) < INFINITY)) acc[r][c][y] += w * v;
+                            }
+                    }
+                }
+            }
+        }
+
+        // the four waves' parts, and the result
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const float l = row_sum(sum[r]);
+            const int row = 16 * r + m;
+            if (g == 0) {
+                join_m[wave][row] = mx[r];
+                join_l[wave][row] = l;
+            }
+#pragma unroll
+            for (int w = 0; w < C::NU; w++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int y = 0; y < C::VW; y += 4)
+                        *reinterpret_cast<f4 *>(&join[wave][row][C::column(4 * g + i, w * C::VW + y)]) =
+                            f4{acc[r][w * C::VW + y][i], acc[r][w * C::VW + y + 1][i], acc[r][w * C::VW + y + 2][i],
+                               acc[r][w * C::VW + y + 3][i]};
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
+            const int r = e / (D / 4), col = e % (D / 4) * 4;
+            const int row = row0 + r;
+            if (row >= rows || col >= a.dv) continue;
+            float top = join_m[0][r];
+            for (int w = 1; w < 4; w++) top = fmaxf(top, join_m[w][r]);
+            const float zero = top == -INFINITY ? 0.0f : top;
+            f4 x = {0, 0, 0, 0};
+            float l = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                const float f = exp_of(join_m[w][r] - zero) * (1.0f / C::lift);
+                l += f * join_l[w][r];
+                x += f * *reinterpret_cast<const f4 *>(&join[w][r][col]);
+            }
+            const long long out = (long long)(tok0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
+            if (a.splits > 1) {
+                const long long at = (long long)split * a.n_tok * a.H * a.G + out;
+                for (int y = 0; y < 4 && col + y < a.dv; y++) a.part_o[at * a.dv + col + y] = x[y];
+                if (col == 0) {
+                    a.part_ml[2 * at] = top;
+                    a.part_ml[2 * at + 1] = l;
+                }
+            } else {
+                // (a row that sees a cell has a weight of 1 in its sum, or NaN)
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                char * o = a.o + ((long long)(tok0 + row / a.G) * a.o_tok + (long long)(h * a.G + row % a.G) * a.o_head) * C::ES;
+                for (int y = 0; y < 4; y++) {
+                    if (col + y >= a.dv) break;
+                    const float v = x[y] * inv;
+                    if constexpr (TYPE == kF32)
+                        reinterpret_cast<float *>(o)[col + y] = v;
+                    else
+                        reinterpret_cast<unsigned short *>(o)[col + y] = (unsigned short)pack2<QT>(v, v);
+                }
+                if (a.lse && col == 0) a.lse[out] = l == 0.0f ? -INFINITY : top + logf(l);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the key ranges: a wave a row.
+template <int QT>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long n = (long long)a.n_tok * a.H * a.G;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= n) return;
+    const int tok = (int)(row / (a.H * a.G)), head = (int)(row % (a.H * a.G));
+    if (tok < a.cu[0] || tok >= a.cu[a.n_seq]) return;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; s++) top = fmaxf(top, a.part_ml[2 * (s * n + row)]);
+    const float zero = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, x[4] = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; s++) {
+        const float f = exp_of(a.part_ml[2 * (s * n + row)] - zero);
+        l += f * a.part_ml[2 * (s * n + row) + 1];
+        for (int j = 0; j < 4; j++)
+            if (lane + 64 * j < a.dv) x[j] += f * a.part_o[(s * n + row) * a.dv + lane + 64 * j];
+    }
+    for (int j = 0; j < 4; j++) {
+        const int col = lane + 64 * j;
+        if (col >= a.dv) break;
+        const float v = l == 0.0f ? 0.0f : x[j] / l;
+        const long long at = (long long)tok * a.o_tok + (long long)head * a.o_head + col;
+        if constexpr (QT == kF32)
+            reinterpret_cast<float *>(a.o)[at] = v;
+        else
+            reinterpret_cast<unsigned short *>(a.o)[at] = (unsigned short)pack2<QT>(v, v);
+    }
+    if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -INFINITY : top + logf(l);
+}
+
+int head_tile(int dk, int dv) {
+    const int d = dk > dv ? dk : dv;
+    return d <= 64 ? 64 : d <= 128 ? 128 : 256;
+}
+
+bool vec_rows(const kvc_heads & x, int bytes) {
+    return ((reinterpret_cast<uintptr_t>(x.data) | (uintptr_t)(x.ld_tok * bytes) | (uintptr_t)(x.ld_head * bytes)) & 15) == 0;
+}
+
+template <int TYPE, int QT, int D, int RT, bool CAREFUL> bool run_rows(const AttnArgs & a, long long blocks, hipStream_t st) {
+    return launch(k_attn_rows<TYPE, QT, D, RT, CAREFUL>, dim3((unsigned)blocks), dim3(256), st, a);
+}
+template <int TYPE, int QT, int D> bool run_rows(const AttnArgs & a, int rt, bool careful, long long blocks, hipStream_t st) {
+    if constexpr (TYPE != kQ8)
+        if (careful) return run_rows<TYPE, QT, D, 1, true>(a, blocks, st);
+    if constexpr (D < 256)
+        if (rt == 2) return run_rows<TYPE, QT, D, 2, false>(a, blocks, st);
+    return run_rows<TYPE, QT, D, 1, false>(a, blocks, st);
+}
+template <int TYPE, int QT> bool run_rows(const AttnArgs & a, int d, int rt, bool careful, long long blocks, hipStream_t st) {
+    if (d == 64) return run_rows<TYPE, QT, 64>(a, rt, careful, blocks, st);
+    if (d == 128) return run_rows<TYPE, QT, 128>(a, rt, careful, blocks, st);
+    return run_rows<TYPE, QT, 256>(a, rt, careful, blocks, st);
+}
+bool run_rows(const AttnArgs & a, int type, int qt, int rt, bool careful, long long blocks, hipStream_t st) {
+    const int d = head_tile(a.dk, a.dv);
+    if (type == kF32) return run_rows<kF32, kF32>(a, d, rt, careful, blocks, st);
+    if (type == kF16) return run_rows<kF16, kF16>(a, d, rt, careful, blocks, st);
+    if (type == kBF16) return run_rows<kBF16, kBF16>(a, d, rt, careful, blocks, st);
+    if (qt == kF16) return run_rows<kQ8, kF16>(a, d, rt, careful, blocks, st);
+    return run_rows<kQ8, kBF16>(a, d, rt, careful, blocks, st);
+}
+
+// Row tiles a wave holds: two where there are more than 16 rows; at 256 wide heads two do not fit the registers
+int row_tiles(int d, bool careful, long long rows) { return rows > 16 && !careful && d < 256 ? 2 : 1; }
+
+int esize(int type) { return type == kF32 ? 4 : 2; }
+
+// Shape of a cache call's launch.
+struct CacheShape {
+    int rt, tiles, splits;
+    bool careful;
+};
+CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
+    CacheShape s{};
+    const int G = a->n_head / c->n_head_kv, es = esize(a->type);
+    // a cache's pages are 16-byte aligned: its rows are where a head is whole 16-byte pieces
+    s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
+    const long long rows = (long long)a->max_new * G;
+    s.rt = row_tiles(head_tile(c->d_k, c->d_v), s.careful, rows);
+    const long long tiles = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    s.tiles = (int)(tiles < 1 ? 1 : tiles > 65536 ? 65536 : tiles);
+    // key ranges: enough blocks to fill the GPU, each with at least 8 tiles of 32 keys
+    const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles;
+    long long want = (1024 + units - 1) / units, most = a->max_len / 256;
+    want = want < most ? want : most;
+    s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
+    return s;
+}
+
+int check_cache_attn(const kvc_cache * c, const kvc_cache_attn_args * a) {
+    if (int rc = check_cache(c)) return rc;
+    if (!a) return -1;
+    if (a->n_seq < 0 || a->n_tok < 0 || a->n_head <= 0 || a->max_new < 0 || a->max_len < 0 || a->mask_words < 0 ||
+        a->layer < 0 || a->layer >= c->n_layers || a->n_head % c->n_head_kv)
+        return -2;
+    if (c->k_type != c->v_type) return KV_COMPACT_E_UNSUPPORTED;
+    if (c->k_type == kQ8 ? a->type != kF16 && a->type != kBF16 : a->type != c->k_type) return KV_COMPACT_E_UNSUPPORTED;
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace kvc
+
+using namespace kvc;
+
+extern "C" {
+
+size_t kvc_attn_cache_workspace(const kvc_cache * c, const kvc_cache_attn_args * a) {
+    if (check_cache_attn(c, a)) return 0;
+    const CacheShape s = cache_shape(c, a);
+    return s.splits > 1 ? (size_t)s.splits * a->n_tok * a->n_head * (c->d_v + 2) * sizeof(float) : 0;
+}
+
+int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws, size_t ws_bytes, void * stream) {
+    if (int rc = check_cache_attn(c, x)) return rc;
+    if (x->n_seq == 0 || x->n_tok == 0) return 0;
+    if (!x->q.data || !x->o.data || !x->cu) return -1;
+    const int es = esize(x->type);
+    if ((reinterpret_cast<uintptr_t>(x->q.data) | reinterpret_cast<uintptr_t>(x->o.data)) & (es - 1))
+        return KV_COMPACT_E_UNSUPPORTED;
+    const CacheShape s = cache_shape(c, x);
+    const size_t need = kvc_attn_cache_workspace(c, x);
+    if (need && !ws) return -1;
+    if (need > ws_bytes) return KVC_E_SCRATCH;
+    AttnArgs a{};
+    const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);
+    const long long vrow = (long long)kv_quant_row_bytes(c->v_type, c->n_head_kv * c->d_v);
+    const long long cells = (long long)c->n_pages * c->page_size;
+    a.k = RowsAt{static_cast<const char *>(c->K) + x->layer * cells * krow, krow, krow / c->n_head_kv};
+    a.v = RowsAt{static_cast<const char *>(c->V) + x->layer * cells * vrow, vrow, vrow / c->n_head_kv};
+    a.q = static_cast<const char *>(x->q.data);
+    a.o = static_cast<char *>(x->o.data);
+    a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;
+    a.lse = x->lse; a.cu = x->cu; a.seqs = x->seqs; a.len = c->len; a.table = c->table;
+    a.bias = c->bias ? c->bias + x->layer * cells * c->n_head_kv : nullptr;
+    a.mask = reinterpret_cast<const unsigned long long *>(x->mask);
+    a.mask_words = x->mask_words; a.n_seq = x->n_seq; a.n_tok = x->n_tok;
+    a.H = c->n_head_kv; a.G = x->n_head / c->n_head_kv; a.dk = c->d_k; a.dv = c->d_v;
+    a.shift = __builtin_ctz(c->page_size); a.n_pages = c->n_pages; a.max_seqs = c->max_seqs; a.max_pages = c->max_pages;
+    a.splits = s.splits; a.tiles = s.tiles;
+    a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)c->d_k);
+    a.part_o = static_cast<float *>(ws);
+    a.part_ml = a.part_o + (size_t)s.splits * x->n_tok * x->n_head * c->d_v;
+    const long long blocks = (long long)x->n_seq * s.tiles * s.splits * a.H;
+    if (blocks > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    StreamDevice dev(st);
+    if (!dev.ok) return KV_COMPACT_E_DEVICE;
+    if (!run_rows(a, c->k_type, x->type, s.rt, s.careful, blocks, st)) return KV_COMPACT_E_DEVICE;
+    if (s.splits > 1) {
+        const long long joins = ((long long)x->n_tok * x->n_head + 3) / 4;
+        const dim3 grid((unsigned)joins);
+        if (!(x->type == kF32   ? launch(k_attn_join<kF32>, grid, dim3(256), st, a)
+              : x->type == kF16 ? launch(k_attn_join<kF16>, grid, dim3(256), st, a)
+                                : launch(k_attn_join<kBF16>, grid, dim3(256), st, a)))
+            return KV_COMPACT_E_DEVICE;
+    }
+    return 0;
+}
+
+int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
+    if (!x) return -1;
+    if (x->n_seq < 0 || x->n_tok < 0 || x->n_head <= 0 || x->n_head_kv <= 0 || x->d_k <= 0 || x->d_v <= 0 ||
+        x->n_head % x->n_head_kv)
+        return -2;
+    if (x->d_k > 256 || x->d_v > 256 || (x->type != kF32 && x->type != kF16 && x->type != kBF16))
+        return KV_COMPACT_E_UNSUPPORTED;
+    if (x->n_seq == 0 || x->n_tok == 0) return 0;
+    if (!x->q.data || !x->k.data || !x->v.data || !x->o.data || !x->cu) return -1;
+    const int es = esize(x->type), G = x->n_head / x->n_head_kv;
+    if ((reinterpret_cast<uintptr_t>(x->q.data) | reinterpret_cast<uintptr_t>(x->k.data) |
+         reinterpret_cast<uintptr_t>(x->v.data) | reinterpret_cast<uintptr_t>(x->o.data)) & (es - 1))
+        return KV_COMPACT_E_UNSUPPORTED;
+    AttnArgs a{};
+    a.k = RowsAt{static_cast<const char *>(x->k.data), x->k.ld_tok * es, x->k.ld_head * es};
+    a.v = RowsAt{static_cast<const char *>(x->v.data), x->v.ld_tok * es, x->v.ld_head * es};
+    a.q = static_cast<const char *>(x->q.data);
+    a.o = static_cast<char *>(x->o.data);
+    a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;
+    a.lse = x->lse; a.cu = x->cu;
+    a.n_seq = x->n_seq; a.n_tok = x->n_tok; a.H = x->n_head_kv; a.G = G; a.dk = x->d_k; a.dv = x->d_v;
+    a.splits = 1;
+    a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)x->d_k);
+    const bool careful = !vec_rows(x->q, es) || !vec_rows(x->k, es) || !vec_rows(x->v, es) || x->d_k * es % 16 ||
+                         x->d_v * es % 16;
+    const int rt = row_tiles(head_tile(x->d_k, x->d_v), careful, (long long)x->n_tok * G);
+    const long long tiles = ((long long)x->n_tok * G + 16 * rt - 1) / (16 * rt) + x->n_seq;
+    if (tiles * a.H > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    StreamDevice dev(st);
+    if (!dev.ok) return KV_COMPACT_E_DEVICE;
+    return run_rows(a, x->type, x->type, rt, careful, tiles * a.H, st) ? 0 : KV_COMPACT_E_DEVICE;
+}
+
+}  // extern "C"

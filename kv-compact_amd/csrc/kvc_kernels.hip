@@ -11,6 +11,7 @@
 //     column order (first maximal |pivot| wins, pivots below 1e-12 skipped).
 // Parallelism comes from independent outputs (keys, queries, heads, chunks,
 // layers); a sum whose order matters always runs in one thread.
+#include "kvc_codec.h"
 #include "kvc_common.h"
 #include "kvc_kernels.h"
 
@@ -6303,23 +6304,6 @@ __device__ __forceinline__ float f16_to_f32_ref(uint16_t hv) {
     return __uint_as_float(bits);
 }
 
-__device__ __forceinline__ uint16_t f32_to_f16_ref(float val) {
-    const uint32_t f = __float_as_uint(val);
-    const uint32_t sign = (f >> 16) & 0x8000;
-    const int32_t e = (int32_t)((f >> 23) & 0xFF) - 127 + 15;
-    uint32_t m = (f >> 13) & 0x3FF;
-    if (e <= 0) {
-        if (e < -10) return (uint16_t)sign;
-        m = (m | 0x400) >> (1 - e);
-        return (uint16_t)(sign | m);
-    } else if (e >= 31) {
-        return (uint16_t)(sign | 0x7C00);
-    }
-    return (uint16_t)(sign | ((uint32_t)e << 10) | m);
-}
-
-__device__ __forceinline__ float fmax_std(float a, float b) { return (a < b) ? b : a; }
-__device__ __forceinline__ float fmin_std(float a, float b) { return (b < a) ? b : a; }
 __device__ __forceinline__ uint16_t load_u16(const uint8_t * p) { return (uint16_t)(p[0] | ((uint16_t)p[1] << 8)); }
 
 // one work item per 32-element block (per element for F32/F16)

@@ -409,3 +409,70 @@ def state_compact(dll, prefix, blob: bytes, params: StateParams, t_max: int):
     data = ctypes.string_at(out.value, n.value) if n.value else b""
     free(out)
     return 0, data, sel
+
+
+# -- paged cache and its attention (include/kvc-cache.h) ------------------
+CACHE_MAX_REQUESTS, REQ_BAD = 1024, -2
+_ll = ctypes.c_longlong
+_f = ctypes.c_float
+
+
+class KvCache(ctypes.Structure):
+    """kvc_cache: shapes and device arrays of a paged cache."""
+    _fields_ = [(n, _i) for n in ("n_layers", "n_pages", "page_size", "max_seqs", "max_pages", "n_head_kv", "d_k", "d_v",
+                                  "k_type", "v_type")] + [(n, _vp) for n in ("K", "V", "bias", "table", "len", "refs")]
+
+
+class Rows(ctypes.Structure):
+    """kvc_rows: strides in bytes."""
+    _fields_ = [("data", _vp), ("ld_layer", _ll), ("ld_row", _ll)]
+
+
+class Values(ctypes.Structure):
+    """kvc_values: strides in bytes."""
+    _fields_ = [("data", _vp), ("ld_layer", _ll), ("ld_row", _ll), ("ld_head", _ll)]
+
+
+class Betas(ctypes.Structure):
+    """kvc_betas: strides in floats."""
+    _fields_ = [("data", _vp), ("ld_layer", _ll), ("ld_head", _ll)]
+
+
+class Heads(ctypes.Structure):
+    """kvc_heads: strides in elements."""
+    _fields_ = [("data", _vp), ("ld_tok", _ll), ("ld_head", _ll)]
+
+
+class PromptArgs(ctypes.Structure):
+    """kvc_prompt_args."""
+    _fields_ = [("q", Heads), ("k", Heads), ("v", Heads), ("o", Heads), ("lse", _vp), ("cu", _vp)] + [
+        (n, _i) for n in ("type", "n_seq", "n_tok", "n_head", "n_head_kv", "d_k", "d_v")] + [("scale", _f)]
+
+
+class CacheAttnArgs(ctypes.Structure):
+    """kvc_cache_attn_args."""
+    _fields_ = [("q", Heads), ("o", Heads), ("lse", _vp), ("seqs", _vp), ("cu", _vp), ("mask", _vp)] + [
+        (n, _i) for n in ("mask_words", "layer", "type", "n_seq", "n_tok", "n_head", "max_new", "max_len")] + [
+        ("scale", _f)]
+
+
+def bind_cache(dll):
+    """Declare the entry points of include/kvc-cache.h. Device arrays go in as addresses (int or None), structs by
+    reference (a ctypes instance is passed as one)."""
+    P, sz = ctypes.POINTER, ctypes.c_size_t
+    for name, args in {
+            "kvc_cache_reset": [P(KvCache), _vp],
+            "kvc_cache_extend": [P(KvCache), _i, _vp, _vp, _vp, _vp, sz, _vp],
+            "kvc_cache_write": [P(KvCache), _i, _i, _i, _vp, _vp, _i, _i, P(Rows), P(Rows), _vp],
+            "kvc_cache_fork": [P(KvCache), _i, _vp, _vp, _vp, _vp],
+            "kvc_cache_free": [P(KvCache), _i, _vp, _vp],
+            "kvc_cache_compact": [P(KvCache), _i, _vp, _vp, _vp, _i, _vp, _ll, P(Values), P(Betas), _vp, _vp, sz, _vp],
+            "kvc_cache_read": [P(KvCache), _i, _i, _i, _vp, _vp, _vp, _vp],
+            "kvc_attn_prompt": [P(PromptArgs), _vp],
+            "kvc_attn_cache": [P(KvCache), P(CacheAttnArgs), _vp, sz, _vp]}.items():
+        f = getattr(dll, name)
+        f.argtypes, f.restype = args, _i
+    dll.kvc_cache_workspace.argtypes, dll.kvc_cache_workspace.restype = [P(KvCache), _i], sz
+    dll.kvc_attn_cache_workspace.argtypes = [P(KvCache), P(CacheAttnArgs)]
+    dll.kvc_attn_cache_workspace.restype = sz
+    return dll
