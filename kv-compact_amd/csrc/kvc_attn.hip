@@ -127,6 +127,86 @@ template <int N, int BYTES, bool CAREFUL> __device__ __forceinline__ void load_c
     }
 }
 
+// A sequence of the call: its tokens, and the keys it holds.
+struct Sequence {
+    int tok0, n_new;
+    int held;            // keys; 0: nothing can be seen
+    int base;            // keys that every token sees
+    const int * table;   // pages, or nullptr: contiguous tokens
+};
+__device__ __forceinline__ Sequence sequence_of(const AttnArgs & a, int s) {
+    Sequence q;
+    int tok0 = a.cu[s], tok1 = a.cu[s + 1];
+    tok0 = tok0 < 0 ? 0 : tok0;
+    tok1 = tok1 > a.n_tok ? a.n_tok : tok1;
+    q.tok0 = tok0;
+    q.n_new = tok1 - tok0;
+    q.held = q.n_new;
+    q.table = nullptr;
+    if (a.table) {
+        const int seq = a.seqs ? a.seqs[s] : s;
+        const bool there = seq >= 0 && seq < a.max_seqs;
+        q.held = there ? a.len[seq] : 0;
+        if (q.held < q.n_new || q.held > (long long)a.max_pages << a.shift) q.held = 0;
+        q.table = a.table + (long long)(there ? seq : 0) * a.max_pages;
+    }
+    q.base = q.held ? q.held - q.n_new : 0;
+    return q;
+}
+
+// The u-th tile of `rows` rows of all sequences together, those of a sequence
+// from its end (the most keys first). False past the last one.
+__device__ __forceinline__ bool find_tile(const AttnArgs & a, int u, int rows, int lane, int & s, int & tile) {
+    int before = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        int tiles = 0;
+        if (s0 + lane < a.n_seq) {
+            const int n = a.cu[s0 + lane + 1] - a.cu[s0 + lane];
+            tiles = n > 0 ? (int)(((long long)n * a.G + rows - 1) / rows) : 0;
+        }
+        int incl = tiles;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(incl, o);
+            if (lane >= o) incl += y;
+        }
+        const unsigned long long hit = __ballot(before + incl > u);
+        if (hit) {
+            const int w = __ffsll((long long)hit) - 1;
+            s = s0 + w;
+            tile = __shfl(tiles, w) - 1 - (u - before - (__shfl(incl, w) - __shfl(tiles, w)));
+            return true;
+        }
+        before += __shfl(incl, 63);
+    }
+    return false;
+}
+
+// Whether token `tok` of a sequence sees key `key` (its score's bias apart)
+template <bool CELLS>
+__device__ __forceinline__ bool row_sees(const AttnArgs & a, const Sequence & q, int tok, int key, bool check_page) {
+    if (key >= q.held) return false;
+    if constexpr (CELLS) {
+        if (check_page) {
+            const int p = q.table[key >> a.shift];
+            if (p < 0 || p >= a.n_pages) return false;
+        }
+    }
+    const int rel = key - q.base;
+    if (rel < 0) return true;
+    if (CELLS && a.mask)
+        return rel < 64 * a.mask_words && (a.mask[(long long)(q.tok0 + tok) * a.mask_words + (rel >> 6)] >> (rel & 63) & 1);
+    return rel <= tok;
+}
+
+// 16 bytes a lane from memory to LDS, lane after lane from `to` (uniform). The
+// compiler does not count these loads: wait_lds_loads() does.
+__device__ __forceinline__ void load_lds16(const char * from, char * to) {
+    const unsigned at = __builtin_amdgcn_readfirstlane(
+        (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+}
+__device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
 typedef u2 u2_any __attribute__((aligned(2)));
 typedef unsigned u1_any __attribute__((aligned(2)));
 
@@ -199,49 +279,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
         s = u / a.tiles;
         tile_step = a.tiles;
     } else {
-        // flat: the u-th row tile of all sequences together, longest keys first
-        // (the order inside a sequence is turned round)
-        int before = 0, found = -1;
-        for (int s0 = 0; s0 < a.n_seq && found < 0; s0 += 64) {
-            int tiles = 0;
-            if (s0 + lane < a.n_seq) {
-                const int n = a.cu[s0 + lane + 1] - a.cu[s0 + lane];
-                tiles = n > 0 ? (int)(((long long)n * a.G + ROWS - 1) / ROWS) : 0;
-            }
-            int incl = tiles;
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(incl, o);
-                if (lane >= o) incl += y;
-            }
-            const unsigned long long hit = __ballot(before + incl > u);
-            if (hit) {
-                const int w = __ffsll((long long)hit) - 1;
-                found = s0 + w;
-                tile = __shfl(tiles, w) - 1 - (u - before - (__shfl(incl, w) - __shfl(tiles, w)));
-            }
-            before += __shfl(incl, 63);
-        }
-        if (found < 0) return;
-        s = found;
+        if (!find_tile(a, u, ROWS, lane, s, tile)) return;
         tile_step = 1 << 30;
     }
     s = __builtin_amdgcn_readfirstlane(s);
     tile = __builtin_amdgcn_readfirstlane(tile);
-    int tok0 = a.cu[s], tok1 = a.cu[s + 1];
-    tok0 = tok0 < 0 ? 0 : tok0;
-    tok1 = tok1 > a.n_tok ? a.n_tok : tok1;
-    const int n_new = tok1 - tok0;
-    if (n_new <= 0) return;
-    const int seq = a.table ? (a.seqs ? a.seqs[s] : s) : 0;
-    int held = n_new;   // keys of the sequence
-    const int * table = nullptr;
-    if (a.table) {
-        const bool there = seq >= 0 && seq < a.max_seqs;
-        held = there ? a.len[seq] : 0;
-        if (held < n_new || held > (long long)a.max_pages << a.shift) held = 0;
-        table = a.table + (long long)(there ? seq : 0) * a.max_pages;
-    }
-    const int base = held ? held - n_new : 0;   // keys that every token sees
+    const Sequence sq = sequence_of(a, s);
+    if (sq.n_new <= 0) return;
+    const int tok0 = sq.tok0, n_new = sq.n_new, held = sq.held, base = sq.base;
+    const int * table = sq.table;
     const int rows = n_new * a.G;
     const int page_mask = a.table ? (1 << a.shift) - 1 : 0;
 
@@ -652,6 +698,347 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: 128 of them a block, 32 a wave, over tiles of BK keys that all
+// four waves read from LDS.
+//
+// Fragments (32x32x16, lane l, n = l % 32, h = l / 32): an operand's lane holds
+// row n and elements 8h .. 8h+7 of the summed axis; a result's lane column n
+// and rows 8x + 4h + y (register 4x + y). As in k_attn_rows the scores of one
+// row of the caller's are one lane's (two lanes', h = 0 and 1), and go into the
+// second product from the registers they were made in: element j of step s is
+// key 16s + 4h + j, or 16s + 8 + 4h + j - 4.
+//
+// K and V reach LDS by direct loads of 16 bytes a lane (no registers), a tile
+// ahead, two buffers. They stand row by row with their 16-byte pieces
+// exchanged, K's by key % 8 or 16 so that the 32 rows of a fragment read
+// different banks, V's in pairs by key % 8 so that the four rows that
+// ds_read_b64_tr_b16 turns round do: it gives a lane four keys of one column,
+// half a fragment of V^T. Pieces past the head's width and rows past the last
+// key are read from a piece of zeros.
+__device__ const u4 zero_piece = {0, 0, 0, 0};
+
+typedef float f16x __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+template <int TYPE> __device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
+    if constexpr (TYPE == kF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float pair_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
+
+template <int TYPE, int D, bool CELLS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a) {
+    constexpr int BK = D == 256 ? 32 : 64, SUB = BK / 32;   // keys of a tile, in parts of 32
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8;     // steps of a score, column tiles, pieces of a row
+    constexpr int NL = BK * CH / 256;                       // direct loads of a wave and tile, K or V
+    constexpr int ROWB = 2 * D, KX = CH < 16 ? CH - 1 : 15, VX = CH < 16 ? CH / 2 - 1 : 7;
+    constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f, log2_lift = TYPE == kF16 ? 10.0f : 0.0f;
+    __shared__ __align__(16) char lds[2][2][BK * ROWB];     // [buffer][K, V]
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hf = lane >> 5;
+
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    int split = 0;
+    if constexpr (CELLS) {
+        split = u % a.splits;
+        u /= a.splits;
+    }
+    int s, tile, tile_step;
+    if (CELLS && a.tiles) {
+        tile = u % a.tiles;
+        s = u / a.tiles;
+        tile_step = a.tiles;
+    } else {
+        if (!find_tile(a, u, 128, lane, s, tile)) return;
+        tile_step = 1 << 30;
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    Sequence q = sequence_of(a, s);
+    if (q.n_new <= 0) return;
+    const int rows = q.n_new * a.G;
+    const int page_mask = CELLS ? (1 << a.shift) - 1 : 0;
+    const bool flip = a.scale < 0.0f;   // (the maximum is taken of products by a positive number)
+    const float scale = fabsf(a.scale);
+    const float c = (CELLS && a.bias ? 1.0f : scale) * kLog2e;
+
+    for (; (long long)tile * 128 < rows; tile += tile_step) {
+        const int row0 = tile * 128, wrow0 = row0 + 32 * wave;
+        const int last_tok = (row0 + 127) / a.G < q.n_new ? (row0 + 127) / a.G : q.n_new - 1;
+        const int end_all = q.held == 0 ? 0 : (CELLS && a.mask ? q.held : q.base + last_tok + 1);
+        // keys before it are seen by every row of this wave
+        const int clear = CELLS && a.mask ? q.base : q.base + (wrow0 < rows ? wrow0 / a.G + 1 : last_tok + 1);
+        const int n_tiles = (end_all + BK - 1) / BK;
+        int t_lo = 0, t_hi = n_tiles;
+        if constexpr (CELLS) {
+            const int per = (n_tiles + a.splits - 1) / a.splits;
+            t_lo = split * per;
+            t_hi = t_lo + per < n_tiles ? t_lo + per : n_tiles;
+        }
+        const int row = wrow0 + n;
+        const bool on = row < rows;
+        const int tok = on ? row / a.G : 0, head = on ? row % a.G : 0;
+        u4 qf[KS];
+        {
+            const char * p = a.q + 2 * ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head);
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                qf[j] = 16 * j + 8 * hf < a.dk ? *reinterpret_cast<const u4 *>(p + 32 * j + 16 * hf) : u4{0, 0, 0, 0};
+                if (flip) qf[j] ^= 0x80008000u;
+            }
+        }
+
+        // where a lane's pieces of a tile come from
+        int piece_key[NL], k_col[NL], v_col[NL];
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int x = (i * 4 + wave) * 64 + lane, key = x / CH, at = x % CH;
+            piece_key[i] = key;
+            k_col[i] = at ^ (key & KX);
+            v_col[i] = at ^ ((key & VX) << 1);
+        }
+        int page[CELLS ? NL : 1];
+        auto find_pages = [&](int t) {
+            if constexpr (CELLS)
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    const int key = t * BK + piece_key[i];
+                    page[i] = t < t_hi && key < q.held ? q.table[key >> a.shift] : -1;
+                }
+        };
+        auto fill = [&](int t, int buf) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int key = t * BK + piece_key[i];
+                long long at;
+                bool ok = key < end_all;
+                if constexpr (CELLS) {
+                    ok = ok && page[i] >= 0 && page[i] < a.n_pages;
+                    at = ((long long)page[i] << a.shift) + (key & page_mask);
+                } else {
+                    at = q.tok0 + key;
+                }
+                const char * z = reinterpret_cast<const char *>(&zero_piece);
+                const char * k = ok && 8 * k_col[i] < a.dk ? a.k.base + at * a.k.ld_tok + h * a.k.ld_head + 16 * k_col[i] : z;
+                const char * v = ok && 8 * v_col[i] < a.dv ? a.v.base + at * a.v.ld_tok + h * a.v.ld_head + 16 * v_col[i] : z;
+                load_lds16(k, &lds[buf][0][(i * 4 + wave) * 1024]);
+                load_lds16(v, &lds[buf][1][(i * 4 + wave) * 1024]);
+            }
+        };
+
+        f16x acc[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+        float mx = -INFINITY, sum = 0.0f;   // (mx: in units of s, kept up to 2^5 below the true maximum)
+        float mc = 0.0f;                    // mx, or 0 while nothing is seen
+
+        find_pages(t_lo);
+        if (t_lo < t_hi) fill(t_lo, 0);
+        find_pages(t_lo + 1);
+        for (int t = t_lo; t < t_hi; t++) {
+            const int buf = (t - t_lo) & 1;
+            wait_lds_loads();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (t + 1 < t_hi) fill(t + 1, buf ^ 1);
+            find_pages(t + 2);
+            const char * kt = lds[buf][0];
+            const char * vt = lds[buf][1];
+            const int key0 = t * BK;
+
+            f16x sc[SUB];
+#pragma unroll
+            for (int x = 0; x < SUB; x++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) sc[x][i] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    const u4 kf = *reinterpret_cast<const u4 *>(kt + (32 * x + n) * ROWB + (((2 * j + hf) ^ (n & KX)) << 4));
+                    sc[x] = mfma32<TYPE>(kf, qf[j], sc[x]);
+                }
+            }
+            bool hidden = false;   // (uniform) a key of the tile that some row does not see
+            if (CELLS && a.bias) {
+#pragma unroll
+                for (int x = 0; x < SUB; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const int key = key0 + 32 * x + 8 * y + 4 * hf;   // four cells of one page
+                        const int p = key < q.held ? q.table[key >> a.shift] : -1;
+                        const bool ok = p >= 0 && p < a.n_pages;
+                        const float * b = a.bias + (((long long)(ok ? p : 0) * a.H + h) << a.shift) + (key & page_mask);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float v = b[i] == -INFINITY ? -INFINITY : sc[x][4 * y + i] * scale + b[i];
+                            sc[x][4 * y + i] = v;
+                            hidden |= v == -INFINITY;
+                        }
+                    }
+            }
+            bool bad_page = false;
+            if constexpr (CELLS) {
+                // (a page number that is none of the cache's hides its cells)
+#pragma unroll
+                for (int x = 0; x < BK / 16; x++) {
+                    const int key = key0 + 16 * x;
+                    const int p = key < q.held ? q.table[key >> a.shift] : 0;
+                    bad_page |= p < 0 || p >= a.n_pages;
+                }
+            }
+            const bool masked = key0 + BK > clear || bad_page;
+            if (masked) {
+#pragma unroll
+                for (int x = 0; x < SUB; x++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int key = key0 + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3);
+                        if (!row_sees<CELLS>(a, q, tok, key, bad_page)) sc[x][i] = -INFINITY;
+                    }
+                hidden = true;
+            }
+            hidden = __ballot(hidden) != 0;
+
+            float top = sc[0][0];
+#pragma unroll
+            for (int x = 0; x < SUB; x++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, sc[x][i]);
+            top = pair_max(top);
+            // weights up to 2^5 are left to grow before the sums are scaled
+            if (__ballot((top - mx) * c > 5.0f)) {
+                const float now = fmaxf(mx, top);
+                const float use = now == -INFINITY ? 0.0f : now;
+                const float f = __builtin_amdgcn_exp2f((mx - use) * c);
+                mx = now;
+                mc = use;
+                sum *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[d][i] *= f;
+            }
+            // V of the tile's parts, weights of the lane's row
+            bool odd = false;
+            float p[SUB][16];
+            float part = 0.0f;
+            const float off = log2_lift - mc * c;
+#pragma unroll
+            for (int x = 0; x < SUB; x++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    // (with a bias the difference first: a score may be the type's lowest value)
+                    p[x][i] = CELLS && a.bias ? __builtin_amdgcn_exp2f((sc[x][i] - mc) * c + log2_lift)
+                                              : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], c, off));
+                    part += p[x][i];
+                }
+            sum += part;
+#pragma unroll
+            for (int x = 0; x < SUB; x++)
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    u4 pf;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pf[e] = pack2<TYPE>(p[x][8 * st + 2 * e], p[x][8 * st + 2 * e + 1]);
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        u2 half[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int r = (lane & 15) >> 2;   // key 4 hf + r of the eight
+                            const int col = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                            const char * at = vt + (32 * x + 16 * st + 8 * e + 4 * hf + r) * ROWB +
+                                              ((col ^ (((4 * hf + r) & VX) << 1)) << 4) + ((lane & 1) << 3);
+                            half[e] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                 (__attribute__((address_space(3))) s4 *)at));
+                        }
+                        u4 vf = {half[0].x, half[0].y, half[1].x, half[1].y};
+                        if (hidden) {
+                            constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                const bool lo = (vf[y] & e) == e, hi = (vf[y] >> 16 & e) == e;
+                                odd |= lo || hi;
+                                vf[y] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                            }
+                        }
+                        acc[d] = mfma32<TYPE>(vf, pf, acc[d]);
+                    }
+                }
+            if (hidden && __ballot(odd)) {
+                // values that are not finite reach only the rows that see their key
+                for (int kk = 0; kk < BK; kk++) {
+                    const int x = kk >> 5, reg = (kk >> 3 & 3) * 4 + (kk & 3);
+                    float w = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < SUB; y++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (y == x && i == reg) w = p[y][i];
+                    w = __shfl(w, n + 32 * (kk >> 2 & 1));
+                    const int key = key0 + kk;
+                    bool see = key < end_all && row_sees<CELLS>(a, q, tok, key, bad_page);
+                    if (CELLS && a.bias && see)
+                        see = a.bias[(((long long)q.table[key >> a.shift] * a.H + h) << a.shift) + (key & page_mask)] != -INFINITY;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int col = 32 * d + 8 * (i >> 2) + 4 * hf + (i & 3);
+                            const float v = value_of<TYPE>(vt + kk * ROWB + (((col >> 3) ^ ((kk & VX) << 1)) << 4), col & 7);
+                            if (see && !(fabsf(v) < INFINITY)) acc[d][i] += w * v;
+                        }
+                }
+            }
+        }
+        sum += __shfl_xor(sum, 32);
+        sum *= 1.0f / lift;
+        const long long out = (long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head;
+        if (CELLS && a.splits > 1) {
+            const long long at = (long long)split * a.n_tok * a.H * a.G + out;
+            if (on) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const int col = 32 * d + 8 * y + 4 * hf;
+                        if (col < a.dv)
+                            *reinterpret_cast<f4 *>(a.part_o + at * a.dv + col) =
+                                f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]} * (1.0f / lift);
+                    }
+                if (hf == 0) {
+                    a.part_ml[2 * at] = CELLS && a.bias ? mx : mx * scale;
+                    a.part_ml[2 * at + 1] = sum;
+                }
+            }
+        } else if (on) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * lift);
+            char * o = a.o + 2 * ((long long)(q.tok0 + tok) * a.o_tok + (long long)(h * a.G + head) * a.o_head);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int col = 32 * d + 8 * y + 4 * hf;
+                    if (col >= a.dv) continue;
+                    const u2 v = {pack2<TYPE>(acc[d][4 * y] * inv, acc[d][4 * y + 1] * inv),
+                                  pack2<TYPE>(acc[d][4 * y + 2] * inv, acc[d][4 * y + 3] * inv)};
+                    *reinterpret_cast<u2 *>(o + 2 * col) = v;
+                }
+            if (a.lse && hf == 0)
+                a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS && a.bias ? mx : mx * scale) + logf(sum);
+        }
+        __syncthreads();
+    }
+}
+
 // Joins the key ranges: a wave a row.
 template <int QT>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
@@ -720,12 +1107,23 @@ bool run_rows(const AttnArgs & a, int type, int qt, int rt, bool careful, long l
 // Row tiles a wave holds: two where there are more than 16 rows; at 256 wide heads two do not fit the registers
 int row_tiles(int d, bool careful, long long rows) { return rows > 16 && !careful && d < 256 ? 2 : 1; }
 
+template <int TYPE, bool CELLS> bool run_tiles(const AttnArgs & a, int d, long long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks);
+    if (d == 64) return launch(k_attn_tiles<TYPE, 64, CELLS>, grid, dim3(256), st, a);
+    if (d == 128) return launch(k_attn_tiles<TYPE, 128, CELLS>, grid, dim3(256), st, a);
+    return launch(k_attn_tiles<TYPE, 256, CELLS>, grid, dim3(256), st, a);
+}
+template <bool CELLS> bool run_tiles(const AttnArgs & a, int type, long long blocks, hipStream_t st) {
+    const int d = head_tile(a.dk, a.dv);
+    return type == kF16 ? run_tiles<kF16, CELLS>(a, d, blocks, st) : run_tiles<kBF16, CELLS>(a, d, blocks, st);
+}
+
 int esize(int type) { return type == kF32 ? 4 : 2; }
 
 // Shape of a cache call's launch.
 struct CacheShape {
     int rt, tiles, splits;
-    bool careful;
+    bool careful, whole;   // whole: k_attn_tiles
 };
 CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     CacheShape s{};
@@ -734,7 +1132,9 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
     const long long rows = (long long)a->max_new * G;
     s.rt = row_tiles(head_tile(c->d_k, c->d_v), s.careful, rows);
-    const long long tiles = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    s.whole = rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es);
+    const int block_rows = s.whole ? 128 : 16 * s.rt;
+    const long long tiles = (rows + block_rows - 1) / block_rows;
     s.tiles = (int)(tiles < 1 ? 1 : tiles > 65536 ? 65536 : tiles);
     // key ranges: enough blocks to fill the GPU, each with at least 8 tiles of 32 keys
     const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles;
@@ -804,7 +1204,8 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    if (!run_rows(a, c->k_type, x->type, s.rt, s.careful, blocks, st)) return KV_COMPACT_E_DEVICE;
+    if (!(s.whole ? run_tiles<true>(a, x->type, blocks, st) : run_rows(a, c->k_type, x->type, s.rt, s.careful, blocks, st)))
+        return KV_COMPACT_E_DEVICE;
     if (s.splits > 1) {
         const long long joins = ((long long)x->n_tok * x->n_head + 3) / 4;
         const dim3 grid((unsigned)joins);
@@ -841,13 +1242,18 @@ int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
     a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)x->d_k);
     const bool careful = !vec_rows(x->q, es) || !vec_rows(x->k, es) || !vec_rows(x->v, es) || x->d_k * es % 16 ||
                          x->d_v * es % 16;
+    const bool whole = x->type != kF32 && !careful && vec_rows(x->o, es);
     const int rt = row_tiles(head_tile(x->d_k, x->d_v), careful, (long long)x->n_tok * G);
-    const long long tiles = ((long long)x->n_tok * G + 16 * rt - 1) / (16 * rt) + x->n_seq;
+    const int block_rows = whole ? 128 : 16 * rt;
+    const long long tiles = ((long long)x->n_tok * G + block_rows - 1) / block_rows + x->n_seq;
     if (tiles * a.H > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    return run_rows(a, x->type, x->type, rt, careful, tiles * a.H, st) ? 0 : KV_COMPACT_E_DEVICE;
+    return (whole ? run_tiles<false>(a, x->type, tiles * a.H, st)
+                  : run_rows(a, x->type, x->type, rt, careful, tiles * a.H, st))
+               ? 0
+               : KV_COMPACT_E_DEVICE;
 }
 
 }  // extern "C"
