@@ -53,7 +53,7 @@ extern "C" {
  * k_row bytes is kv_quant_row_bytes(k_type, n_head_kv * d_k), likewise V.
  * Types: F32, F16, BF16, Q8_0 (d_k and d_v multiples of 32).
  * page_size: a power of two from 16 to 1024. n_pages <= 2^20. d_k, d_v <= 256.
- * K and V 16-byte aligned (hipMalloc's are).
+ * K, V and bias 16-byte aligned, the workspaces too (hipMalloc's are).
  * New pages are the lowest free ones, in request order, so that equal calls
  * on equal caches give equal tables. */
 typedef struct kvc_cache {

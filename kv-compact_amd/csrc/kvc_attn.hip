@@ -17,6 +17,10 @@
 #include <math.h>
 #include <stdint.h>
 
+// (the library is built with contraction off for the kernels that keep the
+// reference's rounding; a multiply-add here may be one rounding)
+#pragma clang fp contract(fast)
+
 namespace kvc {
 
 namespace {
@@ -127,6 +131,11 @@ template <int N, int BYTES, bool CAREFUL> __device__ __forceinline__ void load_c
     }
 }
 
+// a table entry at a uniform address, by a scalar load (nothing writes tables while attention runs)
+__device__ __forceinline__ int uniform_load(const int * p) {
+    return *(const __attribute__((address_space(4))) int *)p;
+}
+
 // A sequence of the call: its tokens, and the keys it holds.
 struct Sequence {
     int tok0, n_new;
@@ -136,7 +145,7 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence_of(const AttnArgs & a, int s) {
     Sequence q;
-    int tok0 = a.cu[s], tok1 = a.cu[s + 1];
+    int tok0 = uniform_load(a.cu + s), tok1 = uniform_load(a.cu + s + 1);
     tok0 = tok0 < 0 ? 0 : tok0;
     tok1 = tok1 > a.n_tok ? a.n_tok : tok1;
     q.tok0 = tok0;
@@ -144,9 +153,9 @@ __device__ __forceinline__ Sequence sequence_of(const AttnArgs & a, int s) {
     q.held = q.n_new;
     q.table = nullptr;
     if (a.table) {
-        const int seq = a.seqs ? a.seqs[s] : s;
+        const int seq = a.seqs ? uniform_load(a.seqs + s) : s;
         const bool there = seq >= 0 && seq < a.max_seqs;
-        q.held = there ? a.len[seq] : 0;
+        q.held = there ? uniform_load(a.len + seq) : 0;
         if (q.held < q.n_new || q.held > (long long)a.max_pages << a.shift) q.held = 0;
         q.table = a.table + (long long)(there ? seq : 0) * a.max_pages;
     }
@@ -181,21 +190,20 @@ __device__ __forceinline__ bool find_tile(const AttnArgs & a, int u, int rows, i
     return false;
 }
 
-// Whether token `tok` of a sequence sees key `key` (its score's bias apart)
-template <bool CELLS>
-__device__ __forceinline__ bool row_sees(const AttnArgs & a, const Sequence & q, int tok, int key, bool check_page) {
-    if (key >= q.held) return false;
-    if constexpr (CELLS) {
-        if (check_page) {
-            const int p = q.table[key >> a.shift];
-            if (p < 0 || p >= a.n_pages) return false;
-        }
-    }
-    const int rel = key - q.base;
-    if (rel < 0) return true;
-    if (CELLS && a.mask)
-        return rel < 64 * a.mask_words && (a.mask[(long long)(q.tok0 + tok) * a.mask_words + (rel >> 6)] >> (rel & 63) & 1);
-    return rel <= tok;
+// Bit i: token `tok` of a sequence sees key key0 + i (its score's bias and its page apart)
+__device__ __forceinline__ unsigned seen32(const AttnArgs & a, const Sequence & q, int tok, int key0) {
+    auto first = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };
+    const unsigned all = first(q.held - key0);
+    const int rel = key0 - q.base;
+    if (rel <= -32) return all;
+    if (!a.mask) return all & first(tok - rel + 1);
+    const unsigned long long * w = a.mask + (long long)(q.tok0 + tok) * a.mask_words;
+    auto word = [&](int i) { return i < a.mask_words ? w[i] : 0ull; };
+    if (rel < 0) return all & ((unsigned)(word(0) << -rel) | first(-rel));
+    const int i = rel >> 6, sh = rel & 63;
+    unsigned long long bits = word(i) >> sh;
+    if (sh > 32) bits |= word(i + 1) << (64 - sh);
+    return all & (unsigned)bits;
 }
 
 // 16 bytes a lane from memory to LDS, lane after lane from `to` (uniform). The
@@ -205,10 +213,25 @@ __device__ __forceinline__ void load_lds16(const char * from, char * to) {
         (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
 }
+// (4 bytes)
+__device__ __forceinline__ void load_lds4(const char * from, char * to) {
+    const unsigned at = __builtin_amdgcn_readfirstlane(
+        (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
+}
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 typedef u2 u2_any __attribute__((aligned(2)));
 typedef unsigned u1_any __attribute__((aligned(2)));
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+// Two signed bytes, chosen by `pick` (as v_perm: 0-3 of b, 4-7 of a; the other
+// halves' bytes 0x0c), as exact fp16: byte + 128 is the low byte of 1024 + it.
+__device__ __forceinline__ unsigned code_pair(unsigned a, unsigned b, unsigned pick) {
+    const unsigned w = __builtin_amdgcn_perm(a, b, pick) ^ 0x64806480u;
+    const h2 x = __builtin_bit_cast(h2, w) - h2{(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(unsigned, x);
+}
 
 // signed byte i of a register pair, as fp32
 __device__ __forceinline__ float byte_value(const unsigned * w, int i) {
@@ -228,9 +251,12 @@ __device__ __forceinline__ float byte_value(const unsigned * w, int i) {
 // VW neighbouring columns of those keys, which makes VW fragments after a
 // 2 x 2 exchange of halves (v_perm), without LDS.
 // F32 sums 4 elements an instruction (16x16x4), one of them a lane's.
-// Q8_0: K's codes are exact in bf16, a block of 32 is one instruction, and its
-// scale multiplies the block's sums in fp32; V is the fp32 product of scale
-// and code as a sum of two bf16.
+// Q8_0: products in fp16, which holds the codes exactly. A block of K is one
+// instruction, and its scale multiplies the block's sums in fp32; bf16 queries
+// become fp16 times a power of two of their row. V is scale times code in fp16
+// (for fp16 results with the remainder as a second term), which is a half step
+// off at most while the scales are between 2^-14 and 2^8; a tile with others
+// takes the product in fp32 as a sum of two bf16, and the weights too.
 template <int TYPE, int QT, int D, int RT, bool CAREFUL>
 struct RowKernel {
     static constexpr int ES = TYPE == kF32 ? 4 : 2;          // bytes of a q element
@@ -244,12 +270,11 @@ struct RowKernel {
     static constexpr int WV = Q8 ? (VW + 3) / 4 : VW * ES / 4;    // registers of a V load
     static constexpr int WK = Q8 ? 2 : 4;
     static constexpr int NKL = Q8 ? NB : NK;
-    static constexpr int MT = Q8 ? kBF16 : TYPE;             // type on the matrix units
-    static constexpr bool SPLIT = Q8 && QT == kF16;          // q and p as two bf16 each
+    static constexpr int MT = Q8 ? kF16 : TYPE;              // type on the matrix units
 
     // fp16 weights are 2^10 times exp(s - m): those under 2^-24 of the largest, not 2^-14, lose bits
-    static constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f;
-    static constexpr float log_lift = TYPE == kF16 ? 6.93147180559945309417f : 0.0f;
+    static constexpr float lift = MT == kF16 ? 0x1p10f : 1.0f;
+    static constexpr float log_lift = MT == kF16 ? 6.93147180559945309417f : 0.0f;
 
     // column of fragment c's lane m
     static __device__ __forceinline__ int column(int m, int c) { return (c / VW) * 16 * VW + VW * m + c % VW; }
@@ -262,7 +287,9 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) float join[4][ROWS][LD];
     __shared__ float join_m[4][ROWS], join_l[4][ROWS];
-    __shared__ __align__(16) float scales[Q8 ? 4 : 1][2][32][Q8 ? C::NB : 1];
+    // Q8_0 scales of a wave's tile, by block and key
+    __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
+    __shared__ __align__(16) _Float16 v_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, g = lane >> 4;
@@ -306,7 +333,8 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
         // rows of this lane
         int tok[RT], head[RT];
         bool on[RT];
-        u4 q[RT][C::NK], q_lo[C::SPLIT ? RT : 1][C::SPLIT ? C::NK : 1];
+        u4 q[RT][C::NK];
+        float row_up[Q8 ? RT : 1], row_more[Q8 ? RT : 1];   // what the row's elements were multiplied by, in two parts
         for (int r = 0; r < RT; r++) {
             const int row = row0 + 16 * r + m;
             on[r] = row < rows;
@@ -316,20 +344,28 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             for (int j = 0; j < C::NK; j++) {
                 unsigned w[4];
                 load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, w);
-                if constexpr (C::SPLIT) {
-                    // an fp16 value is the sum of two bf16
-                    unsigned hi[4], lo[4];
+                q[r][j] = u4{w[0], w[1], w[2], w[3]};
+            }
+            if constexpr (Q8 && QT == kBF16) {
+                // the largest of the row to 2^14 (eight bits of it: exact; others from 2^-28 of it on)
+                unsigned top = 0;
+                for (int j = 0; j < C::NK; j++)
                     for (int i = 0; i < 4; i++) {
-                        const float x = f16_value((unsigned short)w[i]), y = f16_value((unsigned short)(w[i] >> 16));
-                        const unsigned xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
-                        hi[i] = xh >> 16 | yh;
-                        lo[i] = pack2<kBF16>(x - __uint_as_float(xh), y - __uint_as_float(yh));
+                        const unsigned lo = q[r][j][i] & 0x7fffu, hi = q[r][j][i] >> 16 & 0x7fffu;
+                        top = lo > top ? lo : top;
+                        top = hi > top ? hi : top;
                     }
-                    q[r][j] = u4{hi[0], hi[1], hi[2], hi[3]};
-                    q_lo[r][j] = u4{lo[0], lo[1], lo[2], lo[3]};
-                } else {
-                    q[r][j] = u4{w[0], w[1], w[2], w[3]};
-                }
+                top = max(top, (unsigned)__shfl_xor((int)top, 16));
+                top = max(top, (unsigned)__shfl_xor((int)top, 32));
+                int e = (int)(top >> 7) - 127;               // of the largest
+                if (top == 0 || top >= 0x7f80u) e = 14;      // nothing, or not finite: as it is
+                const float up = __builtin_ldexpf(1.0f, (14 - e) / 2), more = __builtin_ldexpf(1.0f, 14 - e - (14 - e) / 2);
+                for (int j = 0; j < C::NK; j++)
+                    for (int i = 0; i < 4; i++)
+                        q[r][j][i] = pack2<kF16>(bf16_value((unsigned short)q[r][j][i]) * up * more,
+                                                 bf16_value((unsigned short)(q[r][j][i] >> 16)) * up * more);
+                row_up[r] = 1.0f / up;
+                row_more[r] = 1.0f / more;
             }
         }
         f4 acc[RT][C::NC];
@@ -340,29 +376,30 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             for (int c = 0; c < C::NC; c++) acc[r][c] = f4{0, 0, 0, 0};
         }
 
-        // address of the first row of 16 keys, and whether they are on a good page
-        auto rows16 = [&](const RowsAt & x, int key, bool & ok, int & page) -> const char * {
-            ok = true;
-            page = 0;
-            if (!table) return x.base + (long long)(tok0 + key) * x.ld_tok + h * x.ld_head;
-            const int col = key >> a.shift;
-            page = key < held ? table[col] : -1;
-            ok = page >= 0 && page < a.n_pages;
-            if (!ok) page = 0;
-            return x.base + (((long long)page << a.shift) + (key & page_mask)) * x.ld_tok + h * x.ld_head;
+        // pages of the two 16-cell groups of a tile (-1 past the end), and a group's first row
+        auto pages_of = [&](int t, int (&pg)[2]) {
+            for (int x = 0; x < 2; x++) {
+                const int key = (t << 5) + 16 * x;
+                pg[x] = !table ? 0 : t < t_hi && key < held ? uniform_load(table + (key >> a.shift)) : -1;
+            }
         };
+        auto good = [&](int pg) { return !table || (pg >= 0 && pg < a.n_pages); };
+        auto rows16 = [&](const RowsAt & x, int key, int pg) -> const char * {
+            if (!table) return x.base + (long long)(tok0 + key) * x.ld_tok + h * x.ld_head;
+            return x.base + (((long long)(good(pg) ? pg : 0) << a.shift) + (key & page_mask)) * x.ld_tok + h * x.ld_head;
+        };
+        // (contiguous rows end with the sequence: those past it repeat the last)
+        auto row_of = [&](int key) { return table ? key & 15 : (key < held ? key : held - 1) - (key & ~15); };
 
         unsigned kr[2][C::NKL][C::WK];
         unsigned vr[8][C::NU][C::WV];
-        for (int t = t_lo + wave; t < t_hi; t += 4) {
-            const int key0 = t << 5;
-            bool ok[2];
-            int page[2];
-            // (contiguous rows end with the sequence: those past it repeat the last)
-            auto row_of = [&](int key) { return table ? key & 15 : (key < held ? key : held - 1) - (key & ~15); };
+        unsigned short ks[Q8 ? C::NB / 2 : 1], vsc[Q8 ? C::NB / 2 : 1];   // scales, a lane pair per key
+        f4 bias[2];
+        auto load_k = [&](int t, const int (&pg)[2]) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                const char * p = rows16(a.k, key0 + 16 * x, ok[x], page[x]) + (long long)row_of(key0 + 16 * x + m) * a.k.ld_tok;
+                const int key = (t << 5) + 16 * x;
+                const char * p = rows16(a.k, key, pg[x]) + (long long)row_of(key + m) * a.k.ld_tok;
 #pragma unroll
                 for (int j = 0; j < C::NKL; j++) {
                     if constexpr (Q8) {
@@ -371,15 +408,31 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                         load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
                     }
                 }
+                // (four cells of one page)
+                if (a.bias)
+                    bias[x] = *reinterpret_cast<const f4 *>(
+                        a.bias + (((long long)(good(pg[x]) ? pg[x] : 0) * a.H + h) << a.shift) + ((key + 4 * g) & page_mask));
             }
+            if constexpr (Q8) {
+                const int key = lane >> 1, half = lane & 1;
+                const char * pk = rows16(a.k, (t << 5) + (key & 16), pg[key >> 4]) + (long long)(key & 15) * a.k.ld_tok;
+                const char * pv = rows16(a.v, (t << 5) + (key & 16), pg[key >> 4]) + (long long)(key & 15) * a.v.ld_tok;
+#pragma unroll
+                for (int b = 0; b < C::NB / 2; b++) {
+                    const int at = 2 * b + half;
+                    ks[b] = 32 * at < a.dk ? *reinterpret_cast<const unsigned short *>(pk + 34 * at) : 0;
+                    vsc[b] = 32 * at < a.dv ? *reinterpret_cast<const unsigned short *>(pv + 34 * at) : 0;
+                }
+            }
+        };
+        auto load_v = [&](int t, const int (&pg)[2]) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                bool o2;
-                int p2;
-                const char * p0 = rows16(a.v, key0 + 16 * x, o2, p2);
+                const int key = (t << 5) + 16 * x;
+                const char * p0 = rows16(a.v, key, pg[x]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const char * p = p0 + (long long)row_of(key0 + 16 * x + 4 * g + i) * a.v.ld_tok;
+                    const char * p = p0 + (long long)row_of(key + 4 * g + i) * a.v.ld_tok;
 #pragma unroll
                     for (int w = 0; w < C::NU; w++) {
                         const int col = C::column(m, w * C::VW);
@@ -395,17 +448,40 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                     }
                 }
             }
+        };
+
+        // K of the next tile is loaded behind the first product, V behind the
+        // second, page numbers a tile earlier: the loads run under the arithmetic
+        int page[2], next[2], later[2];
+        pages_of(t_lo + wave, page);
+        pages_of(t_lo + wave + 4, next);
+        if (t_lo + wave < t_hi) {
+            load_k(t_lo + wave, page);
+            load_v(t_lo + wave, page);
+        }
+        for (int t = t_lo + wave; t < t_hi; t += 4) {
+            const int key0 = t << 5;
+            const bool ok[2] = {good(page[0]), good(page[1])};
+            pages_of(t + 8, later);
+            bool odd = false;    // (uniform) values that are not finite are in this tile
+            bool far = false;    // (uniform) scales that fp16 products do not hold
             if constexpr (Q8) {
-                // scales of K and V: lane pair per key, through LDS for the lanes that hold them elsewhere
+                // to the lanes that hold the blocks' sums and values; cells that are not there weigh nothing
                 const int key = lane >> 1, half = lane & 1;
-                bool o2;
-                int p2;
-                const char * pk = rows16(a.k, key0 + (key & 16), o2, p2) + (long long)(key & 15) * a.k.ld_tok;
-                const char * pv = rows16(a.v, key0 + (key & 16), o2, p2) + (long long)(key & 15) * a.v.ld_tok;
-                for (int b = half; b < C::NB; b += 2) {
-                    scales[wave][0][key][b] = 32 * b < a.dk ? f16_value(*reinterpret_cast<const unsigned short *>(pk + 34 * b)) : 0.0f;
-                    scales[wave][1][key][b] = 32 * b < a.dv ? f16_value(*reinterpret_cast<const unsigned short *>(pv + 34 * b)) : 0.0f;
+                const bool there = key0 + key < held && (key < 16 ? ok[0] : ok[1]);
+#pragma unroll
+                for (int b = 0; b < C::NB / 2; b++) {
+                    k_scale[wave][2 * b + half][key] = f16_value(ks[b]);
+                    unsigned short d = there ? vsc[b] : 0;
+                    const bool whole = (d & 0x7c00u) != 0x7c00u;
+                    odd |= !whole;
+                    if (!whole) d = 0;
+                    const float v = fabsf(f16_value(d));
+                    far |= v != 0.0f && !(v >= 0x1p-14f && v <= 256.0f);
+                    v_scale[wave][2 * b + half][key] = __builtin_bit_cast(_Float16, d);
                 }
+                odd = __ballot(odd) != 0;
+                far = __ballot(far) != 0;
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -417,27 +493,35 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             for (int x = 0; x < 2; x++) {
 #pragma unroll
                 for (int r = 0; r < RT; r++) sc[r][x] = f4{0, 0, 0, 0};
+                if constexpr (TYPE == kF32) {
+                    // (four sums of a quarter of the products each: shorter chains, and less rounding)
+                    f4 part[RT][4];
 #pragma unroll
-                for (int j = 0; j < C::NKL; j++) {
-                    if constexpr (TYPE == kF32) {
+                    for (int r = 0; r < RT; r++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) part[r][e] = f4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < C::NKL; j++)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
 #pragma unroll
                             for (int r = 0; r < RT; r++)
-                                sc[r][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    __uint_as_float(kr[x][j][e]), __uint_as_float(q[r][j][e]), sc[r][x], 0, 0, 0);
-                    } else if constexpr (Q8) {
-                        unsigned w[4];
-                        for (int e = 0; e < 4; e++)
-                            w[e] = __float_as_uint(byte_value(kr[x][j], 2 * e)) >> 16 |
-                                   (__float_as_uint(byte_value(kr[x][j], 2 * e + 1)) & 0xffff0000u);
-                        const u4 kf = {w[0], w[1], w[2], w[3]};
+                                part[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    __uint_as_float(kr[x][j][e]), __uint_as_float(q[r][j][e]), part[r][e], 0, 0, 0);
 #pragma unroll
-                        for (int r = 0; r < RT; r++) {
-                            f4 part = mfma16<kBF16>(kf, q[r][j], f4{0, 0, 0, 0});
-                            if constexpr (C::SPLIT) part = mfma16<kBF16>(kf, q_lo[r][j], part);
-                            for (int i = 0; i < 4; i++) sc[r][x][i] += scales[wave][0][16 * x + 4 * g + i][j] * part[i];
-                        }
+                    for (int r = 0; r < RT; r++) sc[r][x] = (part[r][0] + part[r][1]) + (part[r][2] + part[r][3]);
+                }
+#pragma unroll
+                for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
+                    if constexpr (Q8) {
+                        unsigned w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            w[e] = code_pair(kr[x][j][e >> 1], kr[x][j][e >> 1], e & 1 ? 0x0c030c02u : 0x0c010c00u);
+                        const u4 kf = {w[0], w[1], w[2], w[3]};
+                        const f4 f = *reinterpret_cast<const f4 *>(&k_scale[wave][j][16 * x + 4 * g]);
+#pragma unroll
+                        for (int r = 0; r < RT; r++) sc[r][x] += f * mfma16<kF16>(kf, q[r][j], f4{0, 0, 0, 0});
                     } else {
                         const u4 kf = {kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]};
 #pragma unroll
@@ -447,33 +531,29 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             }
             // scale, bias, masks: a key that a row does not see has -inf
             const bool masked = key0 + 32 > clear || !ok[0] || !ok[1];
+            const f4 tile_bias[2] = {bias[0], bias[1]};
+            if (t + 4 < t_hi) load_k(t + 4, next);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                float b[4] = {0, 0, 0, 0};
-                if (a.bias) {
-                    const int k = (key0 + 16 * x + 4 * g) & page_mask;   // four cells of one page
-                    const float * p = a.bias + (((long long)page[x] * a.H + h) << a.shift) + k;
-                    for (int i = 0; i < 4; i++) b[i] = p[i];
-                }
+            for (int r = 0; r < RT; r++) {
 #pragma unroll
-                for (int r = 0; r < RT; r++)
+                for (int x = 0; x < 2; x++)
+#pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        float v = sc[r][x][i] * a.scale;
-                        if (a.bias) v = b[i] == -INFINITY ? -INFINITY : v + b[i];
-                        if (masked) {
-                            const int key = key0 + 16 * x + 4 * g + i, rel = key - base;
-                            bool see = key < held && ok[x];
-                            if (rel >= 0 && see) {
-                                if (a.mask)
-                                    see = rel < 64 * a.mask_words &&
-                                          (a.mask[(long long)(tok0 + tok[r]) * a.mask_words + (rel >> 6)] >> (rel & 63) & 1);
-                                else
-                                    see = rel <= tok[r];
-                            }
-                            if (!see) v = -INFINITY;
-                        }
+                        float v = sc[r][x][i];
+                        if constexpr (Q8 && QT == kBF16) v = v * row_up[r] * row_more[r];
+                        v *= a.scale;
+                        if (a.bias) v = tile_bias[x][i] == -INFINITY ? -INFINITY : v + tile_bias[x][i];
                         sc[r][x][i] = v;
                     }
+                if (masked) {
+                    unsigned see = seen32(a, sq, tok[r], key0);
+                    see &= (ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (!(see >> (16 * x + 4 * g + i) & 1)) sc[r][x][i] = -INFINITY;
+                }
             }
             // running maximum and sum
             float ref[RT];
@@ -493,8 +573,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             }
             // V of keys that no row may see is not to be multiplied, whatever it holds; and where some
             // rows see a key and others do not, a value that is not finite reaches only those that do
-            bool odd = false;   // (uniform) such values are in this tile
-            if (masked || a.bias) {
+            if (!Q8 && (masked || a.bias)) {
                 bool hidden = false;
 #pragma unroll
                 for (int r = 0; r < RT; r++)
@@ -517,27 +596,17 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                                             bad = true;
                                             z = 0;
                                         }
-                                    } else if constexpr (!Q8) {
+                                    } else {
                                         constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
                                         if ((z & e) == e || (z >> 16 & e) == e) bad = true;
                                         if ((z & e) == e) z &= 0xffff0000u;
                                         if ((z >> 16 & e) == e) z &= 0xffffu;
                                     }
                                 }
-                            if constexpr (Q8)
-                                for (int w = 0; w < C::NU; w++) {
-                                    const int blk = C::column(m, w * C::VW) / 32;
-                                    const float f = scales[wave][1][16 * x + 4 * g + i][blk];
-                                    if (!(fabsf(f) < INFINITY)) {
-                                        bad |= there;
-                                        scales[wave][1][16 * x + 4 * g + i][blk] = 0.0f;
-                                    }
-                                }
                         }
                     odd = __ballot(bad) != 0;
                 }
             }
-            if constexpr (Q8) __builtin_amdgcn_wave_barrier();
             // weights, as the second product's operand
             float p[RT][8];
 #pragma unroll
@@ -561,43 +630,73 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                             acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                                 __uint_as_float(vr[kk][c / C::VW][c % C::VW]), p[r][kk], acc[r][c], 0, 0, 0);
             } else {
-                u4 pf[RT], pl[C::SPLIT ? RT : 1];
+                u4 pf[RT];
 #pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    unsigned w[4], lo[4];
-                    for (int e = 0; e < 4; e++) {
-                        w[e] = pack2<C::MT>(p[r][2 * e], p[r][2 * e + 1]);
-                        if constexpr (C::SPLIT)
-                            lo[e] = pack2<kBF16>(p[r][2 * e] - bf16_value((unsigned short)w[e]),
-                                                 p[r][2 * e + 1] - bf16_value((unsigned short)(w[e] >> 16)));
-                    }
-                    pf[r] = u4{w[0], w[1], w[2], w[3]};
-                    if constexpr (C::SPLIT) pl[r] = u4{lo[0], lo[1], lo[2], lo[3]};
-                }
-                float vs[8];
+                for (int r = 0; r < RT; r++)
+                    pf[r] = u4{pack2<C::MT>(p[r][0], p[r][1]), pack2<C::MT>(p[r][2], p[r][3]), pack2<C::MT>(p[r][4], p[r][5]),
+                               pack2<C::MT>(p[r][6], p[r][7])};
+                if constexpr (Q8) {
+                    if (far) {
+                        u4 ph[RT], pl[RT];
 #pragma unroll
-                for (int c = 0; c < C::NC; c++) {
-                    const int w = c / C::VW, y = c % C::VW;
-                    if constexpr (Q8) {
-                        if (y == 0)
-                            for (int kk = 0; kk < 8; kk++)
-                                vs[kk] = scales[wave][1][16 * (kk >> 2) + 4 * g + (kk & 3)][C::column(m, c) / 32];
-                        unsigned hi[4], lo[4];
-                        for (int e = 0; e < 4; e++) {
-                            const float v0 = vs[2 * e] * byte_value(vr[2 * e][w], y);
-                            const float v1 = vs[2 * e + 1] * byte_value(vr[2 * e + 1][w], y);
-                            const unsigned h0 = __float_as_uint(v0) & 0xffff0000u, h1 = __float_as_uint(v1) & 0xffff0000u;
-                            hi[e] = h0 >> 16 | h1;
-                            lo[e] = pack2<kBF16>(v0 - __uint_as_float(h0), v1 - __uint_as_float(h1));
-                        }
-                        const u4 vh = {hi[0], hi[1], hi[2], hi[3]}, vl = {lo[0], lo[1], lo[2], lo[3]};
+                        for (int r = 0; r < RT; r++)
 #pragma unroll
-                        for (int r = 0; r < RT; r++) {
-                            acc[r][c] = mfma16<kBF16>(vh, pf[r], acc[r][c]);
-                            acc[r][c] = mfma16<kBF16>(vl, pf[r], acc[r][c]);
-                            if constexpr (C::SPLIT) acc[r][c] = mfma16<kBF16>(vh, pl[r], acc[r][c]);
+                            for (int e = 0; e < 4; e++) {
+                                ph[r][e] = pack2<kBF16>(p[r][2 * e], p[r][2 * e + 1]);
+                                pl[r][e] = pack2<kBF16>(p[r][2 * e] - bf16_value((unsigned short)ph[r][e]),
+                                                        p[r][2 * e + 1] - bf16_value((unsigned short)(ph[r][e] >> 16)));
+                            }
+#pragma unroll
+                        for (int c = 0; c < C::NC; c++) {
+                            const int w = c / C::VW, y = c % C::VW, blk = C::column(m, c) / 32;
+                            u4 vh, vl;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int k0 = 16 * (e >> 1) + 4 * g + 2 * (e & 1);
+                                const float v0 = (float)v_scale[wave][blk][k0] * byte_value(vr[2 * e][w], y);
+                                const float v1 = (float)v_scale[wave][blk][k0 + 1] * byte_value(vr[2 * e + 1][w], y);
+                                vh[e] = pack2<kBF16>(v0, v1);
+                                vl[e] = pack2<kBF16>(v0 - bf16_value((unsigned short)vh[e]),
+                                                     v1 - bf16_value((unsigned short)(vh[e] >> 16)));
+                            }
+#pragma unroll
+                            for (int r = 0; r < RT; r++) {
+                                acc[r][c] = mfma16<kBF16>(vh, ph[r], acc[r][c]);
+                                acc[r][c] = mfma16<kBF16>(vl, ph[r], acc[r][c]);
+                                acc[r][c] = mfma16<kBF16>(vh, pl[r], acc[r][c]);
+                            }
                         }
                     } else {
+                        h2 vs[4];
+#pragma unroll
+                        for (int c = 0; c < C::NC; c++) {
+                            const int w = c / C::VW, y = c % C::VW;
+                            if (y == 0) {
+                                const _Float16 * f = &v_scale[wave][C::column(m, c) / 32][4 * g];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) vs[e] = *reinterpret_cast<const h2 *>(f + 16 * (e >> 1) + 2 * (e & 1));
+                            }
+                            u4 vh, vl;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const h2 code = __builtin_bit_cast(h2, code_pair(vr[2 * e + 1][w][y >> 2], vr[2 * e][w][y >> 2],
+                                                                                 0x0c040c00u + 0x00010001u * (y & 3)));
+                                const h2 v = code * vs[e];
+                                vh[e] = __builtin_bit_cast(unsigned, v);
+                                if constexpr (QT == kF16)
+                                    vl[e] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(code, vs[e], -v));
+                            }
+#pragma unroll
+                            for (int r = 0; r < RT; r++) {
+                                acc[r][c] = mfma16<kF16>(vh, pf[r], acc[r][c]);
+                                if constexpr (QT == kF16) acc[r][c] = mfma16<kF16>(vl, pf[r], acc[r][c]);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C::NC; c++) {
+                        const int w = c / C::VW, y = c % C::VW;
                         unsigned f[4];
                         for (int e = 0; e < 4; e++)   // halves y of keys 2e, 2e+1
                             f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][w][y >> 1], vr[2 * e][w][y >> 1],
@@ -611,19 +710,22 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             if (odd) {
                 for (int kk = 0; kk < 32; kk++) {
                     if (key0 + kk >= held || !ok[kk >> 4]) continue;
-                    bool o2;
-                    int p2;
-                    const char * row = rows16(a.v, key0 + (kk & 16), o2, p2) + (long long)(kk & 15) * a.v.ld_tok;
+                    const char * row = rows16(a.v, key0 + (kk & 16), page[kk >> 4]) + (long long)(kk & 15) * a.v.ld_tok;
                     const int from = ((kk & 15) >> 2) * 16 + m;
+#pragma unroll
                     for (int r = 0; r < RT; r++) {
-                        const int e = kk >> 4, i = kk & 3;
-                        const float s0 = i == 0 ? sc[r][e][0] : i == 1 ? sc[r][e][1] : i == 2 ? sc[r][e][2] : sc[r][e][3];
+                        float s0 = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (e == (kk >> 4) * 4 + (kk & 3)) s0 = sc[r][e >> 2][e & 3];
                         const float sv = __shfl(s0, from);
                         const float w = exp_of(sv - ref[r]);
-                        for (int c = 0; c < C::NC && sv != -INFINITY; c++)
+#pragma unroll
+                        for (int c = 0; c < C::NC; c++)
+#pragma unroll
                             for (int y = 0; y < 4; y++) {
                                 const int col = C::column(4 * g + y, c);
-                                if (col >= a.dv) continue;
+                                if (col >= a.dv || sv == -INFINITY) continue;
                                 float v;
                                 if constexpr (Q8)
                                     v = f16_value(*reinterpret_cast<const unsigned short *>(row + col / 32 * 34)) *
@@ -634,6 +736,11 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                             }
                     }
                 }
+            }
+            if (t + 4 < t_hi) load_v(t + 4, next);
+            for (int x = 0; x < 2; x++) {
+                page[x] = next[x];
+                next[x] = later[x];
             }
         }
 
@@ -717,6 +824,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
 // half a fragment of V^T. Pieces past the head's width and rows past the last
 // key are read from a piece of zeros.
 __device__ const u4 zero_piece = {0, 0, 0, 0};
+__device__ const unsigned hidden_word = 0xff800000u;   // -inf
 
 typedef float f16x __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -738,6 +846,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
     constexpr int ROWB = 2 * D, KX = CH < 16 ? CH - 1 : 15, VX = CH < 16 ? CH / 2 - 1 : 7;
     constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f, log2_lift = TYPE == kF16 ? 10.0f : 0.0f;
     __shared__ __align__(16) char lds[2][2][BK * ROWB];     // [buffer][K, V]
+    __shared__ __align__(16) float cells[2][CELLS ? BK : 1];   // bias of each cell; -inf: hidden from every row
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hf = lane >> 5;
@@ -767,7 +876,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
     const int page_mask = CELLS ? (1 << a.shift) - 1 : 0;
     const bool flip = a.scale < 0.0f;   // (the maximum is taken of products by a positive number)
     const float scale = fabsf(a.scale);
-    const float c = (CELLS && a.bias ? 1.0f : scale) * kLog2e;
+    const float c = (CELLS ? 1.0f : scale) * kLog2e;   // (CELLS: scores take the scale with the bias)
 
     for (; (long long)tile * 128 < rows; tile += tile_step) {
         const int row0 = tile * 128, wrow0 = row0 + 32 * wave;
@@ -804,7 +913,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
             k_col[i] = at ^ (key & KX);
             v_col[i] = at ^ ((key & VX) << 1);
         }
-        int page[CELLS ? NL : 1];
+        int page[CELLS ? NL + 1 : 1];   // of the pieces' keys, and of key `lane`
         auto find_pages = [&](int t) {
             if constexpr (CELLS)
 #pragma unroll
@@ -812,6 +921,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                     const int key = t * BK + piece_key[i];
                     page[i] = t < t_hi && key < q.held ? q.table[key >> a.shift] : -1;
                 }
+            if constexpr (CELLS) {
+                const int key = t * BK + lane;
+                page[NL] = t < t_hi && lane < BK && key < q.held ? q.table[key >> a.shift] : -1;
+            }
         };
         auto fill = [&](int t, int buf) {
 #pragma unroll
@@ -830,6 +943,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                 const char * v = ok && 8 * v_col[i] < a.dv ? a.v.base + at * a.v.ld_tok + h * a.v.ld_head + 16 * v_col[i] : z;
                 load_lds16(k, &lds[buf][0][(i * 4 + wave) * 1024]);
                 load_lds16(v, &lds[buf][1][(i * 4 + wave) * 1024]);
+            }
+            if constexpr (CELLS) {
+                const int key = t * BK + lane;
+                const char * b = reinterpret_cast<const char *>(&hidden_word);
+                if (key < end_all && page[NL] >= 0 && page[NL] < a.n_pages)
+                    b = a.bias ? reinterpret_cast<const char *>(a.bias + (((long long)page[NL] * a.H + h) << a.shift) + (key & page_mask))
+                               : reinterpret_cast<const char *>(&zero_piece);
+                if (wave == 0 && lane < BK) load_lds4(b, reinterpret_cast<char *>(cells[buf]));
             }
         };
 
@@ -867,45 +988,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                 }
             }
             bool hidden = false;   // (uniform) a key of the tile that some row does not see
-            if (CELLS && a.bias) {
+            if constexpr (CELLS) {
+                hidden = __ballot(lane < BK && cells[buf][lane & (BK - 1)] == -INFINITY) != 0;
 #pragma unroll
                 for (int x = 0; x < SUB; x++)
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
-                        const int key = key0 + 32 * x + 8 * y + 4 * hf;   // four cells of one page
-                        const int p = key < q.held ? q.table[key >> a.shift] : -1;
-                        const bool ok = p >= 0 && p < a.n_pages;
-                        const float * b = a.bias + (((long long)(ok ? p : 0) * a.H + h) << a.shift) + (key & page_mask);
+                        const f4 b = *reinterpret_cast<const f4 *>(&cells[buf][32 * x + 8 * y + 4 * hf]);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const float v = b[i] == -INFINITY ? -INFINITY : sc[x][4 * y + i] * scale + b[i];
-                            sc[x][4 * y + i] = v;
-                            hidden |= v == -INFINITY;
+                            const float v = sc[x][4 * y + i] * scale + b[i];
+                            sc[x][4 * y + i] = hidden && b[i] == -INFINITY ? -INFINITY : v;
                         }
                     }
             }
-            bool bad_page = false;
-            if constexpr (CELLS) {
-                // (a page number that is none of the cache's hides its cells)
+            if (key0 + BK > clear) {
 #pragma unroll
-                for (int x = 0; x < BK / 16; x++) {
-                    const int key = key0 + 16 * x;
-                    const int p = key < q.held ? q.table[key >> a.shift] : 0;
-                    bad_page |= p < 0 || p >= a.n_pages;
+                for (int x = 0; x < SUB; x++) {
+                    const unsigned see = seen32(a, q, tok, key0 + 32 * x) >> (4 * hf);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (!(see >> (8 * (i >> 2) + (i & 3)) & 1)) sc[x][i] = -INFINITY;
                 }
-            }
-            const bool masked = key0 + BK > clear || bad_page;
-            if (masked) {
-#pragma unroll
-                for (int x = 0; x < SUB; x++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = key0 + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3);
-                        if (!row_sees<CELLS>(a, q, tok, key, bad_page)) sc[x][i] = -INFINITY;
-                    }
                 hidden = true;
             }
-            hidden = __ballot(hidden) != 0;
 
             float top = sc[0][0];
 #pragma unroll
@@ -936,8 +1042,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     // (with a bias the difference first: a score may be the type's lowest value)
-                    p[x][i] = CELLS && a.bias ? __builtin_amdgcn_exp2f((sc[x][i] - mc) * c + log2_lift)
-                                              : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], c, off));
+                    p[x][i] = CELLS ? __builtin_amdgcn_exp2f((sc[x][i] - mc) * c + log2_lift)
+                                    : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], c, off));
                     part += p[x][i];
                 }
             sum += part;
@@ -985,9 +1091,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                             if (y == x && i == reg) w = p[y][i];
                     w = __shfl(w, n + 32 * (kk >> 2 & 1));
                     const int key = key0 + kk;
-                    bool see = key < end_all && row_sees<CELLS>(a, q, tok, key, bad_page);
-                    if (CELLS && a.bias && see)
-                        see = a.bias[(((long long)q.table[key >> a.shift] * a.H + h) << a.shift) + (key & page_mask)] != -INFINITY;
+                    bool see = seen32(a, q, tok, key) & 1;
+                    if constexpr (CELLS) see = see && cells[buf][kk] != -INFINITY;
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -1015,7 +1120,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                                 f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]} * (1.0f / lift);
                     }
                 if (hf == 0) {
-                    a.part_ml[2 * at] = CELLS && a.bias ? mx : mx * scale;
+                    a.part_ml[2 * at] = CELLS ? mx : mx * scale;
                     a.part_ml[2 * at + 1] = sum;
                 }
             }
@@ -1033,13 +1138,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                     *reinterpret_cast<u2 *>(o + 2 * col) = v;
                 }
             if (a.lse && hf == 0)
-                a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS && a.bias ? mx : mx * scale) + logf(sum);
+                a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS ? mx : mx * scale) + logf(sum);
         }
         __syncthreads();
     }
 }
 
-// Joins the key ranges: a wave a row.
+// Joins the key ranges: a wave a row, a lane a range for the weights (64
+// ranges at most), then the ranges' sums eight loads ahead.
 template <int QT>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const int lane = threadIdx.x & 63;
@@ -1048,25 +1154,31 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     if (row >= n) return;
     const int tok = (int)(row / (a.H * a.G)), head = (int)(row % (a.H * a.G));
     if (tok < a.cu[0] || tok >= a.cu[a.n_seq]) return;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; s++) top = fmaxf(top, a.part_ml[2 * (s * n + row)]);
-    const float zero = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, x[4] = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; s++) {
-        const float f = exp_of(a.part_ml[2 * (s * n + row)] - zero);
-        l += f * a.part_ml[2 * (s * n + row) + 1];
-        for (int j = 0; j < 4; j++)
-            if (lane + 64 * j < a.dv) x[j] += f * a.part_o[(s * n + row) * a.dv + lane + 64 * j];
-    }
-    for (int j = 0; j < 4; j++) {
-        const int col = lane + 64 * j;
-        if (col >= a.dv) break;
-        const float v = l == 0.0f ? 0.0f : x[j] / l;
+    const bool mine = lane < a.splits;
+    const float m = mine ? a.part_ml[2 * (lane * n + row)] : -INFINITY;
+    const float part = mine ? a.part_ml[2 * (lane * n + row) + 1] : 0.0f;
+    float top = m;
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float w = exp_of(m - (top == -INFINITY ? 0.0f : top));
+    float l = w * part;
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int col = lane; col < ((a.dv + 63) & ~63); col += 64) {
+        const float * from = a.part_o + row * a.dv + (col < a.dv ? col : 0);
+        float x = 0.0f;
+        for (int s = 0; s < a.splits; s += 8) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = s + j < a.splits ? from[(s + j) * n * a.dv] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x += __shfl(w, (s + j) & 63) * y[j];
+        }
+        if (col >= a.dv) continue;
         const long long at = (long long)tok * a.o_tok + (long long)head * a.o_head + col;
         if constexpr (QT == kF32)
-            reinterpret_cast<float *>(a.o)[at] = v;
+            reinterpret_cast<float *>(a.o)[at] = x * inv;
         else
-            reinterpret_cast<unsigned short *>(a.o)[at] = (unsigned short)pack2<QT>(v, v);
+            reinterpret_cast<unsigned short *>(a.o)[at] = (unsigned short)pack2<QT>(x * inv, x * inv);
     }
     if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -INFINITY : top + logf(l);
 }
@@ -1104,7 +1216,8 @@ bool run_rows(const AttnArgs & a, int type, int qt, int rt, bool careful, long l
     return run_rows<kQ8, kBF16>(a, d, rt, careful, blocks, st);
 }
 
-// Row tiles a wave holds: two where there are more than 16 rows; at 256 wide heads two do not fit the registers
+// Row tiles a wave holds: two where there are more than 16 rows; at 256 wide
+// heads two do not fit the registers.
 int row_tiles(int d, bool careful, long long rows) { return rows > 16 && !careful && d < 256 ? 2 : 1; }
 
 template <int TYPE, bool CELLS> bool run_tiles(const AttnArgs & a, int d, long long blocks, hipStream_t st) {
@@ -1179,6 +1292,7 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     const CacheShape s = cache_shape(c, x);
     const size_t need = kvc_attn_cache_workspace(c, x);
     if (need && !ws) return -1;
+    if (reinterpret_cast<uintptr_t>(ws) & 15) return KV_COMPACT_E_UNSUPPORTED;
     if (need > ws_bytes) return KVC_E_SCRATCH;
     AttnArgs a{};
     const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);

@@ -769,7 +769,8 @@ int check_cache(const kvc_cache * c) {
         return KV_COMPACT_E_UNSUPPORTED;
     if ((c->k_type == KV_TYPE_Q8_0 && c->d_k % 32) || (c->v_type == KV_TYPE_Q8_0 && c->d_v % 32))
         return KV_COMPACT_E_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V)) & 15) return KV_COMPACT_E_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V) | reinterpret_cast<uintptr_t>(c->bias)) & 15)
+        return KV_COMPACT_E_UNSUPPORTED;
     return 0;
 }
 

@@ -37,7 +37,7 @@ BAD_CACHES = [
     (dict(page_size=8), -5), (dict(page_size=48), -5), (dict(page_size=2048), -5), (dict(page_size=0), -5),
     (dict(n_pages=(1 << 20) + 1), -5), (dict(max_pages=(1 << 20) + 1), -5), (dict(d_k=257), -5), (dict(d_v=300), -5),
     (dict(k_type=2), -5), (dict(v_type=3), -5), (dict(k_type=99), -5), (dict(k_type=Q8_0, d_k=48), -5),
-    (dict(v_type=Q8_0, d_v=16), -5), (dict(K=FAKE + 8), -5), (dict(V=FAKE + 2), -5), (dict(n_layers=20000), -5),
+    (dict(v_type=Q8_0, d_v=16), -5), (dict(K=FAKE + 8), -5), (dict(V=FAKE + 2), -5), (dict(bias=FAKE + 4), -5), (dict(n_layers=20000), -5),
 ]
 
 
