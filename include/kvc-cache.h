@@ -145,7 +145,8 @@ int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_
 
 /* ---- attention ------------------------------------------------------------
  * Token i, head h of an array: data + i*ld_tok + h*ld_head elements, the d
- * values of a head side by side. Any strides and base alignment; rows that
+ * values of a head side by side. Any strides (of K and V tokens: from 0 to
+ * under 2^24 bytes, a cache's rows too) and base alignment; rows that
  * are 16-byte aligned (base and strides) with d_k and d_v multiples of 8 are
  * the fast ones. n_head is a multiple of n_head_kv: query heads h*g ..
  * h*g+g-1 read KV head h. d_k, d_v from 1 to 256. Sums and softmax statistics

@@ -17,6 +17,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 // (the library is built with contraction off for the kernels that keep the
 // reference's rounding; a multiply-add here may be one rounding)
 #pragma clang fp contract(fast)
@@ -37,7 +39,8 @@ constexpr int kF32 = KV_TYPE_F32, kF16 = KV_TYPE_F16, kBF16 = KV_TYPE_BF16, kQ8 
 // Where rows of K or V stand: pages of a pool (table set), or one array.
 struct RowsAt {
     const char * base;
-    long long ld_tok, ld_head;   // bytes
+    long long ld_head;   // bytes
+    unsigned ld_tok;     // bytes, under 2^24
 };
 
 struct AttnArgs {
@@ -103,27 +106,30 @@ template <int TYPE> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// N elements (16 bytes, or 8) from column `col` of a row of d: whole vectors
-// where rows are aligned and d is a multiple of the vector, one by one
-// otherwise. Nothing is read at or past column d.
-template <int N, int BYTES, bool CAREFUL> __device__ __forceinline__ void load_cols(const char * row, int col, int d,
-                                                                                     unsigned * out) {
+// How the columns of a row are read: FULL the heads are as wide as the form,
+// PART rows are 16-byte aligned and heads whole vectors, ANY element by element.
+enum Columns { FULL, PART, ANY };
+
+// N elements (16 bytes, or 8) from column `col` of a row of d that stands at
+// base + row. Nothing is read at or past column d: zeros there.
+template <int N, int BYTES, Columns COLS>
+__device__ __forceinline__ void load_cols(const char * base, unsigned row, int col, int d, unsigned * out) {
     constexpr int W = N * BYTES / 4;
-    if constexpr (!CAREFUL) {
-        if (col < d) {
+    if constexpr (COLS != ANY) {
+        if (COLS == FULL || col < d) {
             if constexpr (W == 4)
-                *reinterpret_cast<u4 *>(out) = *reinterpret_cast<const u4 *>(row + (long long)col * BYTES);
+                *reinterpret_cast<u4 *>(out) = *reinterpret_cast<const u4 *>(base + (row + (unsigned)col * BYTES));
             else
-                *reinterpret_cast<u2 *>(out) = *reinterpret_cast<const u2 *>(row + (long long)col * BYTES);
+                *reinterpret_cast<u2 *>(out) = *reinterpret_cast<const u2 *>(base + (row + (unsigned)col * BYTES));
         } else {
             for (int i = 0; i < W; i++) out[i] = 0;
         }
     } else {
         for (int i = 0; i < W; i++) {
             if constexpr (BYTES == 4) {
-                out[i] = col + i < d ? reinterpret_cast<const unsigned *>(row)[col + i] : 0;
+                out[i] = col + i < d ? reinterpret_cast<const unsigned *>(base + row)[col + i] : 0;
             } else {
-                const unsigned short * r = reinterpret_cast<const unsigned short *>(row);
+                const unsigned short * r = reinterpret_cast<const unsigned short *>(base + row);
                 const unsigned a = col + 2 * i < d ? r[col + 2 * i] : 0, b = col + 2 * i + 1 < d ? r[col + 2 * i + 1] : 0;
                 out[i] = a | b << 16;
             }
@@ -256,8 +262,8 @@ __device__ __forceinline__ float byte_value(const unsigned * w, int i) {
 // become fp16 times a power of two of their row. V is scale times code in fp16
 // (for fp16 results with the remainder as a second term), which is a half step
 // off at most while the scales are between 2^-14 and 2^8; a tile with others
-// takes the product in fp32 as a sum of two bf16, and the weights too.
-template <int TYPE, int QT, int D, int RT, bool CAREFUL>
+// multiplies in fp32 (16x16x4).
+template <int TYPE, int QT, int D, int RT, Columns COLS>
 struct RowKernel {
     static constexpr int ES = TYPE == kF32 ? 4 : 2;          // bytes of a q element
     static constexpr int KV = 16 / ES;                       // q / k elements a 16-byte load holds
@@ -280,9 +286,51 @@ struct RowKernel {
     static __device__ __forceinline__ int column(int m, int c) { return (c / VW) * 16 * VW + VW * m + c % VW; }
 };
 
-template <int TYPE, int QT, int D, int RT, bool CAREFUL>
-__global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
-    using C = RowKernel<TYPE, QT, D, RT, CAREFUL>;
+// Values of V that are not finite, for the rows of tiles that left them out:
+// one by one, the scores computed again.
+template <int TYPE, int QT> struct Odd {
+    const AttnArgs & a;
+    const Sequence & q;
+    int h, tok, head;
+
+    __device__ __forceinline__ const char * row_of(const RowsAt & x, int key) const {
+        long long row = q.tok0 + key;
+        if (q.table) {
+            const int p = q.table[key >> a.shift];
+            if (p < 0 || p >= a.n_pages) return nullptr;
+            row = ((long long)p << a.shift) + (key & ((1 << a.shift) - 1));
+        }
+        return x.base + h * x.ld_head + row * x.ld_tok;
+    }
+    static __device__ __forceinline__ float at(const char * row, int col) {
+        if constexpr (TYPE == kQ8)
+            return f16_value(*reinterpret_cast<const unsigned short *>(row + col / 32 * 34)) *
+                   (float)*reinterpret_cast<const signed char *>(row + col / 32 * 34 + 2 + col % 32);
+        else
+            return value_of<TYPE>(row, col);
+    }
+    // weight (relative to exp(top)) times value where the value is not finite and the row sees its key, else 0
+    __device__ __forceinline__ float term(int key, int col, float top) const {
+        const char * v = row_of(a.v, key);
+        if (!v) return 0.0f;
+        const float x = at(v, col);
+        if (fabsf(x) < INFINITY || !(seen32(a, q, tok, key) & 1)) return 0.0f;
+        float b = 0.0f;
+        if (a.bias)
+            b = a.bias[(((long long)q.table[key >> a.shift] * a.H + h) << a.shift) + (key & ((1 << a.shift) - 1))];
+        if (b == -INFINITY) return 0.0f;
+        const char * k = row_of(a.k, key);
+        const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * (QT == kF32 ? 4 : 2);
+        float s = 0.0f;
+#pragma nounroll
+        for (int i = 0; i < a.dk; i++) s += value_of<QT>(p, i) * at(k, i);
+        return exp_of(s * a.scale + b - top) * x;
+    }
+};
+
+template <int TYPE, int QT, int D, int RT, Columns COLS>
+__global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D * RT > 128) ? 2 : 1) void k_attn_rows(AttnArgs a) {
+    using C = RowKernel<TYPE, QT, D, RT, COLS>;
     constexpr int ROWS = 16 * RT, LD = D + 4;
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) float join[4][ROWS][LD];
@@ -334,22 +382,28 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
         int tok[RT], head[RT];
         bool on[RT];
         u4 q[RT][C::NK];
-        float row_up[Q8 ? RT : 1], row_more[Q8 ? RT : 1];   // what the row's elements were multiplied by, in two parts
+        float to_score[RT], rest[RT];   // what turns a row's products into scores, in two parts (rest: 1 but for Q8_0 rows of extreme size)
+#pragma unroll
         for (int r = 0; r < RT; r++) {
             const int row = row0 + 16 * r + m;
             on[r] = row < rows;
             tok[r] = on[r] ? row / a.G : 0;
             head[r] = on[r] ? row % a.G : 0;
+            to_score[r] = a.scale;
+            rest[r] = 1.0f;
             const char * p = a.q + ((long long)(tok0 + tok[r]) * a.q_tok + (long long)(h * a.G + head[r]) * a.q_head) * C::ES;
+#pragma unroll
             for (int j = 0; j < C::NK; j++) {
                 unsigned w[4];
-                load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, w);
+                load_cols<C::KV, C::ES, COLS>(p, 0, 4 * C::KV * j + C::KV * g, a.dk, w);
                 q[r][j] = u4{w[0], w[1], w[2], w[3]};
             }
             if constexpr (Q8 && QT == kBF16) {
                 // the largest of the row to 2^14 (eight bits of it: exact; others from 2^-28 of it on)
                 unsigned top = 0;
+#pragma unroll
                 for (int j = 0; j < C::NK; j++)
+#pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const unsigned lo = q[r][j][i] & 0x7fffu, hi = q[r][j][i] >> 16 & 0x7fffu;
                         top = lo > top ? lo : top;
@@ -359,37 +413,48 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                 top = max(top, (unsigned)__shfl_xor((int)top, 32));
                 int e = (int)(top >> 7) - 127;               // of the largest
                 if (top == 0 || top >= 0x7f80u) e = 14;      // nothing, or not finite: as it is
-                const float up = __builtin_ldexpf(1.0f, (14 - e) / 2), more = __builtin_ldexpf(1.0f, 14 - e - (14 - e) / 2);
+                const int near = 14 - e > 100 ? 100 : 14 - e < -100 ? -100 : 14 - e;
+                const float up = __builtin_ldexpf(1.0f, near), more = __builtin_ldexpf(1.0f, 14 - e - near);
+#pragma unroll
                 for (int j = 0; j < C::NK; j++)
+#pragma unroll
                     for (int i = 0; i < 4; i++)
                         q[r][j][i] = pack2<kF16>(bf16_value((unsigned short)q[r][j][i]) * up * more,
                                                  bf16_value((unsigned short)(q[r][j][i] >> 16)) * up * more);
-                row_up[r] = 1.0f / up;
-                row_more[r] = 1.0f / more;
+                to_score[r] = a.scale * __builtin_ldexpf(1.0f, -near);
+                rest[r] = __builtin_ldexpf(1.0f, near - (14 - e));
             }
         }
         f4 acc[RT][C::NC];
         float mx[RT], sum[RT];
+#pragma unroll
         for (int r = 0; r < RT; r++) {
             mx[r] = -INFINITY;
             sum[r] = 0.0f;
+#pragma unroll
             for (int c = 0; c < C::NC; c++) acc[r][c] = f4{0, 0, 0, 0};
         }
 
         // pages of the two 16-cell groups of a tile (-1 past the end), and a group's first row
         auto pages_of = [&](int t, int (&pg)[2]) {
+#pragma unroll
             for (int x = 0; x < 2; x++) {
                 const int key = (t << 5) + 16 * x;
                 pg[x] = !table ? 0 : t < t_hi && key < held ? uniform_load(table + (key >> a.shift)) : -1;
             }
         };
         auto good = [&](int pg) { return !table || (pg >= 0 && pg < a.n_pages); };
+        // a group's first row (uniform), and the place of its row r behind it
         auto rows16 = [&](const RowsAt & x, int key, int pg) -> const char * {
-            if (!table) return x.base + (long long)(tok0 + key) * x.ld_tok + h * x.ld_head;
-            return x.base + (((long long)(good(pg) ? pg : 0) << a.shift) + (key & page_mask)) * x.ld_tok + h * x.ld_head;
+            const unsigned row = table ? ((unsigned)(good(pg) ? pg : 0) << a.shift) + (key & page_mask)
+                                       : (unsigned)(tok0 + (key < held ? key : held - 1));
+            return x.base + h * x.ld_head + (unsigned long long)row * x.ld_tok;
         };
-        // (contiguous rows end with the sequence: those past it repeat the last)
-        auto row_of = [&](int key) { return table ? key & 15 : (key < held ? key : held - 1) - (key & ~15); };
+        auto row_of = [&](const RowsAt & x, int key, int r) -> unsigned {
+            // (contiguous rows end with the sequence: those past it repeat the last)
+            if (!table) r = key + r < held ? r : key < held ? held - 1 - key : 0;
+            return (unsigned)__umul24(r, x.ld_tok);
+        };
 
         unsigned kr[2][C::NKL][C::WK];
         unsigned vr[8][C::NU][C::WV];
@@ -399,13 +464,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 const int key = (t << 5) + 16 * x;
-                const char * p = rows16(a.k, key, pg[x]) + (long long)row_of(key + m) * a.k.ld_tok;
+                const char * p = rows16(a.k, key, pg[x]);
+                const unsigned row = row_of(a.k, key, m);
 #pragma unroll
                 for (int j = 0; j < C::NKL; j++) {
                     if constexpr (Q8) {
-                        *reinterpret_cast<u2 *>(kr[x][j]) = 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + 34 * j + 2 + 8 * g) : u2{0, 0};
+                        *reinterpret_cast<u2 *>(kr[x][j]) =
+                            COLS == FULL || 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + (row + 34 * j + 2 + 8 * g)) : u2{0, 0};
                     } else {
-                        load_cols<C::KV, C::ES, CAREFUL>(p, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
+                        load_cols<C::KV, C::ES, COLS>(p, row, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
                     }
                 }
                 // (four cells of one page)
@@ -415,13 +482,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             }
             if constexpr (Q8) {
                 const int key = lane >> 1, half = lane & 1;
-                const char * pk = rows16(a.k, (t << 5) + (key & 16), pg[key >> 4]) + (long long)(key & 15) * a.k.ld_tok;
-                const char * pv = rows16(a.v, (t << 5) + (key & 16), pg[key >> 4]) + (long long)(key & 15) * a.v.ld_tok;
+                const char * pk = key < 16 ? rows16(a.k, t << 5, pg[0]) : rows16(a.k, (t << 5) + 16, pg[1]);
+                const char * pv = key < 16 ? rows16(a.v, t << 5, pg[0]) : rows16(a.v, (t << 5) + 16, pg[1]);
+                pk += __umul24(key & 15, a.k.ld_tok) + 34 * half;
+                pv += __umul24(key & 15, a.v.ld_tok) + 34 * half;
 #pragma unroll
                 for (int b = 0; b < C::NB / 2; b++) {
                     const int at = 2 * b + half;
-                    ks[b] = 32 * at < a.dk ? *reinterpret_cast<const unsigned short *>(pk + 34 * at) : 0;
-                    vsc[b] = 32 * at < a.dv ? *reinterpret_cast<const unsigned short *>(pv + 34 * at) : 0;
+                    ks[b] = COLS == FULL || 32 * at < a.dk ? *reinterpret_cast<const unsigned short *>(pk + 68 * b) : 0;
+                    vsc[b] = COLS == FULL || 32 * at < a.dv ? *reinterpret_cast<const unsigned short *>(pv + 68 * b) : 0;
                 }
             }
         };
@@ -432,39 +501,58 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                 const char * p0 = rows16(a.v, key, pg[x]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const char * p = p0 + (long long)row_of(key + 4 * g + i) * a.v.ld_tok;
+                    const unsigned row = row_of(a.v, key, 4 * g + i);
 #pragma unroll
                     for (int w = 0; w < C::NU; w++) {
                         const int col = C::column(m, w * C::VW);
                         if constexpr (Q8) {
-                            const char * b = p + col / 32 * 34 + 2 + col % 32;
+                            const char * b = p0 + (row + col / 32 * 34 + 2 + col % 32);
                             if constexpr (C::WV == 2)
-                                *reinterpret_cast<u2 *>(vr[4 * x + i][w]) = col < a.dv ? *reinterpret_cast<const u2_any *>(b) : u2{0, 0};
+                                *reinterpret_cast<u2 *>(vr[4 * x + i][w]) = COLS == FULL || col < a.dv ? *reinterpret_cast<const u2_any *>(b) : u2{0, 0};
                             else
-                                vr[4 * x + i][w][0] = col < a.dv ? *reinterpret_cast<const u1_any *>(b) : 0;
+                                vr[4 * x + i][w][0] = COLS == FULL || col < a.dv ? *reinterpret_cast<const u1_any *>(b) : 0;
                         } else {
-                            load_cols<C::VW, C::ES, CAREFUL>(p, col, a.dv, vr[4 * x + i][w]);
+                            load_cols<C::VW, C::ES, COLS>(p0, row, col, a.dv, vr[4 * x + i][w]);
                         }
                     }
                 }
             }
         };
 
+        int page[2], next[2], later[2];
+        f4 sc[RT][2];
+        bool odd = false;    // values of this lane's that are not finite (they are left out, and added at the end)
         // K of the next tile is loaded behind the first product, V behind the
         // second, page numbers a tile earlier: the loads run under the arithmetic
-        int page[2], next[2], later[2];
         pages_of(t_lo + wave, page);
         pages_of(t_lo + wave + 4, next);
         if (t_lo + wave < t_hi) {
             load_k(t_lo + wave, page);
             load_v(t_lo + wave, page);
         }
-        for (int t = t_lo + wave; t < t_hi; t += 4) {
+        // A tile that is not plain: a key hidden from some row, a bad page, Q8_0
+        // scales that fp16 products do not hold, or not finite.
+        auto special = [&](int t) {
+            bool any = (t << 5) + 32 > clear || !good(page[0]) || !good(page[1]);
+            bool mine = false;
+            if (a.bias)
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mine |= bias[x][i] == -INFINITY;
+            if constexpr (Q8)
+#pragma unroll
+                for (int b = 0; b < C::NB / 2; b++) {
+                    const float v = fabsf(f16_value(vsc[b]));
+                    mine |= v != 0.0f && !(v >= 0x1p-14f && v <= 256.0f);
+                }
+            return any || __ballot(mine) != 0;
+        };
+        auto step = [&](int t, auto kind) {
+            constexpr bool SPECIAL = decltype(kind)::value;
             const int key0 = t << 5;
             const bool ok[2] = {good(page[0]), good(page[1])};
             pages_of(t + 8, later);
-            bool odd = false;    // (uniform) values that are not finite are in this tile
-            bool far = false;    // (uniform) scales that fp16 products do not hold
             if constexpr (Q8) {
                 // to the lanes that hold the blocks' sums and values; cells that are not there weigh nothing
                 const int key = lane >> 1, half = lane & 1;
@@ -472,23 +560,22 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
 #pragma unroll
                 for (int b = 0; b < C::NB / 2; b++) {
                     k_scale[wave][2 * b + half][key] = f16_value(ks[b]);
-                    unsigned short d = there ? vsc[b] : 0;
-                    const bool whole = (d & 0x7c00u) != 0x7c00u;
-                    odd |= !whole;
-                    if (!whole) d = 0;
-                    const float v = fabsf(f16_value(d));
-                    far |= v != 0.0f && !(v >= 0x1p-14f && v <= 256.0f);
+                    unsigned short d = vsc[b];
+                    if constexpr (SPECIAL) {
+                        if (!there) d = 0;
+                        if ((d & 0x7c00u) == 0x7c00u) {
+                            odd = true;
+                            d = 0;
+                        }
+                    }
                     v_scale[wave][2 * b + half][key] = __builtin_bit_cast(_Float16, d);
                 }
-                odd = __ballot(odd) != 0;
-                far = __ballot(far) != 0;
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             }
 
             // S^T of both halves
-            f4 sc[RT][2];
 #pragma unroll
             for (int x = 0; x < 2; x++) {
 #pragma unroll
@@ -530,7 +617,6 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                 }
             }
             // scale, bias, masks: a key that a row does not see has -inf
-            const bool masked = key0 + 32 > clear || !ok[0] || !ok[1];
             const f4 tile_bias[2] = {bias[0], bias[1]};
             if (t + 4 < t_hi) load_k(t + 4, next);
 #pragma unroll
@@ -539,13 +625,12 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                 for (int x = 0; x < 2; x++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        float v = sc[r][x][i];
-                        if constexpr (Q8 && QT == kBF16) v = v * row_up[r] * row_more[r];
-                        v *= a.scale;
-                        if (a.bias) v = tile_bias[x][i] == -INFINITY ? -INFINITY : v + tile_bias[x][i];
+                        float v = sc[r][x][i] * to_score[r];
+                        if constexpr (Q8 && QT == kBF16) v *= rest[r];
+                        if (a.bias) v = SPECIAL && tile_bias[x][i] == -INFINITY ? -INFINITY : v + tile_bias[x][i];
                         sc[r][x][i] = v;
                     }
-                if (masked) {
+                if constexpr (SPECIAL) {
                     unsigned see = seen32(a, sq, tok[r], key0);
                     see &= (ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u);
 #pragma unroll
@@ -561,51 +646,46 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             for (int r = 0; r < RT; r++) {
                 float t0 = fmaxf(fmaxf(sc[r][0][0], sc[r][0][1]), fmaxf(sc[r][0][2], sc[r][0][3]));
                 float t1 = fmaxf(fmaxf(sc[r][1][0], sc[r][1][1]), fmaxf(sc[r][1][2], sc[r][1][3]));
-                const float now = fmaxf(mx[r], row_max(fmaxf(t0, t1)));
-                const float top = now == -INFINITY ? 0.0f : now;
-                ref[r] = top - C::log_lift;
-                if (__ballot(now != mx[r])) {
-                    const float f = exp_of(mx[r] - top);
+                const float now = row_max(fmaxf(t0, t1));
+                // (weights up to e^3 are left to grow before the sums are scaled)
+                if (__ballot(now - mx[r] > 3.0f)) {
+                    const float to = fmaxf(mx[r], now);
+                    const float f = exp_of(mx[r] - (to == -INFINITY ? 0.0f : to));
+                    mx[r] = to;
                     sum[r] *= f;
+#pragma unroll
                     for (int c = 0; c < C::NC; c++) acc[r][c] *= f;
                 }
-                mx[r] = now;
+                ref[r] = (mx[r] == -INFINITY ? 0.0f : mx[r]) - C::log_lift;
             }
             // V of keys that no row may see is not to be multiplied, whatever it holds; and where some
             // rows see a key and others do not, a value that is not finite reaches only those that do
-            if (!Q8 && (masked || a.bias)) {
-                bool hidden = false;
+            if constexpr (SPECIAL && !Q8) {
 #pragma unroll
-                for (int r = 0; r < RT; r++)
-                    for (int x = 0; x < 2; x++)
-                        for (int i = 0; i < 4; i++) hidden |= sc[r][x][i] == -INFINITY;
-                if (__ballot(hidden)) {
-                    bool bad = false;
+                for (int x = 0; x < 2; x++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                    for (int i = 0; i < 4; i++) {
+                        const int kk = 4 * x + i;
+                        const bool there = key0 + 16 * x + 4 * g + i < held && ok[x];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int kk = 4 * x + i;
-                            const bool there = key0 + 16 * x + 4 * g + i < held && ok[x];
-                            for (int w = 0; w < C::NU; w++)
-                                for (int y = 0; y < C::WV; y++) {
-                                    unsigned & z = vr[kk][w][y];
-                                    if (!there) z = 0;
-                                    if constexpr (TYPE == kF32) {
-                                        if ((z & 0x7f800000u) == 0x7f800000u) {
-                                            bad = true;
-                                            z = 0;
-                                        }
-                                    } else {
-                                        constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
-                                        if ((z & e) == e || (z >> 16 & e) == e) bad = true;
-                                        if ((z & e) == e) z &= 0xffff0000u;
-                                        if ((z >> 16 & e) == e) z &= 0xffffu;
+                        for (int w = 0; w < C::NU; w++)
+#pragma unroll
+                            for (int y = 0; y < C::WV; y++) {
+                                unsigned & z = vr[kk][w][y];
+                                if (!there) z = 0;
+                                if constexpr (TYPE == kF32) {
+                                    if ((z & 0x7f800000u) == 0x7f800000u) {
+                                        odd = true;
+                                        z = 0;
                                     }
+                                } else {
+                                    constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
+                                    odd |= (z & e) == e || (z >> 16 & e) == e;
+                                    if ((z & e) == e) z &= 0xffff0000u;
+                                    if ((z >> 16 & e) == e) z &= 0xffffu;
                                 }
-                        }
-                    odd = __ballot(bad) != 0;
-                }
+                            }
+                    }
             }
             // weights, as the second product's operand
             float p[RT][8];
@@ -636,36 +716,17 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                     pf[r] = u4{pack2<C::MT>(p[r][0], p[r][1]), pack2<C::MT>(p[r][2], p[r][3]), pack2<C::MT>(p[r][4], p[r][5]),
                                pack2<C::MT>(p[r][6], p[r][7])};
                 if constexpr (Q8) {
-                    if (far) {
-                        u4 ph[RT], pl[RT];
+                    if constexpr (SPECIAL) {
 #pragma unroll
-                        for (int r = 0; r < RT; r++)
+                        for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                ph[r][e] = pack2<kBF16>(p[r][2 * e], p[r][2 * e + 1]);
-                                pl[r][e] = pack2<kBF16>(p[r][2 * e] - bf16_value((unsigned short)ph[r][e]),
-                                                        p[r][2 * e + 1] - bf16_value((unsigned short)(ph[r][e] >> 16)));
+                            for (int c = 0; c < C::NC; c++) {
+                                const float v = (float)v_scale[wave][C::column(m, c) / 32][16 * (kk >> 2) + 4 * g + (kk & 3)] *
+                                                byte_value(vr[kk][c / C::VW], c % C::VW);
+#pragma unroll
+                                for (int r = 0; r < RT; r++)
+                                    acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[r][kk], acc[r][c], 0, 0, 0);
                             }
-#pragma unroll
-                        for (int c = 0; c < C::NC; c++) {
-                            const int w = c / C::VW, y = c % C::VW, blk = C::column(m, c) / 32;
-                            u4 vh, vl;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int k0 = 16 * (e >> 1) + 4 * g + 2 * (e & 1);
-                                const float v0 = (float)v_scale[wave][blk][k0] * byte_value(vr[2 * e][w], y);
-                                const float v1 = (float)v_scale[wave][blk][k0 + 1] * byte_value(vr[2 * e + 1][w], y);
-                                vh[e] = pack2<kBF16>(v0, v1);
-                                vl[e] = pack2<kBF16>(v0 - bf16_value((unsigned short)vh[e]),
-                                                     v1 - bf16_value((unsigned short)(vh[e] >> 16)));
-                            }
-#pragma unroll
-                            for (int r = 0; r < RT; r++) {
-                                acc[r][c] = mfma16<kBF16>(vh, ph[r], acc[r][c]);
-                                acc[r][c] = mfma16<kBF16>(vl, ph[r], acc[r][c]);
-                                acc[r][c] = mfma16<kBF16>(vh, pl[r], acc[r][c]);
-                            }
-                        }
                     } else {
                         h2 vs[4];
 #pragma unroll
@@ -698,6 +759,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                     for (int c = 0; c < C::NC; c++) {
                         const int w = c / C::VW, y = c % C::VW;
                         unsigned f[4];
+#pragma unroll
                         for (int e = 0; e < 4; e++)   // halves y of keys 2e, 2e+1
                             f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][w][y >> 1], vr[2 * e][w][y >> 1],
                                                          y & 1 ? 0x07060302u : 0x05040100u);
@@ -707,41 +769,16 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                     }
                 }
             }
-            if (odd) {
-                for (int kk = 0; kk < 32; kk++) {
-                    if (key0 + kk >= held || !ok[kk >> 4]) continue;
-                    const char * row = rows16(a.v, key0 + (kk & 16), page[kk >> 4]) + (long long)(kk & 15) * a.v.ld_tok;
-                    const int from = ((kk & 15) >> 2) * 16 + m;
-#pragma unroll
-                    for (int r = 0; r < RT; r++) {
-                        float s0 = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (e == (kk >> 4) * 4 + (kk & 3)) s0 = sc[r][e >> 2][e & 3];
-                        const float sv = __shfl(s0, from);
-                        const float w = exp_of(sv - ref[r]);
-#pragma unroll
-                        for (int c = 0; c < C::NC; c++)
-#pragma unroll
-                            for (int y = 0; y < 4; y++) {
-                                const int col = C::column(4 * g + y, c);
-                                if (col >= a.dv || sv == -INFINITY) continue;
-                                float v;
-                                if constexpr (Q8)
-                                    v = f16_value(*reinterpret_cast<const unsigned short *>(row + col / 32 * 34)) *
-                                        (float)*reinterpret_cast<const signed char *>(row + col / 32 * 34 + 2 + col % 32);
-                                else
-                                    v = value_of<TYPE>(row, col);
-                                if (!(fabsf(v) < INFINITY)) acc[r][c][y] += w * v;
-                            }
-                    }
-                }
-            }
             if (t + 4 < t_hi) load_v(t + 4, next);
+#pragma unroll
             for (int x = 0; x < 2; x++) {
                 page[x] = next[x];
                 next[x] = later[x];
             }
+        };
+        for (int t = t_lo + wave; t < t_hi;) {
+            for (; t < t_hi && !special(t); t += 4) step(t, std::false_type{});
+            for (; t < t_hi && special(t); t += 4) step(t, std::true_type{});
         }
 
         // the four waves' parts, and the result
@@ -763,7 +800,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                             f4{acc[r][w * C::VW + y][i], acc[r][w * C::VW + y + 1][i], acc[r][w * C::VW + y + 2][i],
                                acc[r][w * C::VW + y + 3][i]};
         }
-        __syncthreads();
+        const bool any_odd = __syncthreads_or(odd);
         for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
             const int r = e / (D / 4), col = e % (D / 4) * 4;
             const int row = row0 + r;
@@ -773,10 +810,25 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
             const float zero = top == -INFINITY ? 0.0f : top;
             f4 x = {0, 0, 0, 0};
             float l = 0.0f;
+#pragma unroll
             for (int w = 0; w < 4; w++) {
                 const float f = exp_of(join_m[w][r] - zero) * (1.0f / C::lift);
                 l += f * join_l[w][r];
                 x += f * *reinterpret_cast<const f4 *>(&join[w][r][col]);
+            }
+            if (__builtin_expect(any_odd, 0)) {
+                // what was left out reaches the rows that see its key
+                Odd<TYPE, QT> o{a, sq, h, row / a.G, row % a.G};
+#pragma nounroll
+                for (int key = t_lo * 32; key < t_hi * 32 && key < held; key++)
+#pragma nounroll
+                    for (int y = 0; y < 4 && col + y < a.dv; y++) {
+                        const float add = o.term(key, col + y, zero);
+                        x[0] += y == 0 ? add : 0.0f;
+                        x[1] += y == 1 ? add : 0.0f;
+                        x[2] += y == 2 ? add : 0.0f;
+                        x[3] += y == 3 ? add : 0.0f;
+                    }
             }
             const long long out = (long long)(tok0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
             if (a.splits > 1) {
@@ -790,6 +842,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
                 // (a row that sees a cell has a weight of 1 in its sum, or NaN)
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 char * o = a.o + ((long long)(tok0 + row / a.G) * a.o_tok + (long long)(h * a.G + row % a.G) * a.o_head) * C::ES;
+#pragma unroll
                 for (int y = 0; y < 4; y++) {
                     if (col + y >= a.dv) break;
                     const float v = x[y] * inv;
@@ -959,6 +1012,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+        bool odd = false;                   // values of this lane's fragments that are not finite (left out, see below)
         float mx = -INFINITY, sum = 0.0f;   // (mx: in units of s, kept up to 2^5 below the true maximum)
         float mc = 0.0f;                    // mx, or 0 while nothing is seen
 
@@ -1033,7 +1087,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                     for (int i = 0; i < 16; i++) acc[d][i] *= f;
             }
             // V of the tile's parts, weights of the lane's row
-            bool odd = false;
             float p[SUB][16];
             float part = 0.0f;
             const float off = log2_lift - mc * c;
@@ -1079,30 +1132,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                         acc[d] = mfma32<TYPE>(vf, pf, acc[d]);
                     }
                 }
-            if (hidden && __ballot(odd)) {
-                // values that are not finite reach only the rows that see their key
-                for (int kk = 0; kk < BK; kk++) {
-                    const int x = kk >> 5, reg = (kk >> 3 & 3) * 4 + (kk & 3);
-                    float w = 0.0f;
-#pragma unroll
-                    for (int y = 0; y < SUB; y++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (y == x && i == reg) w = p[y][i];
-                    w = __shfl(w, n + 32 * (kk >> 2 & 1));
-                    const int key = key0 + kk;
-                    bool see = seen32(a, q, tok, key) & 1;
-                    if constexpr (CELLS) see = see && cells[buf][kk] != -INFINITY;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int col = 32 * d + 8 * (i >> 2) + 4 * hf + (i & 3);
-                            const float v = value_of<TYPE>(vt + kk * ROWB + (((col >> 3) ^ ((kk & VX) << 1)) << 4), col & 7);
-                            if (see && !(fabsf(v) < INFINITY)) acc[d][i] += w * v;
-                        }
-                }
-            }
         }
         sum += __shfl_xor(sum, 32);
         sum *= 1.0f / lift;
@@ -1139,6 +1168,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                 }
             if (a.lse && hf == 0)
                 a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS ? mx : mx * scale) + logf(sum);
+        }
+        if (__builtin_expect(__ballot(odd) != 0, 0) && on && sum == sum) {
+            // Values that are not finite were left out of tiles where a key is
+            // hidden from some row. They decide every result they reach (of rows
+            // that are not NaN by their scores): those are written again.
+            Odd<TYPE, TYPE> o{a, q, h, tok, head};
+            const float top = (mx == -INFINITY ? 0.0f : mx) * (CELLS ? 1.0f : scale);
+#pragma nounroll
+            for (int col = hf; col < a.dv; col += 2) {
+                float x = 0.0f;
+#pragma nounroll
+                for (int key = t_lo * BK; key < t_hi * BK && key < q.held; key++) x += o.term(key, col, top);
+                if (x == 0.0f) continue;
+                if (CELLS && a.splits > 1)
+                    a.part_o[((long long)split * a.n_tok * a.H * a.G + out) * a.dv + col] = x;
+                else
+                    reinterpret_cast<unsigned short *>(a.o)[(long long)(q.tok0 + tok) * a.o_tok +
+                                                            (long long)(h * a.G + head) * a.o_head + col] =
+                        (unsigned short)pack2<TYPE>(x, x);
+            }
         }
         __syncthreads();
     }
@@ -1192,15 +1241,16 @@ bool vec_rows(const kvc_heads & x, int bytes) {
     return ((reinterpret_cast<uintptr_t>(x.data) | (uintptr_t)(x.ld_tok * bytes) | (uintptr_t)(x.ld_head * bytes)) & 15) == 0;
 }
 
-template <int TYPE, int QT, int D, int RT, bool CAREFUL> bool run_rows(const AttnArgs & a, long long blocks, hipStream_t st) {
-    return launch(k_attn_rows<TYPE, QT, D, RT, CAREFUL>, dim3((unsigned)blocks), dim3(256), st, a);
+template <int TYPE, int QT, int D, int RT, Columns COLS> bool run_rows(const AttnArgs & a, long long blocks, hipStream_t st) {
+    return launch(k_attn_rows<TYPE, QT, D, RT, COLS>, dim3((unsigned)blocks), dim3(256), st, a);
 }
 template <int TYPE, int QT, int D> bool run_rows(const AttnArgs & a, int rt, bool careful, long long blocks, hipStream_t st) {
     if constexpr (TYPE != kQ8)
-        if (careful) return run_rows<TYPE, QT, D, 1, true>(a, blocks, st);
+        if (careful) return run_rows<TYPE, QT, D, 1, ANY>(a, blocks, st);
+    const bool full = a.dk == D && a.dv == D;
     if constexpr (D < 256)
-        if (rt == 2) return run_rows<TYPE, QT, D, 2, false>(a, blocks, st);
-    return run_rows<TYPE, QT, D, 1, false>(a, blocks, st);
+        if (rt == 2) return full ? run_rows<TYPE, QT, D, 2, FULL>(a, blocks, st) : run_rows<TYPE, QT, D, 2, PART>(a, blocks, st);
+    return full ? run_rows<TYPE, QT, D, 1, FULL>(a, blocks, st) : run_rows<TYPE, QT, D, 1, PART>(a, blocks, st);
 }
 template <int TYPE, int QT> bool run_rows(const AttnArgs & a, int d, int rt, bool careful, long long blocks, hipStream_t st) {
     if (d == 64) return run_rows<TYPE, QT, 64>(a, rt, careful, blocks, st);
@@ -1294,12 +1344,13 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     if (need && !ws) return -1;
     if (reinterpret_cast<uintptr_t>(ws) & 15) return KV_COMPACT_E_UNSUPPORTED;
     if (need > ws_bytes) return KVC_E_SCRATCH;
-    AttnArgs a{};
     const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);
     const long long vrow = (long long)kv_quant_row_bytes(c->v_type, c->n_head_kv * c->d_v);
     const long long cells = (long long)c->n_pages * c->page_size;
-    a.k = RowsAt{static_cast<const char *>(c->K) + x->layer * cells * krow, krow, krow / c->n_head_kv};
-    a.v = RowsAt{static_cast<const char *>(c->V) + x->layer * cells * vrow, vrow, vrow / c->n_head_kv};
+    if (krow >= 1 << 24 || vrow >= 1 << 24) return KV_COMPACT_E_UNSUPPORTED;
+    AttnArgs a{};
+    a.k = RowsAt{static_cast<const char *>(c->K) + x->layer * cells * krow, krow / c->n_head_kv, (unsigned)krow};
+    a.v = RowsAt{static_cast<const char *>(c->V) + x->layer * cells * vrow, vrow / c->n_head_kv, (unsigned)vrow};
     a.q = static_cast<const char *>(x->q.data);
     a.o = static_cast<char *>(x->o.data);
     a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;
@@ -1344,9 +1395,11 @@ int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
     if ((reinterpret_cast<uintptr_t>(x->q.data) | reinterpret_cast<uintptr_t>(x->k.data) |
          reinterpret_cast<uintptr_t>(x->v.data) | reinterpret_cast<uintptr_t>(x->o.data)) & (es - 1))
         return KV_COMPACT_E_UNSUPPORTED;
+    if (x->k.ld_tok < 0 || x->k.ld_tok * es >= 1 << 24 || x->v.ld_tok < 0 || x->v.ld_tok * es >= 1 << 24)
+        return KV_COMPACT_E_UNSUPPORTED;
     AttnArgs a{};
-    a.k = RowsAt{static_cast<const char *>(x->k.data), x->k.ld_tok * es, x->k.ld_head * es};
-    a.v = RowsAt{static_cast<const char *>(x->v.data), x->v.ld_tok * es, x->v.ld_head * es};
+    a.k = RowsAt{static_cast<const char *>(x->k.data), x->k.ld_head * es, (unsigned)(x->k.ld_tok * es)};
+    a.v = RowsAt{static_cast<const char *>(x->v.data), x->v.ld_head * es, (unsigned)(x->v.ld_tok * es)};
     a.q = static_cast<const char *>(x->q.data);
     a.o = static_cast<char *>(x->o.data);
     a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;

@@ -180,7 +180,8 @@ def test_prompt_arguments(dll):
                      (dict(cu=None), -1), (dict(n_seq=-1), -2), (dict(n_tok=-1), -2), (dict(n_head=0), -2),
                      (dict(n_head_kv=0), -2), (dict(n_head=5), -2), (dict(d_k=0), -2), (dict(d_v=0), -2),
                      (dict(d_k=257), -5), (dict(d_v=512), -5), (dict(type=Q8_0), -5), (dict(type=3), -5), (dict(q=odd), -5),
-                     (dict(k=odd), -5), (dict(v=odd), -5), (dict(o=odd), -5), (dict(n_seq=0), 0), (dict(n_tok=0), 0),
+                     (dict(k=odd), -5), (dict(v=odd), -5), (dict(k=kc.Heads(FAKE, 1 << 23, 64)), -5),
+                     (dict(v=kc.Heads(FAKE, -256, 64)), -5), (dict(o=odd), -5), (dict(n_seq=0), 0), (dict(n_tok=0), 0),
                      (dict(type=F32), kc.E_DEVICE), (dict(type=BF16), kc.E_DEVICE)):
         assert call(**kw) == code, kw
 
