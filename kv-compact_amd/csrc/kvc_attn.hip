@@ -57,7 +57,8 @@ struct AttnArgs {
     const unsigned long long * mask;
     int mask_words, n_seq, n_tok, H, G, dk, dv;
     int shift, n_pages, max_seqs, max_pages;
-    int splits, tiles;     // key ranges; row tiles the grid has for each sequence (0: flat over all sequences)
+    int splits, range;     // key ranges of at least `range` keys: a short sequence fills the first few
+    int tiles;             // row tiles the grid has for each sequence (0: flat over all sequences)
     float scale;
     float * part_o;        // [splits][n_tok * n_head][dv]
     float * part_ml;       // [splits][n_tok * n_head][2]
@@ -169,6 +170,14 @@ __device__ __forceinline__ Sequence sequence_of(const AttnArgs & a, int s) {
     return q;
 }
 
+// Tiles of a key range, of n_tiles in all. Ranges of the same size for all
+// sequences are blocks of the same length; more keys than the launch was told
+// of make them longer.
+__device__ __forceinline__ int range_tiles(const AttnArgs & a, int n_tiles, int keys) {
+    const int even = (n_tiles + a.splits - 1) / a.splits, said = (a.range + keys - 1) / keys;
+    return even > said ? even : said;
+}
+
 // The u-th tile of `rows` rows of all sequences together, those of a sequence
 // from its end (the most keys first). False past the last one.
 __device__ __forceinline__ bool find_tile(const AttnArgs & a, int u, int rows, int lane, int & s, int & tile) {
@@ -212,20 +221,23 @@ __device__ __forceinline__ unsigned seen32(const AttnArgs & a, const Sequence & 
     return all & (unsigned)bits;
 }
 
-// 16 bytes a lane from memory to LDS, lane after lane from `to` (uniform). The
-// compiler does not count these loads: wait_lds_loads() does.
-__device__ __forceinline__ void load_lds16(const char * from, char * to) {
-    const unsigned at = __builtin_amdgcn_readfirstlane(
-        (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+// 16 bytes a lane from memory to LDS, lane l's to `to` + 16 l (`from` and `to`
+// uniform; lanes that are off leave theirs as it is). The compiler does not
+// count these loads: wait_lds_loads() does.
+__device__ __forceinline__ void load_lds16(const char * from, unsigned offset, char * to) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory");
 }
-// (4 bytes)
+// (4 bytes, each from an address of its own)
 __device__ __forceinline__ void load_lds4(const char * from, char * to) {
     const unsigned at = __builtin_amdgcn_readfirstlane(
         (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
 }
-__device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// until at most N of the wave's loads are on their way
+template <int N> __device__ __forceinline__ void wait_lds_loads() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 
 typedef u2 u2_any __attribute__((aligned(2)));
 typedef unsigned u1_any __attribute__((aligned(2)));
@@ -335,6 +347,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) float join[4][ROWS][LD];
     __shared__ float join_m[4][ROWS], join_l[4][ROWS];
+    __shared__ int join_odd[4][2];
     // Q8_0 scales of a wave's tile, by block and key
     __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
     __shared__ __align__(16) _Float16 v_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
@@ -375,7 +388,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
         const int first_tok = row0 / a.G;
         const int clear = a.mask ? base : base + first_tok + 1;   // keys before it are seen by every row
         const int n_tiles = (end_all + 31) >> 5;
-        const int per = (n_tiles + a.splits - 1) / a.splits;
+        const int per = range_tiles(a, n_tiles, 32);
         const int t_lo = split * per, t_hi = t_lo + per < n_tiles ? t_lo + per : n_tiles;
 
         // rows of this lane
@@ -521,7 +534,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 
         int page[2], next[2], later[2];
         f4 sc[RT][2];
-        bool odd = false;    // values of this lane's that are not finite (they are left out, and added at the end)
+        int odd_lo = 1 << 30, odd_hi = 0;   // tiles with values that are not finite (they are left out, and added at the end)
         // K of the next tile is loaded behind the first product, V behind the
         // second, page numbers a tile earlier: the loads run under the arithmetic
         pages_of(t_lo + wave, page);
@@ -550,6 +563,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
         };
         auto step = [&](int t, auto kind) {
             constexpr bool SPECIAL = decltype(kind)::value;
+            bool odd = false;
             const int key0 = t << 5;
             const bool ok[2] = {good(page[0]), good(page[1])};
             pages_of(t + 8, later);
@@ -769,6 +783,10 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                     }
                 }
             }
+            if (SPECIAL && __ballot(odd)) {
+                odd_lo = t < odd_lo ? t : odd_lo;
+                odd_hi = t + 1;
+            }
             if (t + 4 < t_hi) load_v(t + 4, next);
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -800,7 +818,15 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                             f4{acc[r][w * C::VW + y][i], acc[r][w * C::VW + y + 1][i], acc[r][w * C::VW + y + 2][i],
                                acc[r][w * C::VW + y + 3][i]};
         }
-        const bool any_odd = __syncthreads_or(odd);
+        if (lane == 0) {
+            join_odd[wave][0] = odd_lo;
+            join_odd[wave][1] = odd_hi;
+        }
+        __syncthreads();
+        for (int w = 0; w < 4; w++) {
+            odd_lo = min(odd_lo, join_odd[w][0]);
+            odd_hi = max(odd_hi, join_odd[w][1]);
+        }
         for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
             const int r = e / (D / 4), col = e % (D / 4) * 4;
             const int row = row0 + r;
@@ -816,11 +842,11 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                 l += f * join_l[w][r];
                 x += f * *reinterpret_cast<const f4 *>(&join[w][r][col]);
             }
-            if (__builtin_expect(any_odd, 0)) {
+            if (__builtin_expect(odd_lo < odd_hi, 0)) {
                 // what was left out reaches the rows that see its key
                 Odd<TYPE, QT> o{a, sq, h, row / a.G, row % a.G};
 #pragma nounroll
-                for (int key = t_lo * 32; key < t_hi * 32 && key < held; key++)
+                for (int key = odd_lo * 32; key < odd_hi * 32 && key < held; key++)
 #pragma nounroll
                     for (int y = 0; y < 4 && col + y < a.dv; y++) {
                         const float add = o.term(key, col + y, zero);
@@ -833,7 +859,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
             const long long out = (long long)(tok0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
             if (a.splits > 1) {
                 const long long at = (long long)split * a.n_tok * a.H * a.G + out;
-                for (int y = 0; y < 4 && col + y < a.dv; y++) a.part_o[at * a.dv + col + y] = x[y];
+                for (int y = 0; y < 4 && col + y < a.dv && t_lo < t_hi; y++) a.part_o[at * a.dv + col + y] = x[y];
                 if (col == 0) {
                     a.part_ml[2 * at] = top;
                     a.part_ml[2 * at + 1] = l;
@@ -859,8 +885,10 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: 128 of them a block, 32 a wave, over tiles of BK keys that all
-// four waves read from LDS.
+// Many rows: 32 of them a wave, RW waves of rows (32 RW rows a block), over
+// tiles of 64 keys that all waves read from LDS. KW = 2: half of the waves
+// take the first 32 keys of each tile, half the others, and they join at the
+// end.
 //
 // Fragments (32x32x16, lane l, n = l % 32, h = l / 32): an operand's lane holds
 // row n and elements 8h .. 8h+7 of the summed axis; a result's lane column n
@@ -869,14 +897,18 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // second product from the registers they were made in: element j of step s is
 // key 16s + 4h + j, or 16s + 8 + 4h + j - 4.
 //
-// K and V reach LDS by direct loads of 16 bytes a lane (no registers), a tile
-// ahead, two buffers. They stand row by row with their 16-byte pieces
-// exchanged, K's by key % 8 or 16 so that the 32 rows of a fragment read
-// different banks, V's in pairs by key % 8 so that the four rows that
+// K and V reach LDS by direct loads of 16 bytes a lane (no registers), a
+// uniform address and a lane's constant offset each. They stand row by row with
+// their 16-byte pieces exchanged, K's by key % 8 so that the rows of a fragment
+// read different banks, V's in pairs by key % 8 so that the four rows that
 // ds_read_b64_tr_b16 turns round do: it gives a lane four keys of one column,
-// half a fragment of V^T. Pieces past the head's width and rows past the last
-// key are read from a piece of zeros.
-__device__ const u4 zero_piece = {0, 0, 0, 0};
+// half a fragment of V^T. Pieces past a head's width stay zero.
+//
+// A prompt's blocks are four waves, two of them on a CU: one's softmax runs
+// under the other's products, and K and V come from L2 (one tile ahead). Over
+// a cache HBM has to be kept busy: eight waves share four buffers (RW = 4: 96
+// KB on their way), or two blocks of four waves two buffers each (RW = 2).
+__device__ const unsigned zero_word = 0;
 __device__ const unsigned hidden_word = 0xff800000u;   // -inf
 
 typedef float f16x __attribute__((ext_vector_type(16)));
@@ -891,17 +923,23 @@ template <int TYPE> __device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
 
 __device__ __forceinline__ float pair_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
 
-template <int TYPE, int D, bool CELLS>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a) {
-    constexpr int BK = D == 256 ? 32 : 64, SUB = BK / 32;   // keys of a tile, in parts of 32
+template <int TYPE, int D, bool CELLS, int RW>
+__global__ __launch_bounds__(64 * RW * (CELLS ? 2 : 1), CELLS && RW == 4 && D < 256 ? 2 : D == 256 ? 1 : 2)
+void k_attn_tiles(AttnArgs a) {
+    constexpr int KW = CELLS ? 2 : 1, WAVES = RW * KW, ROWS = 32 * RW;
+    constexpr int BK = !CELLS && D == 256 ? 32 : 64, SUB = BK / 32 / KW;   // keys of a tile; of a wave, in parts of 32
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8;     // steps of a score, column tiles, pieces of a row
-    constexpr int NL = BK * CH / 256;                       // direct loads of a wave and tile, K or V
-    constexpr int ROWB = 2 * D, KX = CH < 16 ? CH - 1 : 15, VX = CH < 16 ? CH / 2 - 1 : 7;
+    constexpr int NL = BK * CH / (64 * WAVES);              // direct loads of a wave and tile, K or V
+    constexpr int KPL = 512 / D;                            // keys of one: rows of one 16-cell group
+    constexpr int BUFS = CELLS && RW == 4 && D < 256 ? 4 : 2, AHEAD = BUFS - 1;
+    constexpr int ROWB = 2 * D, VX = CH < 16 ? CH / 2 - 1 : 7;
+    constexpr int LOADS = 2 * NL + (CELLS ? 1 : 0);         // of a wave and tile
     constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f, log2_lift = TYPE == kF16 ? 10.0f : 0.0f;
-    __shared__ __align__(16) char lds[2][2][BK * ROWB];     // [buffer][K, V]
-    __shared__ __align__(16) float cells[2][CELLS ? BK : 1];   // bias of each cell; -inf: hidden from every row
+    __shared__ __align__(16) char lds[BUFS][2][BK * ROWB];  // [buffer][K, V]
+    __shared__ __align__(16) float cells[BUFS][CELLS ? BK : 1];   // bias of each cell; -inf: hidden from every row
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rw = wave % RW, kw = wave / RW;
     const int n = lane & 31, hf = lane >> 5;
 
     int u = blockIdx.x;
@@ -918,12 +956,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
         s = u / a.tiles;
         tile_step = a.tiles;
     } else {
-        if (!find_tile(a, u, 128, lane, s, tile)) return;
+        if (!find_tile(a, u, ROWS, lane, s, tile)) return;
         tile_step = 1 << 30;
     }
     s = __builtin_amdgcn_readfirstlane(s);
     tile = __builtin_amdgcn_readfirstlane(tile);
-    Sequence q = sequence_of(a, s);
+    const Sequence q = sequence_of(a, s);
     if (q.n_new <= 0) return;
     const int rows = q.n_new * a.G;
     const int page_mask = CELLS ? (1 << a.shift) - 1 : 0;
@@ -931,16 +969,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
     const float scale = fabsf(a.scale);
     const float c = (CELLS ? 1.0f : scale) * kLog2e;   // (CELLS: scores take the scale with the bias)
 
-    for (; (long long)tile * 128 < rows; tile += tile_step) {
-        const int row0 = tile * 128, wrow0 = row0 + 32 * wave;
-        const int last_tok = (row0 + 127) / a.G < q.n_new ? (row0 + 127) / a.G : q.n_new - 1;
+    // A lane's piece of a direct load: its row there, and where that stands.
+    // (The exchange of pieces is the same in all of a wave's loads.)
+    const int piece_row = lane / CH, piece_key = wave * KPL + piece_row;
+    const unsigned k_col = (lane % CH) ^ (piece_key & 7), v_col = (lane % CH) ^ ((piece_key & VX) << 1);
+    const unsigned k_off = __umul24(piece_row, a.k.ld_tok) + 16 * k_col, v_off = __umul24(piece_row, a.v.ld_tok) + 16 * v_col;
+    const bool k_piece = (int)(8 * k_col) < a.dk, v_piece = (int)(8 * v_col) < a.dv;
+    const char * k_head = a.k.base + h * a.k.ld_head;
+    const char * v_head = a.v.base + h * a.v.ld_head;
+    for (int i = threadIdx.x; i < BUFS * 2 * BK * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+    __syncthreads();
+
+    for (; (long long)tile * ROWS < rows; tile += tile_step) {
+        const int row0 = tile * ROWS, wrow0 = row0 + 32 * rw;
+        const int last_tok = (row0 + ROWS - 1) / a.G < q.n_new ? (row0 + ROWS - 1) / a.G : q.n_new - 1;
         const int end_all = q.held == 0 ? 0 : (CELLS && a.mask ? q.held : q.base + last_tok + 1);
         // keys before it are seen by every row of this wave
         const int clear = CELLS && a.mask ? q.base : q.base + (wrow0 < rows ? wrow0 / a.G + 1 : last_tok + 1);
         const int n_tiles = (end_all + BK - 1) / BK;
         int t_lo = 0, t_hi = n_tiles;
         if constexpr (CELLS) {
-            const int per = (n_tiles + a.splits - 1) / a.splits;
+            const int per = range_tiles(a, n_tiles, BK);
             t_lo = split * per;
             t_hi = t_lo + per < n_tiles ? t_lo + per : n_tiles;
         }
@@ -957,53 +1006,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
             }
         }
 
-        // where a lane's pieces of a tile come from
-        int piece_key[NL], k_col[NL], v_col[NL];
-#pragma unroll
-        for (int i = 0; i < NL; i++) {
-            const int x = (i * 4 + wave) * 64 + lane, key = x / CH, at = x % CH;
-            piece_key[i] = key;
-            k_col[i] = at ^ (key & KX);
-            v_col[i] = at ^ ((key & VX) << 1);
-        }
-        int page[CELLS ? NL + 1 : 1];   // of the pieces' keys, and of key `lane`
+        // pages of a tile's pieces, and of the 16 cells whose biases this wave loads
+        int page[CELLS ? NL + 1 : 1];
+        auto page_at = [&](int key) { return key < end_all ? uniform_load(q.table + (key >> a.shift)) : -1; };
         auto find_pages = [&](int t) {
-            if constexpr (CELLS)
-#pragma unroll
-                for (int i = 0; i < NL; i++) {
-                    const int key = t * BK + piece_key[i];
-                    page[i] = t < t_hi && key < q.held ? q.table[key >> a.shift] : -1;
-                }
             if constexpr (CELLS) {
-                const int key = t * BK + lane;
-                page[NL] = t < t_hi && lane < BK && key < q.held ? q.table[key >> a.shift] : -1;
+#pragma unroll
+                for (int i = 0; i < NL; i++) page[i] = page_at(t * BK + (i * WAVES + wave) * KPL);
+                page[NL] = page_at(t * BK + 16 * (wave % (BK / 16)));
             }
         };
+        // (Rows of a page past the last cell are loaded as they are, those of a
+        // bad page from page 0: their cells are hidden. Rows past the end of
+        // contiguous tokens are not loaded. A tile past the last one is loaded
+        // like the last, so that every wave has the same loads on their way.)
         auto fill = [&](int t, int buf) {
+            if (t >= t_hi) t = t_hi - 1;
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int key = t * BK + piece_key[i];
-                long long at;
-                bool ok = key < end_all;
+                const int key = t * BK + (i * WAVES + wave) * KPL;
+                unsigned at;
+                bool there = true;
                 if constexpr (CELLS) {
-                    ok = ok && page[i] >= 0 && page[i] < a.n_pages;
-                    at = ((long long)page[i] << a.shift) + (key & page_mask);
+                    const int p = page[i] >= 0 && page[i] < a.n_pages ? page[i] : 0;
+                    at = ((unsigned)p << a.shift) + (key & page_mask);
                 } else {
-                    at = q.tok0 + key;
+                    at = (unsigned)(q.tok0 + key);
+                    there = key + piece_row < q.held;
                 }
-                const char * z = reinterpret_cast<const char *>(&zero_piece);
-                const char * k = ok && 8 * k_col[i] < a.dk ? a.k.base + at * a.k.ld_tok + h * a.k.ld_head + 16 * k_col[i] : z;
-                const char * v = ok && 8 * v_col[i] < a.dv ? a.v.base + at * a.v.ld_tok + h * a.v.ld_head + 16 * v_col[i] : z;
-                load_lds16(k, &lds[buf][0][(i * 4 + wave) * 1024]);
-                load_lds16(v, &lds[buf][1][(i * 4 + wave) * 1024]);
+                char * to = &lds[buf][0][(i * WAVES + wave) * 1024];
+                if (there && k_piece) load_lds16(k_head + (unsigned long long)at * a.k.ld_tok, k_off, to);
+                if (there && v_piece) load_lds16(v_head + (unsigned long long)at * a.v.ld_tok, v_off, to + BK * ROWB);
             }
             if constexpr (CELLS) {
-                const int key = t * BK + lane;
+                const int in = 16 * (wave % (BK / 16)), key = t * BK + in + (lane & 15);
                 const char * b = reinterpret_cast<const char *>(&hidden_word);
                 if (key < end_all && page[NL] >= 0 && page[NL] < a.n_pages)
                     b = a.bias ? reinterpret_cast<const char *>(a.bias + (((long long)page[NL] * a.H + h) << a.shift) + (key & page_mask))
-                               : reinterpret_cast<const char *>(&zero_piece);
-                if (wave == 0 && lane < BK) load_lds4(b, reinterpret_cast<char *>(cells[buf]));
+                               : reinterpret_cast<const char *>(&zero_word);
+                if (lane < 16) load_lds4(b, reinterpret_cast<char *>(&cells[buf][in]));
             }
         };
 
@@ -1012,23 +1053,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-        bool odd = false;                   // values of this lane's fragments that are not finite (left out, see below)
+        int odd_lo = 1 << 30, odd_hi = 0;   // tiles with values that are not finite and were left out (see below)
         float mx = -INFINITY, sum = 0.0f;   // (mx: in units of s, kept up to 2^5 below the true maximum)
         float mc = 0.0f;                    // mx, or 0 while nothing is seen
 
-        find_pages(t_lo);
-        if (t_lo < t_hi) fill(t_lo, 0);
-        find_pages(t_lo + 1);
+        if (t_lo < t_hi) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                find_pages(t_lo + i < t_hi ? t_lo + i : t_hi - 1);
+                fill(t_lo + i, i);
+            }
+            find_pages(t_lo + AHEAD < t_hi ? t_lo + AHEAD : t_hi - 1);
+        }
         for (int t = t_lo; t < t_hi; t++) {
-            const int buf = (t - t_lo) & 1;
-            wait_lds_loads();
+            const int buf = (t - t_lo) % BUFS;
+            wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (t + 1 < t_hi) fill(t + 1, buf ^ 1);
-            find_pages(t + 2);
-            const char * kt = lds[buf][0];
-            const char * vt = lds[buf][1];
-            const int key0 = t * BK;
+            fill(t + AHEAD, (buf + AHEAD) % BUFS);
+            find_pages(t + AHEAD + 1 < t_hi ? t + AHEAD + 1 : t_hi - 1);
+            const int part0 = 32 * SUB * kw, key0 = t * BK + part0;   // this wave's keys of the tile
+            const char * kt = lds[buf][0] + part0 * ROWB;
+            const char * vt = lds[buf][1] + part0 * ROWB;
 
             f16x sc[SUB];
 #pragma unroll
@@ -1037,26 +1083,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                 for (int i = 0; i < 16; i++) sc[x][i] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < KS; j++) {
-                    const u4 kf = *reinterpret_cast<const u4 *>(kt + (32 * x + n) * ROWB + (((2 * j + hf) ^ (n & KX)) << 4));
+                    const u4 kf = *reinterpret_cast<const u4 *>(kt + (32 * x + n) * ROWB + (((2 * j + hf) ^ (n & 7)) << 4));
                     sc[x] = mfma32<TYPE>(kf, qf[j], sc[x]);
                 }
             }
-            bool hidden = false;   // (uniform) a key of the tile that some row does not see
+            bool hidden = false;   // (uniform) a key that some row does not see
             if constexpr (CELLS) {
-                hidden = __ballot(lane < BK && cells[buf][lane & (BK - 1)] == -INFINITY) != 0;
+                hidden = __ballot(cells[buf][part0 + (lane & (32 * SUB - 1))] == -INFINITY) != 0;
 #pragma unroll
                 for (int x = 0; x < SUB; x++)
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
-                        const f4 b = *reinterpret_cast<const f4 *>(&cells[buf][32 * x + 8 * y + 4 * hf]);
+                        const f4 b = *reinterpret_cast<const f4 *>(&cells[buf][part0 + 32 * x + 8 * y + 4 * hf]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float v = sc[x][4 * y + i] * scale + b[i];
-                            sc[x][4 * y + i] = hidden && b[i] == -INFINITY ? -INFINITY : v;
-                        }
+                        for (int i = 0; i < 4; i++) sc[x][4 * y + i] = sc[x][4 * y + i] * scale + b[i];
                     }
+                if (hidden) {   // (whatever the product was)
+#pragma unroll
+                    for (int x = 0; x < SUB; x++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (cells[buf][part0 + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3)] == -INFINITY) sc[x][i] = -INFINITY;
+                }
             }
-            if (key0 + BK > clear) {
+            if (key0 + 32 * SUB > clear) {
 #pragma unroll
                 for (int x = 0; x < SUB; x++) {
                     const unsigned see = seen32(a, q, tok, key0 + 32 * x) >> (4 * hf);
@@ -1086,7 +1136,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[d][i] *= f;
             }
-            // V of the tile's parts, weights of the lane's row
+            // weights, and V
             float p[SUB][16];
             float part = 0.0f;
             const float off = log2_lift - mc * c;
@@ -1100,6 +1150,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                     part += p[x][i];
                 }
             sum += part;
+            bool odd = false;
 #pragma unroll
             for (int x = 0; x < SUB; x++)
 #pragma unroll
@@ -1125,26 +1176,66 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
 #pragma unroll
                             for (int y = 0; y < 4; y++) {
                                 const bool lo = (vf[y] & e) == e, hi = (vf[y] >> 16 & e) == e;
-                                odd |= lo || hi;
+                                // (cells that no row sees, past the end among them, are nothing)
+                                const int kk = 32 * x + 16 * st + 8 * (y >> 1) + 4 * hf + 2 * (y & 1);
+                                if (lo) odd |= CELLS ? cells[buf][part0 + kk] != -INFINITY : key0 + kk < q.held;
+                                if (hi) odd |= CELLS ? cells[buf][part0 + kk + 1] != -INFINITY : key0 + kk + 1 < q.held;
                                 vf[y] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
                             }
                         }
                         acc[d] = mfma32<TYPE>(vf, pf, acc[d]);
                     }
                 }
+            if (hidden && __ballot(odd)) {
+                odd_lo = t < odd_lo ? t : odd_lo;
+                odd_hi = t + 1;
+            }
         }
+        wait_lds_loads<0>();   // (LDS is given up, or used again, with no load to it on its way)
         sum += __shfl_xor(sum, 32);
+        if constexpr (KW == 2) {
+            // the second half of the waves hands its part over, lane for lane
+            f4 * over = reinterpret_cast<f4 *>(lds) + rw * (DT * 4 + 1) * 64 + lane;
+            __syncthreads();
+            if (kw == 1) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        over[(4 * d + y) * 64] = f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]};
+                over[DT * 4 * 64] = f4{mx, sum, __int_as_float(odd_lo), __int_as_float(odd_hi)};
+            }
+            __syncthreads();
+            if (kw == 0) {
+                const f4 other = over[DT * 4 * 64];
+                const float top = fmaxf(mx, other[0]), use = top == -INFINITY ? 0.0f : top;
+                const float f = __builtin_amdgcn_exp2f((mx - use) * c), g = __builtin_amdgcn_exp2f((other[0] - use) * c);
+                mx = top;
+                sum = sum * f + other[1] * g;
+                odd_lo = min(odd_lo, __float_as_int(other[2]));
+                odd_hi = max(odd_hi, __float_as_int(other[3]));
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const f4 x = over[(4 * d + y) * 64];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[d][4 * y + i] = acc[d][4 * y + i] * f + x[i] * g;
+                    }
+            }
+        }
         sum *= 1.0f / lift;
         const long long out = (long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head;
+        const bool write = on && kw == 0;
         if (CELLS && a.splits > 1) {
             const long long at = (long long)split * a.n_tok * a.H * a.G + out;
-            if (on) {
+            if (write) {
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
                         const int col = 32 * d + 8 * y + 4 * hf;
-                        if (col < a.dv)
+                        if (col < a.dv && t_lo < t_hi)
                             *reinterpret_cast<f4 *>(a.part_o + at * a.dv + col) =
                                 f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]} * (1.0f / lift);
                     }
@@ -1153,7 +1244,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
                     a.part_ml[2 * at + 1] = sum;
                 }
             }
-        } else if (on) {
+        } else if (write) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * lift);
             char * o = a.o + 2 * ((long long)(q.tok0 + tok) * a.o_tok + (long long)(h * a.G + head) * a.o_head);
 #pragma unroll
@@ -1169,7 +1260,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
             if (a.lse && hf == 0)
                 a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS ? mx : mx * scale) + logf(sum);
         }
-        if (__builtin_expect(__ballot(odd) != 0, 0) && on && sum == sum) {
+        if (__builtin_expect(odd_lo < odd_hi, 0) && write && sum == sum) {
             // Values that are not finite were left out of tiles where a key is
             // hidden from some row. They decide every result they reach (of rows
             // that are not NaN by their scores): those are written again.
@@ -1179,7 +1270,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
             for (int col = hf; col < a.dv; col += 2) {
                 float x = 0.0f;
 #pragma nounroll
-                for (int key = t_lo * BK; key < t_hi * BK && key < q.held; key++) x += o.term(key, col, top);
+                for (int key = odd_lo * BK; key < odd_hi * BK && key < q.held; key++) x += o.term(key, col, top);
                 if (x == 0.0f) continue;
                 if (CELLS && a.splits > 1)
                     a.part_o[((long long)split * a.n_tok * a.H * a.G + out) * a.dv + col] = x;
@@ -1190,6 +1281,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tiles(AttnArgs a
             }
         }
         __syncthreads();
+        if (KW == 2 && (long long)(tile + tile_step) * ROWS < rows) {
+            // (what was handed over stood on pieces that are to be zero)
+            for (int i = threadIdx.x; i < BUFS * 2 * BK * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+            __syncthreads();
+        }
     }
 }
 
@@ -1216,11 +1312,14 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         const float * from = a.part_o + row * a.dv + (col < a.dv ? col : 0);
         float x = 0.0f;
         for (int s = 0; s < a.splits; s += 8) {
-            float y[8];
+            float f[8], y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = s + j < a.splits ? from[(s + j) * n * a.dv] : 0.0f;
+            for (int j = 0; j < 8; j++) f[j] = s + j < 64 ? __shfl(w, s + j) : 0.0f;
+            // (a range that saw nothing has no sums)
 #pragma unroll
-            for (int j = 0; j < 8; j++) x += __shfl(w, (s + j) & 63) * y[j];
+            for (int j = 0; j < 8; j++) y[j] = f[j] != 0.0f ? from[(s + j) * n * a.dv] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x += f[j] * y[j];
         }
         if (col >= a.dv) continue;
         const long long at = (long long)tok * a.o_tok + (long long)head * a.o_head + col;
@@ -1248,6 +1347,8 @@ template <int TYPE, int QT, int D> bool run_rows(const AttnArgs & a, int rt, boo
     if constexpr (TYPE != kQ8)
         if (careful) return run_rows<TYPE, QT, D, 1, ANY>(a, blocks, st);
     const bool full = a.dk == D && a.dv == D;
+    if constexpr (TYPE == kQ8 && D < 256)
+        if (rt == 4) return full ? run_rows<TYPE, QT, D, 4, FULL>(a, blocks, st) : run_rows<TYPE, QT, D, 4, PART>(a, blocks, st);
     if constexpr (D < 256)
         if (rt == 2) return full ? run_rows<TYPE, QT, D, 2, FULL>(a, blocks, st) : run_rows<TYPE, QT, D, 2, PART>(a, blocks, st);
     return full ? run_rows<TYPE, QT, D, 1, FULL>(a, blocks, st) : run_rows<TYPE, QT, D, 1, PART>(a, blocks, st);
@@ -1266,27 +1367,34 @@ bool run_rows(const AttnArgs & a, int type, int qt, int rt, bool careful, long l
     return run_rows<kQ8, kBF16>(a, d, rt, careful, blocks, st);
 }
 
-// Row tiles a wave holds: two where there are more than 16 rows; at 256 wide
-// heads two do not fit the registers.
-int row_tiles(int d, bool careful, long long rows) { return rows > 16 && !careful && d < 256 ? 2 : 1; }
-
-template <int TYPE, bool CELLS> bool run_tiles(const AttnArgs & a, int d, long long blocks, hipStream_t st) {
-    const dim3 grid((unsigned)blocks);
-    if (d == 64) return launch(k_attn_tiles<TYPE, 64, CELLS>, grid, dim3(256), st, a);
-    if (d == 128) return launch(k_attn_tiles<TYPE, 128, CELLS>, grid, dim3(256), st, a);
-    return launch(k_attn_tiles<TYPE, 256, CELLS>, grid, dim3(256), st, a);
+// Row tiles a wave holds: two where there are more than 16 rows, and over a
+// Q8_0 cache, whose rows cost more to decode than to multiply, four where
+// there are more than 32; at 256 wide heads more than one does not fit the
+// registers.
+int row_tiles(int type, int d, bool careful, long long rows) {
+    if (rows <= 16 || careful || d == 256) return 1;
+    return rows > 32 && type == kQ8 ? 4 : 2;
 }
-template <bool CELLS> bool run_tiles(const AttnArgs & a, int type, long long blocks, hipStream_t st) {
+
+template <int TYPE, bool CELLS, int RW> bool run_tiles(const AttnArgs & a, int d, long long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks), block(64 * RW * (CELLS ? 2 : 1));
+    if (d == 64) return launch(k_attn_tiles<TYPE, 64, CELLS, RW>, grid, block, st, a);
+    if (d == 128) return launch(k_attn_tiles<TYPE, 128, CELLS, RW>, grid, block, st, a);
+    if constexpr (CELLS && RW == 4) return false;   // (not asked for: eight waves' sums of 256 columns do not fit)
+    else return launch(k_attn_tiles<TYPE, 256, CELLS, RW>, grid, block, st, a);
+}
+template <bool CELLS, int RW> bool run_tiles(const AttnArgs & a, int type, long long blocks, hipStream_t st) {
     const int d = head_tile(a.dk, a.dv);
-    return type == kF16 ? run_tiles<kF16, CELLS>(a, d, blocks, st) : run_tiles<kBF16, CELLS>(a, d, blocks, st);
+    return type == kF16 ? run_tiles<kF16, CELLS, RW>(a, d, blocks, st) : run_tiles<kBF16, CELLS, RW>(a, d, blocks, st);
 }
 
 int esize(int type) { return type == kF32 ? 4 : 2; }
 
 // Shape of a cache call's launch.
 struct CacheShape {
-    int rt, tiles, splits;
-    bool careful, whole;   // whole: k_attn_tiles
+    int rt, tiles, splits, range;
+    bool careful;
+    int whole;   // waves of rows of k_attn_tiles, 0: k_attn_rows
 };
 CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     CacheShape s{};
@@ -1294,16 +1402,21 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     // a cache's pages are 16-byte aligned: its rows are where a head is whole 16-byte pieces
     s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
     const long long rows = (long long)a->max_new * G;
-    s.rt = row_tiles(head_tile(c->d_k, c->d_v), s.careful, rows);
-    s.whole = rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es);
-    const int block_rows = s.whole ? 128 : 16 * s.rt;
+    s.rt = row_tiles(c->k_type, head_tile(c->d_k, c->d_v), s.careful, rows);
+    if (rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es)) 
+        s.whole = rows > 64 && c->d_k <= 128 && c->d_v <= 128 ? 4 : 2;
+    const int block_rows = s.whole ? 32 * s.whole : 16 * s.rt;
     const long long tiles = (rows + block_rows - 1) / block_rows;
     s.tiles = (int)(tiles < 1 ? 1 : tiles > 65536 ? 65536 : tiles);
-    // key ranges: enough blocks to fill the GPU, each with at least 8 tiles of 32 keys
-    const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles;
-    long long want = (1024 + units - 1) / units, most = a->max_len / 256;
+    // Key ranges: enough blocks to fill the GPU, each with at least 8 tiles of
+    // 32 keys. Ranges of the same size in all sequences; four row tiles a wave
+    // (one block a CU, and its time goes with its keys) take the same number
+    // of ranges of each sequence instead.
+    const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles, blocks = s.whole || s.rt == 4 ? 1024 : 4096;
+    long long want = (blocks + units - 1) / units, most = a->max_len / 256;
     want = want < most ? want : most;
     s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
+    s.range = s.rt == 4 ? 0 : (a->max_len + s.splits - 1) / s.splits;
     return s;
 }
 
@@ -1360,7 +1473,7 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     a.mask_words = x->mask_words; a.n_seq = x->n_seq; a.n_tok = x->n_tok;
     a.H = c->n_head_kv; a.G = x->n_head / c->n_head_kv; a.dk = c->d_k; a.dv = c->d_v;
     a.shift = __builtin_ctz(c->page_size); a.n_pages = c->n_pages; a.max_seqs = c->max_seqs; a.max_pages = c->max_pages;
-    a.splits = s.splits; a.tiles = s.tiles;
+    a.splits = s.splits; a.range = s.range; a.tiles = s.tiles;
     a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)c->d_k);
     a.part_o = static_cast<float *>(ws);
     a.part_ml = a.part_o + (size_t)s.splits * x->n_tok * x->n_head * c->d_v;
@@ -1369,7 +1482,9 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    if (!(s.whole ? run_tiles<true>(a, x->type, blocks, st) : run_rows(a, c->k_type, x->type, s.rt, s.careful, blocks, st)))
+    if (!(s.whole == 4   ? run_tiles<true, 4>(a, x->type, blocks, st)
+          : s.whole == 2 ? run_tiles<true, 2>(a, x->type, blocks, st)
+                         : run_rows(a, c->k_type, x->type, s.rt, s.careful, blocks, st)))
         return KV_COMPACT_E_DEVICE;
     if (s.splits > 1) {
         const long long joins = ((long long)x->n_tok * x->n_head + 3) / 4;
@@ -1410,14 +1525,14 @@ int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
     const bool careful = !vec_rows(x->q, es) || !vec_rows(x->k, es) || !vec_rows(x->v, es) || x->d_k * es % 16 ||
                          x->d_v * es % 16;
     const bool whole = x->type != kF32 && !careful && vec_rows(x->o, es);
-    const int rt = row_tiles(head_tile(x->d_k, x->d_v), careful, (long long)x->n_tok * G);
+    const int rt = row_tiles(x->type, head_tile(x->d_k, x->d_v), careful, (long long)x->n_tok * G);
     const int block_rows = whole ? 128 : 16 * rt;
     const long long tiles = ((long long)x->n_tok * G + block_rows - 1) / block_rows + x->n_seq;
     if (tiles * a.H > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    return (whole ? run_tiles<false>(a, x->type, tiles * a.H, st)
+    return (whole ? run_tiles<false, 4>(a, x->type, tiles * a.H, st)
                   : run_rows(a, x->type, x->type, rt, careful, tiles * a.H, st))
                ? 0
                : KV_COMPACT_E_DEVICE;
