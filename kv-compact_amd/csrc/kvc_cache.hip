@@ -137,6 +137,27 @@ __device__ int grant(const Pages & c, int n, int need, int * list, int * lds, in
     return need < 0 ? -1 : at;
 }
 
+// The pages of all requests as one list: first[r] is where request r's count[r]
+// pages begin (in `first`), *total their number. A bookkeeping call is a chain
+// of loads, and a thread per page makes it one chain for all requests.
+__device__ const int * page_pairs(const int * count, int * first, int * lds, int * total) {
+    const int i = threadIdx.x;
+    const int at = block_scan(count[i], lds, total);
+    first[i] = at;
+    __syncthreads();
+    return first;
+}
+// the request of entry x: the last one that begins at or before it
+__device__ int request_of(const int * first, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 // seqs[i], or -1 when out of range or named by an earlier request
 __device__ int request_seq(const Pages & c, int n, const int * seqs, int * ids) {
     const int i = threadIdx.x;
@@ -171,8 +192,7 @@ __global__ __launch_bounds__(256) void k_cache_reset(Pages c) {
 // shared; that page's cells become a move job (identity, the old page in
 // saved[job][0]).
 __global__ __launch_bounds__(kPlan) void k_cache_extend(Pages c, int n, const int * seqs, const int * count,
-                                                        int * status, int * n_jobs, Job * jobs, int * saved,
-                                                        int * list) {
+                                                        int * status, Job * jobs, int * saved, int * list) {
     __shared__ int lds[kWaves], ids[kPlan], slots[kPlan], r_col[kPlan], r_need[kPlan], r_at[kPlan];
     const int i = threadIdx.x;
     const int page = 1 << c.shift;
@@ -205,32 +225,30 @@ __global__ __launch_bounds__(kPlan) void k_cache_extend(Pages c, int n, const in
     r_at[i] = at;
     r_col[i] = (int)(((long long)old + page - 1) >> c.shift) - copied;
     ids[i] = seq;
-    int total;
-    const int job = block_scan(done && copied, lds, &total);
-    if (i < n) status[i] = done ? 0 : (missing ? missing : KVC_REQ_BAD);
-    if (done) {
-        if (copied) {
-            const int first = old & ~(page - 1);
-            jobs[job] = Job{seq, first, old, 0, 0, old, 1};
-            saved[(long long)job * c.max_pages] = last;
+    if (i < n) {
+        status[i] = done ? 0 : (missing ? missing : KVC_REQ_BAD);
+        Job j{};
+        if (done && copied) {
+            j = Job{seq, old & ~(page - 1), old, 0, 0, old, 1};
+            saved[(long long)i * c.max_pages] = last;
             atomicSub(&c.refs[last], 1);
         }
-        c.len[seq] = old + add;
+        jobs[i] = j;
+        if (done && add) c.len[seq] = old + add;
     }
-    if (i == 0) *n_jobs = total;
     __syncthreads();
-    for (int r = i >> 6; r < n; r += kWaves) {
-        const int k = r_need[r];
-        for (int j = lane_id(); j < k; j += 64) {
-            const int p = list[r_at[r] + j];
-            c.table[(long long)ids[r] * c.max_pages + r_col[r] + j] = p;
-            c.refs[p] = 1;
-        }
+    int total;
+    const int * first = page_pairs(r_need, slots, lds, &total);
+    for (int x = i; x < total; x += kPlan) {
+        const int r = request_of(first, n, x), j = x - first[r];
+        const int p = list[r_at[r] + j];
+        c.table[(long long)ids[r] * c.max_pages + r_col[r] + j] = p;
+        c.refs[p] = 1;
     }
 }
 
 __global__ __launch_bounds__(kPlan) void k_cache_fork(Pages c, int n, const int * src, const int * dst, int * status) {
-    __shared__ int ids[kPlan], from[kPlan], held[kPlan];
+    __shared__ int lds[kWaves], ids[kPlan], from[kPlan], held[kPlan], at[kPlan];
     const int i = threadIdx.x;
     const int to = request_seq(c, n, dst, ids);
     int a = -1, cells = 0;
@@ -240,44 +258,40 @@ __global__ __launch_bounds__(kPlan) void k_cache_fork(Pages c, int n, const int 
         if (a == to || cells < 0 || cells > ((long long)c.max_pages << c.shift) || c.len[to] != 0) a = -1;
     }
     from[i] = a;
-    held[i] = a >= 0 ? cells : 0;
+    held[i] = a >= 0 ? (int)(((long long)cells + (1 << c.shift) - 1) >> c.shift) : 0;
     ids[i] = to;
     __syncthreads();
     if (i < n) status[i] = a >= 0 ? 0 : KVC_REQ_BAD;
     if (a >= 0) c.len[to] = cells;
     // (a source that this call fills was empty before it: no page of it is read)
-    for (int r = i >> 6; r < n; r += kWaves) {
-        if (from[r] < 0) continue;
-        const int k = (int)(((long long)held[r] + (1 << c.shift) - 1) >> c.shift);
-        const int * t = c.table + (long long)from[r] * c.max_pages;
-        int * u = c.table + (long long)ids[r] * c.max_pages;
-        for (int j = lane_id(); j < k; j += 64) {
-            const int p = t[j];
-            u[j] = p;
-            if (good_page(c, p)) atomicAdd(&c.refs[p], 1);
-        }
+    int total;
+    const int * first = page_pairs(held, at, lds, &total);
+    for (int x = i; x < total; x += kPlan) {
+        const int r = request_of(first, n, x), j = x - first[r];
+        const int p = c.table[(long long)from[r] * c.max_pages + j];
+        c.table[(long long)ids[r] * c.max_pages + j] = p;
+        if (good_page(c, p)) atomicAdd(&c.refs[p], 1);
     }
 }
 
 __global__ __launch_bounds__(kPlan) void k_cache_free(Pages c, int n, const int * seqs) {
-    __shared__ int ids[kPlan], held[kPlan];
+    __shared__ int lds[kWaves], ids[kPlan], held[kPlan], at[kPlan];
     const int i = threadIdx.x;
     const int seq = request_seq(c, n, seqs, ids);
     const int cells = seq >= 0 ? c.len[seq] : 0;
     ids[i] = seq;
-    held[i] = cells < 0 ? 0 : cells;
+    const long long pages = cells <= 0 ? 0 : ((long long)cells + (1 << c.shift) - 1) >> c.shift;
+    held[i] = pages < c.max_pages ? (int)pages : c.max_pages;
     __syncthreads();
     if (seq >= 0) c.len[seq] = 0;
-    for (int r = i >> 6; r < n; r += kWaves) {
-        if (ids[r] < 0) continue;
-        long long k = ((long long)held[r] + (1 << c.shift) - 1) >> c.shift;
-        if (k > c.max_pages) k = c.max_pages;
-        int * t = c.table + (long long)ids[r] * c.max_pages;
-        for (int j = lane_id(); j < k; j += 64) {
-            const int p = t[j];
-            t[j] = -1;
-            if (good_page(c, p)) atomicSub(&c.refs[p], 1);
-        }
+    int total;
+    const int * first = page_pairs(held, at, lds, &total);
+    for (int x = i; x < total; x += kPlan) {
+        const int r = request_of(first, n, x);
+        int * t = c.table + (long long)ids[r] * c.max_pages + (x - first[r]);
+        const int p = *t;
+        *t = -1;
+        if (good_page(c, p)) atomicSub(&c.refs[p], 1);
     }
 }
 
@@ -286,7 +300,7 @@ __global__ __launch_bounds__(kPlan) void k_cache_free(Pages c, int n, const int 
 // move job. saved[r] holds the table before the call from column start/page
 // on, with kShared set where the page is replaced.
 __global__ __launch_bounds__(kPlan) void k_cache_plan_compact(Pages c, int n, const int * seqs, const int * start,
-                                                              const int * cu, int n_idx, int * status, int * n_jobs,
+                                                              const int * cu, int n_idx, int * status,
                                                               Job * jobs, int * saved, int * list) {
     __shared__ int lds[kWaves], ids[kPlan], slots[kPlan], r_first[kPlan], r_written[kPlan], r_held[kPlan],
         r_need[kPlan];
@@ -348,7 +362,6 @@ __global__ __launch_bounds__(kPlan) void k_cache_plan_compact(Pages c, int n, co
         }
         jobs[i] = j;
     }
-    if (i == 0) *n_jobs = n;
     // (every count that decides a page was read before the barrier above)
     __syncthreads();
     for (int r = i >> 6; r < n; r += kWaves) {
@@ -438,11 +451,10 @@ __device__ void cell_places(const Pages & c, const Job & j, const int * saved, c
 // Bound by HBM, or by the latency of one column's chain where a long job moves
 // in place.
 template <class U>
-__global__ __launch_bounds__(256) void k_cache_move(Pages c, const int * n_jobs, const Job * jobs, const int * saved,
+__global__ __launch_bounds__(256) void k_cache_move(Pages c, const Job * jobs, const int * saved,
                                                     Move mv, int col_blocks) {
     __shared__ int src[kCells], dst[kCells];
     const int job = blockIdx.z;
-    if (job >= *n_jobs) return;
     const Job j = jobs[job];
     const int m = j.start - j.first + j.kept;
     if (m <= 0) return;
@@ -521,14 +533,15 @@ __global__ __launch_bounds__(256) void k_cache_move(Pages c, const int * n_jobs,
 // Row r of the call's packed rows: its sequence's cell, as a row of the pool
 // (page * page_size + cell), or -1. All threads; the answer for the block's
 // rows r0 .. r0+kRows-1 in place[].
+// (rows: of a block, at most kRows)
 constexpr int kRows = 8;
-__device__ void new_row_places(const Pages & c, int n, const int * seqs, const int * cu, int r0, int n_rows, int * place) {
+__device__ void new_row_places(const Pages & c, int n, const int * seqs, const int * cu, int r0, int rows, int n_rows, int * place) {
     if (threadIdx.x < kRows) place[threadIdx.x] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const int a = cu[i], b = cu[i + 1];
         const int lo = a > r0 ? a : r0;
-        int hi = b < r0 + kRows ? b : r0 + kRows;
+        int hi = b < r0 + rows ? b : r0 + rows;
         if (hi > n_rows) hi = n_rows;
         if (lo >= hi) continue;
         const int s = seqs[i];
@@ -550,17 +563,18 @@ struct RowSource {
     long long ld_layer, ld_row;
 };
 
-// New rows of the cache's own type: blocks of kRows rows of one layer.
+// New rows of the cache's own type: blocks of `rows` rows of one layer.
 template <class U>
 __global__ __launch_bounds__(256) void k_cache_write(Pages c, int layer0, int n, const int * seqs, const int * cu,
-                                                     int n_rows, RowSource k, RowSource v) {
+                                                     int n_rows, int rows, RowSource k, RowSource v) {
     __shared__ int place[kRows];
-    const int r0 = blockIdx.x * kRows, layer = layer0 + blockIdx.y;
-    new_row_places(c, n, seqs, cu, r0, n_rows, place);
+    const int r0 = blockIdx.x * rows, layer = layer0 + blockIdx.y;
+    new_row_places(c, n, seqs, cu, r0, rows, n_rows, place);
     const int kc = (int)(c.krow / (int)sizeof(U)), vc = (int)(c.vrow / (int)sizeof(U));
     const long long base = (long long)layer * c.n_pages << c.shift;
-    for (long long w = threadIdx.x; w < (long long)kRows * (kc + vc); w += 256) {
-        const int e = (int)(w / (kc + vc)), x = (int)(w % (kc + vc));
+#pragma unroll 4
+    for (unsigned w = threadIdx.x; w < (unsigned)rows * (unsigned)(kc + vc); w += 256) {
+        const int e = (int)(w / (unsigned)(kc + vc)), x = (int)(w % (unsigned)(kc + vc));
         if (place[e] < 0) continue;
         const bool is_v = x >= kc;
         const RowSource & s = is_v ? v : k;
@@ -571,7 +585,7 @@ __global__ __launch_bounds__(256) void k_cache_write(Pages c, int layer0, int n,
         *reinterpret_cast<U *>(to + (long long)col * (int)sizeof(U)) = val;
     }
     if (c.bias)
-        for (int w = threadIdx.x; w < kRows * c.H; w += 256) {
+        for (int w = threadIdx.x; w < rows * c.H; w += 256) {
             const int p = place[w / c.H], h = w % c.H;
             if (p >= 0)
                 c.bias[((((long long)layer * c.n_pages + (p >> c.shift)) * c.H + h) << c.shift) +
@@ -593,7 +607,7 @@ __global__ __launch_bounds__(256) void k_cache_write_q8(Pages c, int layer0, int
                                                         int n_rows, int type, RowSource k, RowSource v) {
     __shared__ int place[kRows];
     const int r0 = blockIdx.x * kRows, layer = layer0 + blockIdx.y;
-    new_row_places(c, n, seqs, cu, r0, n_rows, place);
+    new_row_places(c, n, seqs, cu, r0, kRows, n_rows, place);
     const int kb = (int)(c.krow / 34), vb = (int)(c.vrow / 34);
     const long long base = (long long)layer * c.n_pages << c.shift;
     const int work = kRows * (kb + vb) * 4;
@@ -694,10 +708,9 @@ Pages pages_of(const kvc_cache * c) {
     return p;
 }
 
-// Workspace of extend and compact: the job count, the jobs, each request's
+// Workspace of extend and compact: the jobs, each request's
 // table before the call, the free pages found.
 struct PlanWork {
-    int * n_jobs;
     Job * jobs;
     int * saved;
     int * list;
@@ -712,7 +725,6 @@ PlanWork plan_work(const kvc_cache * c, int n, void * ws) {
         off += (bytes + 255) & ~(size_t)255;
         return q;
     };
-    w.n_jobs = reinterpret_cast<int *>(take(sizeof(int)));
     w.jobs = reinterpret_cast<Job *>(take(sizeof(Job) * n));
     w.saved = reinterpret_cast<int *>(take(sizeof(int) * (size_t)n * c->max_pages));
     w.list = reinterpret_cast<int *>(take(sizeof(int) * (size_t)c->n_pages));
@@ -747,12 +759,12 @@ bool launch_move(const kvc_cache * c, const Pages & p, const PlanWork & w, int n
     parts = parts < most ? parts : most;
     const dim3 grid((unsigned)(col_blocks * (parts > 1 ? parts : 1)), (unsigned)(c->n_layers * kinds), (unsigned)n);
     if (unit == 16)
-        return launch(k_cache_move<U16>, grid, dim3(256), st, p, (const int *)w.n_jobs, (const Job *)w.jobs,
+        return launch(k_cache_move<U16>, grid, dim3(256), st, p, (const Job *)w.jobs,
                       (const int *)w.saved, mv, col_blocks);
     if (unit == 4)
-        return launch(k_cache_move<unsigned>, grid, dim3(256), st, p, (const int *)w.n_jobs, (const Job *)w.jobs,
+        return launch(k_cache_move<unsigned>, grid, dim3(256), st, p, (const Job *)w.jobs,
                       (const int *)w.saved, mv, col_blocks);
-    return launch(k_cache_move<unsigned short>, grid, dim3(256), st, p, (const int *)w.n_jobs, (const Job *)w.jobs,
+    return launch(k_cache_move<unsigned short>, grid, dim3(256), st, p, (const Job *)w.jobs,
                   (const int *)w.saved, mv, col_blocks);
 }
 
@@ -806,7 +818,7 @@ int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * c
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
     const Pages p = pages_of(c);
     // (whole pages are 16-byte aligned, rows of a page may not be)
-    if (!launch(k_cache_extend, dim3(1), dim3(kPlan), st, p, n, seqs, count, status, w.n_jobs, w.jobs, w.saved, w.list) ||
+    if (!launch(k_cache_extend, dim3(1), dim3(kPlan), st, p, n, seqs, count, status, w.jobs, w.saved, w.list) ||
         !launch_move(c, p, w, n, c->page_size, Move{}, unit_of({p.krow, p.vrow}), st))
         return KV_COMPACT_E_DEVICE;
     return 0;
@@ -837,9 +849,12 @@ int kvc_cache_write(const kvc_cache * c, int layer, int n_layers, int n, const i
         ok = launch(k_cache_write_q8, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, src_type, k, v);
     } else {
         const int unit = unit_of({any, p.krow, p.vrow});
-        ok = unit == 16  ? launch(k_cache_write<U16>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, k, v)
-             : unit == 4 ? launch(k_cache_write<unsigned>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, k, v)
-                         : launch(k_cache_write<unsigned short>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, k, v);
+        // eight rows a block find their cells together; two where that would leave CUs idle
+        const int rows = (long long)((n_rows + kRows - 1) / kRows) * n_layers < 1024 ? 2 : kRows;
+        const dim3 grid((unsigned)((n_rows + rows - 1) / rows), (unsigned)n_layers);
+        ok = unit == 16  ? launch(k_cache_write<U16>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, rows, k, v)
+             : unit == 4 ? launch(k_cache_write<unsigned>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, rows, k, v)
+                         : launch(k_cache_write<unsigned short>, grid, dim3(256), st, p, layer, n, seqs, cu, n_rows, rows, k, v);
     }
     return ok ? 0 : KV_COMPACT_E_DEVICE;
 }
@@ -894,7 +909,7 @@ int kvc_cache_compact(const kvc_cache * c, int n, const int * seqs, const int * 
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    if (!launch(k_cache_plan_compact, dim3(1), dim3(kPlan), st, p, n, seqs, start, cu, n_idx, status, w.n_jobs, w.jobs,
+    if (!launch(k_cache_plan_compact, dim3(1), dim3(kPlan), st, p, n, seqs, start, cu, n_idx, status, w.jobs,
                 w.saved, w.list))
         return KV_COMPACT_E_DEVICE;
     if (n_idx && !launch_move(c, p, w, n, n_idx, mv, unit_of({any}), st)) return KV_COMPACT_E_DEVICE;
