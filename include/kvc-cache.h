@@ -93,7 +93,10 @@ int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * c
  * becomes 0. K and V rows of src_type: a cache of the same type takes the
  * bytes, a Q8_0 cache also F32, F16 and BF16 rows, encoded as by
  * kv_quantize_row. Row r of layer layer+j at byte j*ld_layer + r*ld_row;
- * both strides multiples of 2 (F32: 4). */
+ * both strides multiples of 2 (F32: 4). n_rows <= 2^24.
+ * The cells are those that the last kvc_cache_extend reserved: a sequence is
+ * forked before it is extended or after its rows are written, not in between
+ * (a write goes to the page as it is, and a shared page is another's too). */
 typedef struct kvc_rows {
     const void * data;
     long long ld_layer, ld_row;   /* bytes */
@@ -139,7 +142,7 @@ int kvc_cache_compact(const kvc_cache * c, int n, const int * seqs, const int * 
 /* Cells start .. start+count-1 of sequence seq, all layers, as contiguous
  * rows: K_out [n_layers][count][k_row bytes], V_out likewise, bias_out
  * [n_layers][n_head_kv][count] (any may be NULL). Cells past the sequence's
- * end read as zero bytes. */
+ * end read as zero bytes. count <= 2^24. */
 int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_out, void * V_out,
                    float * bias_out, void * stream);
 
@@ -151,7 +154,8 @@ int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_
  * the fast ones. n_head is a multiple of n_head_kv: query heads h*g ..
  * h*g+g-1 read KV head h. d_k, d_v from 1 to 256. Sums and softmax statistics
  * are fp32; F16 and BF16 round the softmax weights to that type before the
- * product with V, and the result once. A row that sees no cell gives zeros
+ * product with V (a Q8_0 cache: to fp16), and the result once. At most 2^30
+ * rows (n_tok * n_head) a call. o and lse overlap no input. A row that sees no cell gives zeros
  * and lse -inf. lse = log(sum exp(scale q.k + bias)), float [n_tok][n_head],
  * may be NULL. scale 0: 1/sqrt(d_k). */
 typedef struct kvc_heads {

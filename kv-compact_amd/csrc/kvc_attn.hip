@@ -107,6 +107,11 @@ template <int TYPE> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
+// loads from 2-byte boundaries (one instruction each: the memory takes any address)
+typedef u4 u4_any __attribute__((aligned(2)));
+typedef u2 u2_any __attribute__((aligned(2)));
+typedef unsigned u1_any __attribute__((aligned(2)));
+
 // How the columns of a row are read: FULL the heads are as wide as the form,
 // PART rows are 16-byte aligned and heads whole vectors, ANY element by element.
 enum Columns { FULL, PART, ANY };
@@ -238,9 +243,6 @@ __device__ __forceinline__ void load_lds4(const char * from, char * to) {
 template <int N> __device__ __forceinline__ void wait_lds_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
-
-typedef u2 u2_any __attribute__((aligned(2)));
-typedef unsigned u1_any __attribute__((aligned(2)));
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 // Two signed bytes, chosen by `pick` (as v_perm: 0-3 of b, 4-7 of a; the other
@@ -407,9 +409,14 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
             const char * p = a.q + ((long long)(tok0 + tok[r]) * a.q_tok + (long long)(h * a.G + head[r]) * a.q_head) * C::ES;
 #pragma unroll
             for (int j = 0; j < C::NK; j++) {
-                unsigned w[4];
-                load_cols<C::KV, C::ES, COLS>(p, 0, 4 * C::KV * j + C::KV * g, a.dk, w);
-                q[r][j] = u4{w[0], w[1], w[2], w[3]};
+                const int col = 4 * C::KV * j + C::KV * g;
+                if constexpr (Q8) {   // (the cache is aligned, the queries may not be)
+                    q[r][j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
+                } else {
+                    unsigned w[4];
+                    load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, w);
+                    q[r][j] = u4{w[0], w[1], w[2], w[3]};
+                }
             }
             if constexpr (Q8 && QT == kBF16) {
                 // the largest of the row to 2^14 (eight bits of it: exact; others from 2^-28 of it on)
@@ -936,6 +943,7 @@ void k_attn_tiles(AttnArgs a) {
     constexpr int LOADS = 2 * NL + (CELLS ? 1 : 0);         // of a wave and tile
     constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f, log2_lift = TYPE == kF16 ? 10.0f : 0.0f;
     __shared__ __align__(16) char lds[BUFS][2][BK * ROWB];  // [buffer][K, V]
+    static_assert(KW == 1 || RW * (DT * 4 + 1) * 64 * 16 <= BUFS * 2 * BK * ROWB, "parts handed over fit the tiles");
     __shared__ __align__(16) float cells[BUFS][CELLS ? BK : 1];   // bias of each cell; -inf: hidden from every row
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1415,6 +1423,10 @@ template <bool CELLS, int RW> bool run_tiles(const AttnArgs & a, int type, long 
 
 int esize(int type) { return type == kF32 ? 4 : 2; }
 
+// Row numbers stay clear of 2^31 with a tile added, and a launch has fewer than
+// 2^32 threads (blocks of 512 at most).
+constexpr long long kMaxRows = 1 << 30, kMaxBlocks = (1 << 23) - 1;
+
 // Shape of a cache call's launch.
 struct CacheShape {
     int rt, tiles, splits, range;
@@ -1428,7 +1440,7 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
     const long long rows = (long long)a->max_new * G;
     s.rt = row_tiles(c->k_type, head_tile(c->d_k, c->d_v), s.careful, rows);
-    if (rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es)) 
+    if (rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es))
         s.whole = rows > 64 && c->d_k <= 128 && c->d_v <= 128 ? 4 : 2;
     const int block_rows = s.whole ? 32 * s.whole : 16 * s.rt;
     const long long tiles = (rows + block_rows - 1) / block_rows;
@@ -1440,6 +1452,7 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles, blocks = s.whole || s.rt == 4 ? 1024 : 4096;
     long long want = (blocks + units - 1) / units, most = a->max_len / 256;
     want = want < most ? want : most;
+    if ((long long)a->n_tok * a->n_head > 1 << 24) want = 1;   // (the join's launch: a block a row or four; so many need no ranges)
     s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
     s.range = s.rt == 4 ? 0 : (a->max_len + s.splits - 1) / s.splits;
     return s;
@@ -1451,6 +1464,8 @@ int check_cache_attn(const kvc_cache * c, const kvc_cache_attn_args * a) {
     if (a->n_seq < 0 || a->n_tok < 0 || a->n_head <= 0 || a->max_new < 0 || a->max_len < 0 || a->mask_words < 0 ||
         a->layer < 0 || a->layer >= c->n_layers || a->n_head % c->n_head_kv)
         return -2;
+    if ((long long)a->n_tok * a->n_head > kMaxRows || (long long)a->max_new * (a->n_head / c->n_head_kv) > kMaxRows)
+        return KV_COMPACT_E_UNSUPPORTED;
     if (c->k_type != c->v_type) return KV_COMPACT_E_UNSUPPORTED;
     if (c->k_type == kQ8 ? a->type != kF16 && a->type != kBF16 : a->type != c->k_type) return KV_COMPACT_E_UNSUPPORTED;
     return 0;
@@ -1465,7 +1480,7 @@ using namespace kvc;
 extern "C" {
 
 size_t kvc_attn_cache_workspace(const kvc_cache * c, const kvc_cache_attn_args * a) {
-    if (check_cache_attn(c, a)) return 0;
+    if (check_cache_attn(c, a) || a->n_seq == 0 || a->n_tok == 0) return 0;
     const CacheShape s = cache_shape(c, a);
     return s.splits > 1 ? (size_t)s.splits * a->n_tok * a->n_head * (c->d_v + 2) * sizeof(float) : 0;
 }
@@ -1503,7 +1518,7 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     a.part_o = static_cast<float *>(ws);
     a.part_ml = a.part_o + (size_t)s.splits * x->n_tok * x->n_head * c->d_v;
     const long long blocks = (long long)x->n_seq * s.tiles * s.splits * a.H;
-    if (blocks > 0x7fffffffll || (long long)x->n_tok * x->n_head > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
+    if (blocks > kMaxBlocks) return KV_COMPACT_E_UNSUPPORTED;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
@@ -1523,7 +1538,7 @@ int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
     if (x->n_seq < 0 || x->n_tok < 0 || x->n_head <= 0 || x->n_head_kv <= 0 || x->d_k <= 0 || x->d_v <= 0 ||
         x->n_head % x->n_head_kv)
         return -2;
-    if (x->d_k > 256 || x->d_v > 256 || (x->type != kF32 && x->type != kF16 && x->type != kBF16))
+    if ((long long)x->n_tok * x->n_head > kMaxRows || x->d_k > 256 || x->d_v > 256 || (x->type != kF32 && x->type != kF16 && x->type != kBF16))
         return KV_COMPACT_E_UNSUPPORTED;
     if (x->n_seq == 0 || x->n_tok == 0) return 0;
     if (!x->q.data || !x->k.data || !x->v.data || !x->o.data || !x->cu) return -1;
@@ -1549,7 +1564,7 @@ int kvc_attn_prompt(const kvc_prompt_args * x, void * stream) {
     const int rt = row_tiles(x->type, head_tile(x->d_k, x->d_v), careful, (long long)x->n_tok * G);
     const int block_rows = whole ? 128 : 16 * rt;
     const long long tiles = ((long long)x->n_tok * G + block_rows - 1) / block_rows + x->n_seq;
-    if (tiles * a.H > 0x7fffffffll) return KV_COMPACT_E_UNSUPPORTED;
+    if (tiles * a.H > kMaxBlocks) return KV_COMPACT_E_UNSUPPORTED;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;

@@ -25,6 +25,7 @@ constexpr int kPlan = 1024;               // threads of a bookkeeping block
 constexpr int kWaves = kPlan / 64;
 constexpr int kShared = 1 << 30;          // saved table entry: the page has other holders
 constexpr int kMaxPages = 1 << 20;
+constexpr int kMaxRows = 1 << 24;          // of a write or read: row numbers and a launch's threads stay in range
 
 // Arrays and shapes of a cache as kernels take them.
 struct Pages {
@@ -829,6 +830,7 @@ int kvc_cache_write(const kvc_cache * c, int layer, int n_layers, int n, const i
     if (int rc = check_cache(c)) return rc;
     if (int rc = check_requests(n)) return rc;
     if (layer < 0 || n_layers < 0 || n_rows < 0 || layer > c->n_layers - n_layers) return -2;
+    if (n_rows > kMaxRows) return KV_COMPACT_E_UNSUPPORTED;
     if (n == 0 || n_layers == 0 || n_rows == 0) return 0;
     if (!seqs || !cu || !K || !V || !K->data || !V->data) return -1;
     const bool encode = src_type != KV_TYPE_Q8_0 && c->k_type == KV_TYPE_Q8_0 && c->v_type == KV_TYPE_Q8_0 &&
@@ -920,7 +922,7 @@ int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_
                    void * stream) {
     if (int rc = check_cache(c)) return rc;
     if (seq < 0 || seq >= c->max_seqs || start < 0 || count < 0) return -2;
-    if (bias_out && !c->bias) return KV_COMPACT_E_UNSUPPORTED;
+    if (count > kMaxRows || (bias_out && !c->bias)) return KV_COMPACT_E_UNSUPPORTED;
     if (count == 0 || (!K_out && !V_out && !bias_out)) return 0;
     if ((reinterpret_cast<uintptr_t>(K_out) | reinterpret_cast<uintptr_t>(V_out)) & 1) return KV_COMPACT_E_UNSUPPORTED;
     const hipStream_t st = static_cast<hipStream_t>(stream);

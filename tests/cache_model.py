@@ -232,7 +232,7 @@ def attend(q, k, v, seen, bias, scale, typ, split_kv=False):
     """fp64 attention of one sequence: q [N][Hq][dk], k [M][H][dk], v [M][H][dv], seen [N][M], bias [H][M] or None.
 
     Returns o, lse and how far each may be off. With u the half step of the type (2^-24, 2^-11, 2^-8) and e = 2^-24:
-      a score is off by at most e (dk + 4) scale sum |q||k| (sums of dk products in fp32, the scale, the bias) and
+      a score is off by at most e (dk + 4) |scale| sum |q||k| (sums of dk products in fp32, the scale, the bias) and
       its weight's exponent by 2 e max |s - m|: together ds, so a weight by 2 ds + 4 e relative (exp and the
       running rescales; ds is small);
       weights are rounded by u (16-bit types; sums of M of them by M e), and the result by u.
@@ -254,7 +254,7 @@ def attend(q, k, v, seen, bias, scale, typ, split_kv=False):
             if not len(j):
                 continue
             s = (k[j, g] @ q[i, h]) * scale
-            mag = (np.abs(k[j, g]) @ np.abs(q[i, h])) * scale
+            mag = (np.abs(k[j, g]) @ np.abs(q[i, h])) * abs(scale)   # (a size: a negative scale has the same)
             if bias is not None:
                 s = s + bias[g, j]
                 mag = mag + np.abs(bias[g, j])

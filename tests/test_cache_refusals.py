@@ -190,3 +190,24 @@ def test_struct_sizes():
     # include/kvc-cache.h on x86-64
     assert [ctypes.sizeof(x) for x in (kc.KvCache, kc.Rows, kc.Values, kc.Betas, kc.Heads, kc.PromptArgs,
                                        kc.CacheAttnArgs)] == [88, 24, 32, 24, 24, 144, 120]
+
+
+def test_sizes_at_the_ends(dll):
+    # nothing to do needs no workspace, and rows, cells and blocks stay within what the kernels count with
+    c, top, h = cache(), (1 << 31) - 1, kc.Heads(FAKE, 256, 64)
+    for kw in (dict(n_seq=0), dict(n_tok=0), dict(n_seq=0, n_tok=0, max_new=0, max_len=0)):
+        assert dll.kvc_attn_cache_workspace(c, attn(**kw)) == 0
+        assert dll.kvc_attn_cache(c, attn(**kw), None, 0, None) == 0
+    size = 1 << 62
+    for kw, code in ((dict(n_tok=top), -5), (dict(n_tok=(1 << 28) + 1), -5), (dict(max_new=top), -5),
+                     (dict(n_tok=1 << 28), kc.E_DEVICE), (dict(max_len=top), kc.E_DEVICE), (dict(n_seq=top), -5)):
+        assert dll.kvc_attn_cache(c, attn(**kw), FAKE, size, None) == code, kw
+    for kw, code in ((dict(n_tok=top), -5), (dict(n_tok=(1 << 28) + 1), -5), (dict(n_seq=top), -5),
+                     (dict(n_tok=1 << 22), kc.E_DEVICE)):
+        d = dict(q=h, k=h, v=h, o=h, lse=None, cu=FAKE, type=F16, n_seq=2, n_tok=9, n_head=4, n_head_kv=2, d_k=64, d_v=64)
+        d.update(kw)
+        assert dll.kvc_attn_prompt(kc.PromptArgs(**d), None) == code, kw
+    r = kc.Rows(FAKE, 0, 256)
+    for n, code in ((top, -5), ((1 << 24) + 1, -5), (1 << 24, kc.E_DEVICE)):
+        assert dll.kvc_cache_write(c, 0, 1, 2, FAKE, FAKE, n, F16, r, r, None) == code
+        assert dll.kvc_cache_read(c, 0, 0, n, FAKE, FAKE, FAKE, None) == code

@@ -409,3 +409,70 @@ def test_wide_ranges_of_values(dll, typ, cache):
         v *= np.exp2(np.random.default_rng(1).integers(-10, 11, v.shape[:3]))[..., None]
         k *= np.exp2(np.random.default_rng(2).integers(-10, 3, k.shape[:3]))[..., None]
     run_cells(dll, typ, cache, [200], [3], 2, 2, 128, 128, page=32, seed=11, edit=edit)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [64, 256])
+def test_negative_scale(dll, typ, d):
+    # the largest score is then that of the smallest product
+    run_prompt(dll, typ, [5, 140], 1, 2, d, d, seed=20, scale=-0.1)
+    run_cells(dll, typ, typ, [150, 30], [3, 1], 1, 2, d, d, tree=True, bias=True, seed=21, scale=-0.1)
+    run_cells(dll, typ, typ, [190, 80], [70, 40], 1, 2, d, d, tree=True, words=2, seed=22, scale=-0.1)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+def test_many_prompts(dll, typ):
+    # more sequences than a wave has lanes, empty ones among them
+    run_prompt(dll, typ, [(7 * i) % 5 * 9 for i in range(150)], 1, 2, 64, 64, seed=23, first=2, tail=3)
+
+
+@pytest.mark.parametrize("typ,cache", [(F16, F16), (BF16, Q8_0)])
+def test_many_sequences(dll, typ, cache):
+    run_cells(dll, typ, cache, [1 + 11 * i % 60 for i in range(150)], [1 + i % 2 if 1 + 11 * i % 60 > 1 else 1 for i in range(150)],
+              1, 2, 64, 64, seed=24, bias=True)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+@pytest.mark.parametrize("d,said", [(64, 17), (64, 40), (96, 17), (96, 40), (128, 40), (256, 17), (256, 40), (200, 40)])
+def test_trees_of_several_row_tiles(dll, typ, d, said):
+    # a block that takes several tiles of rows, one after the other, where more tokens come than were announced; heads
+    # narrower than the form; what the next row tile finds in LDS
+    run_cells(dll, typ, typ, [700, 290, 200], [140, 129, 3], 2, 2, d, d, page=32, bias=d != 96, tree=True, words=3, seed=d + said,
+              max_new=said, max_len=200, runs=2)
+
+
+@pytest.mark.parametrize("typ,cache", KINDS)
+@pytest.mark.parametrize("G", [7, 40, 100])
+def test_large_groups(dll, typ, cache, G):
+    run_cells(dll, typ, cache, [300, 20, 5], [1, 2, 3], 1, G, 64, 64, tree=True, seed=G)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,G", [(12, 1), (12, 2), (10, 4), (20, 4)])
+def test_q8_rows_that_are_not_finite(dll, typ, d, n, G):
+    # scales of drafted tokens that are not finite, or far from one, with few and many rows
+    def edit(q, k, v, b, cell):
+        for j, x in ((101, 1e-7), (102, 2e3), (103, 2.0 ** -20), (105, 1e8)):
+            p, c = cell(0, j)
+            v[p, c, 0, :32] *= x
+    run_cells(dll, typ, Q8_0, [100 + n], [n], 1, G, d, d, tree=True, bias=True, seed=d + n, edit=edit)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+@pytest.mark.parametrize("G", [1, 3, 12])
+def test_q8_queries_of_any_alignment(dll, typ, G):
+    run_cells(dll, typ, Q8_0, [100, 45], [7, 1], 2, G, 96, 64, bias=True, tree=True, seed=25, pad=1, shift=1)
+    run_cells(dll, typ, Q8_0, [100, 45], [7, 1], 1, G, 128, 128, seed=26, pad=3, shift=1)
+
+
+@pytest.mark.parametrize("typ,cache", KINDS)
+def test_nothing_announced(dll, typ, cache):
+    # max_new and max_len 0; a sequence without cells beside others; one without tokens
+    run_cells(dll, typ, cache, [40, 0, 9], [40, 0, 0], 2, 2, 64, 64, seed=27, max_new=0, max_len=0)
+
+
+@pytest.mark.parametrize("typ,cache", KINDS)
+def test_the_same_sequence_twice(dll, typ, cache):
+    # (reads only: each entry sees the whole sequence)
+    run_cells(dll, typ, cache, [90, 90, 50], [3, 3, 3], 1, 2, 64, 64, seed=28, seqs=[2, 2, 0])
