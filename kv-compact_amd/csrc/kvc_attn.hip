@@ -895,7 +895,8 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // Many rows: 32 of them a wave, RW waves of rows (32 RW rows a block), over
 // tiles of 64 keys that all waves read from LDS. KW = 2: half of the waves
 // take the first 32 keys of each tile, half the others, and they join at the
-// end.
+// end (over a cache); or, PAIR, they swap their weights through LDS in every
+// tile, and each sums half of the columns (prompts of heads wider than 128).
 //
 // Fragments (32x32x16, lane l, n = l % 32, h = l / 32): an operand's lane holds
 // row n and elements 8h .. 8h+7 of the summed axis; a result's lane column n
@@ -912,9 +913,21 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // half a fragment of V^T. Pieces past a head's width stay zero.
 //
 // A prompt's blocks are four waves, two of them on a CU: one's softmax runs
-// under the other's products, and K and V come from L2 (one tile ahead). Over
-// a cache HBM has to be kept busy: eight waves share four buffers (RW = 4: 96
-// KB on their way), or two blocks of four waves two buffers each (RW = 2).
+// under the other's products, and K and V come from L2 (one tile ahead). They
+// are bound by what issues beside the products: 16384 tokens of 32 heads of 128
+// take 2.27 ms, 971 TFLOP/s (85 % of a large matrix product's rate; 2.36 ms
+// with one loop for plain and masked tiles), 12 prompts of as many in all 0.57 ms.
+// At 256 columns a wave's sums and queries alone are 192 registers, which
+// leaves one wave a SIMD and a third of its instructions moves between the
+// halves of the file: 5003 tokens in three prompts of 8 heads took 132 us that
+// way and take 89 us in pairs (128 + 16 KB of LDS, one block a CU; bound by the
+// longest prompt's chain of tiles, which three barriers a tile stretch).
+//
+// Over a cache HBM has to be kept busy: eight waves share four buffers (RW = 4:
+// 96 KB on their way), or two blocks of four waves two buffers each (RW = 2).
+// Eight sequences of up to 20000 F16 cells, 8 x 128, with 32 drafts of 32 heads
+// take 163 us, 2.6 TB/s; bound by the last blocks of ragged sequences and by a
+// step's latency, 2.2 us where its loads alone would take 1.7.
 __device__ const unsigned zero_word = 0;
 __device__ const unsigned hidden_word = 0xff800000u;   // -inf
 
@@ -930,12 +943,17 @@ template <int TYPE> __device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
 
 __device__ __forceinline__ float pair_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
 
+// KW: halves of a tile's keys that waves share out
+constexpr int tile_halves(bool cells, int d) { return cells || d == 256 ? 2 : 1; }
+
 template <int TYPE, int D, bool CELLS, int RW>
-__global__ __launch_bounds__(64 * RW * (CELLS ? 2 : 1), CELLS && RW == 4 && D < 256 ? 2 : D == 256 ? 1 : 2)
+__global__ __launch_bounds__(64 * RW * tile_halves(CELLS, D), CELLS && D == 256 ? 1 : 2)
 void k_attn_tiles(AttnArgs a) {
-    constexpr int KW = CELLS ? 2 : 1, WAVES = RW * KW, ROWS = 32 * RW;
-    constexpr int BK = !CELLS && D == 256 ? 32 : 64, SUB = BK / 32 / KW;   // keys of a tile; of a wave, in parts of 32
-    constexpr int KS = D / 16, DT = D / 32, CH = D / 8;     // steps of a score, column tiles, pieces of a row
+    constexpr bool PAIR = !CELLS && D == 256;               // two waves share their rows' weights, and halve the columns
+    constexpr int KW = tile_halves(CELLS, D), WAVES = RW * KW, ROWS = 32 * RW;
+    constexpr int BK = 64, SUB = BK / 32 / KW;              // keys of a tile; of a wave's scores, in parts of 32
+    constexpr int KS = D / 16, DT = D / 32 / (PAIR ? 2 : 1), CH = D / 8;   // steps of a score, column tiles, pieces of a row
+    constexpr int PV = PAIR ? 2 : SUB;                      // parts of 32 keys in a wave's second product
     constexpr int NL = BK * CH / (64 * WAVES);              // direct loads of a wave and tile, K or V
     constexpr int KPL = 512 / D;                            // keys of one: rows of one 16-cell group
     constexpr int BUFS = CELLS && RW == 4 && D < 256 ? 4 : 2, AHEAD = BUFS - 1;
@@ -943,12 +961,21 @@ void k_attn_tiles(AttnArgs a) {
     constexpr int LOADS = 2 * NL + (CELLS ? 1 : 0);         // of a wave and tile
     constexpr float lift = TYPE == kF16 ? 0x1p10f : 1.0f, log2_lift = TYPE == kF16 ? 10.0f : 0.0f;
     __shared__ __align__(16) char lds[BUFS][2][BK * ROWB];  // [buffer][K, V]
-    static_assert(KW == 1 || RW * (DT * 4 + 1) * 64 * 16 <= BUFS * 2 * BK * ROWB, "parts handed over fit the tiles");
+    static_assert(KW == 1 || PAIR || RW * (DT * 4 + 1) * 64 * 16 <= BUFS * 2 * BK * ROWB, "parts handed over fit the tiles");
+    __shared__ __align__(16) u4 swap[PAIR ? WAVES : 1][2][64];     // a wave's weights, lane for lane
+    __shared__ float swap_top[PAIR ? WAVES : 1][64];
     __shared__ __align__(16) float cells[BUFS][CELLS ? BK : 1];   // bias of each cell; -inf: hidden from every row
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rw = wave % RW, kw = wave / RW;
     const int n = lane & 31, hf = lane >> 5;
+    const int other = PAIR ? rw + RW * (1 - kw) : 0;         // the wave of the same rows
+    const int d0 = PAIR ? DT * kw : 0;                       // column tiles: this one and DT - 1 more
+    auto meet = [] {   // (direct loads stay on their way)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
 
     int u = blockIdx.x;
     const int h = u % a.H;
@@ -1073,7 +1100,9 @@ void k_attn_tiles(AttnArgs a) {
             }
             find_pages(t_lo + AHEAD < t_hi ? t_lo + AHEAD : t_hi - 1);
         }
-        for (int t = t_lo; t < t_hi; t++) {
+        // PLAIN: no key of the tile is hidden from a row of the block
+        auto step = [&](int t, auto kind) {
+            constexpr bool PLAIN = decltype(kind)::value;
             const int buf = (t - t_lo) % BUFS;
             wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
@@ -1082,7 +1111,7 @@ void k_attn_tiles(AttnArgs a) {
             find_pages(t + AHEAD + 1 < t_hi ? t + AHEAD + 1 : t_hi - 1);
             const int part0 = 32 * SUB * kw, key0 = t * BK + part0;   // this wave's keys of the tile
             const char * kt = lds[buf][0] + part0 * ROWB;
-            const char * vt = lds[buf][1] + part0 * ROWB;
+            const char * vt = lds[buf][1] + (PAIR ? 0 : part0 * ROWB);
 
             f16x sc[SUB];
 #pragma unroll
@@ -1114,7 +1143,7 @@ void k_attn_tiles(AttnArgs a) {
                             if (cells[buf][part0 + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3)] == -INFINITY) sc[x][i] = -INFINITY;
                 }
             }
-            if (key0 + 32 * SUB > clear) {
+            if (!PLAIN && key0 + 32 * SUB > clear) {
 #pragma unroll
                 for (int x = 0; x < SUB; x++) {
                     const unsigned see = seen32(a, q, tok, key0 + 32 * x) >> (4 * hf);
@@ -1131,6 +1160,12 @@ void k_attn_tiles(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) top = fmaxf(top, sc[x][i]);
             top = pair_max(top);
+            if constexpr (PAIR) {
+                swap_top[wave][lane] = top;
+                meet();
+                top = fmaxf(top, swap_top[other][lane]);
+                hidden = !PLAIN && t * BK + BK > clear;   // (V of both halves)
+            }
             // weights up to 2^5 are left to grow before the sums are scaled
             if (__ballot((top - mx) * c > 5.0f)) {
                 const float now = fmaxf(mx, top);
@@ -1158,50 +1193,73 @@ void k_attn_tiles(AttnArgs a) {
                     part += p[x][i];
                 }
             sum += part;
-            bool odd = false;
+            u4 pf[PV][2];
 #pragma unroll
             for (int x = 0; x < SUB; x++)
 #pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    u4 pf;
+                for (int st = 0; st < 2; st++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) pf[e] = pack2<TYPE>(p[x][8 * st + 2 * e], p[x][8 * st + 2 * e + 1]);
+                    for (int e = 0; e < 4; e++) pf[x][st][e] = pack2<TYPE>(p[x][8 * st + 2 * e], p[x][8 * st + 2 * e + 1]);
+            if constexpr (PAIR) {   // (the wave's own part first, then the other's)
+                swap[wave][0][lane] = pf[0][0];
+                swap[wave][1][lane] = pf[0][1];
+                meet();
+                pf[1][0] = swap[other][0][lane];
+                pf[1][1] = swap[other][1][lane];
+            }
+            bool odd = false;
+#pragma unroll
+            for (int x0 = 0; x0 < PV; x0++)
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    const int x = PAIR ? x0 ^ kw : x0;
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
                         u2 half[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int r = (lane & 15) >> 2;   // key 4 hf + r of the eight
-                            const int col = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                            const int col = 4 * (d0 + d) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
                             const char * at = vt + (32 * x + 16 * st + 8 * e + 4 * hf + r) * ROWB +
                                               ((col ^ (((4 * hf + r) & VX) << 1)) << 4) + ((lane & 1) << 3);
                             half[e] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                                  (__attribute__((address_space(3))) s4 *)at));
                         }
                         u4 vf = {half[0].x, half[0].y, half[1].x, half[1].y};
-                        if (hidden) {
+                        if (!PLAIN && hidden) {
                             constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
                             for (int y = 0; y < 4; y++) {
                                 const bool lo = (vf[y] & e) == e, hi = (vf[y] >> 16 & e) == e;
                                 // (cells that no row sees, past the end among them, are nothing)
                                 const int kk = 32 * x + 16 * st + 8 * (y >> 1) + 4 * hf + 2 * (y & 1);
-                                if (lo) odd |= CELLS ? cells[buf][part0 + kk] != -INFINITY : key0 + kk < q.held;
-                                if (hi) odd |= CELLS ? cells[buf][part0 + kk + 1] != -INFINITY : key0 + kk + 1 < q.held;
+                                if (lo) odd |= CELLS ? cells[buf][part0 + kk] != -INFINITY : (PAIR ? t * BK : key0) + kk < q.held;
+                                if (hi) odd |= CELLS ? cells[buf][part0 + kk + 1] != -INFINITY : (PAIR ? t * BK : key0) + kk + 1 < q.held;
                                 vf[y] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
                             }
                         }
-                        acc[d] = mfma32<TYPE>(vf, pf, acc[d]);
+                        acc[d] = mfma32<TYPE>(vf, pf[x0][st], acc[d]);
                     }
                 }
-            if (hidden && __ballot(odd)) {
+            if (!PLAIN && hidden && __ballot(odd)) {
                 odd_lo = t < odd_lo ? t : odd_lo;
                 odd_hi = t + 1;
             }
+        };
+        int t = t_lo;
+        if constexpr (!CELLS) {
+            // (a branch around each product would keep it behind its own load of V)
+            const int plain = min((q.base + row0 / a.G + 1) / BK, t_hi);
+            for (; t < plain; t++) step(t, std::true_type{});
         }
+        for (; t < t_hi; t++) step(t, std::false_type{});
         wait_lds_loads<0>();   // (LDS is given up, or used again, with no load to it on its way)
         sum += __shfl_xor(sum, 32);
-        if constexpr (KW == 2) {
+        if constexpr (PAIR) {
+            swap_top[wave][lane] = sum;
+            __syncthreads();
+            sum = kw ? swap_top[other][lane] + sum : sum + swap_top[other][lane];
+        } else if constexpr (KW == 2) {
             // the second half of the waves hands its part over, lane for lane
             f4 * over = reinterpret_cast<f4 *>(lds) + rw * (DT * 4 + 1) * 64 + lane;
             __syncthreads();
@@ -1215,13 +1273,13 @@ void k_attn_tiles(AttnArgs a) {
             }
             __syncthreads();
             if (kw == 0) {
-                const f4 other = over[DT * 4 * 64];
-                const float top = fmaxf(mx, other[0]), use = top == -INFINITY ? 0.0f : top;
-                const float f = __builtin_amdgcn_exp2f((mx - use) * c), g = __builtin_amdgcn_exp2f((other[0] - use) * c);
+                const f4 theirs = over[DT * 4 * 64];
+                const float top = fmaxf(mx, theirs[0]), use = top == -INFINITY ? 0.0f : top;
+                const float f = __builtin_amdgcn_exp2f((mx - use) * c), g = __builtin_amdgcn_exp2f((theirs[0] - use) * c);
                 mx = top;
-                sum = sum * f + other[1] * g;
-                odd_lo = min(odd_lo, __float_as_int(other[2]));
-                odd_hi = max(odd_hi, __float_as_int(other[3]));
+                sum = sum * f + theirs[1] * g;
+                odd_lo = min(odd_lo, __float_as_int(theirs[2]));
+                odd_hi = max(odd_hi, __float_as_int(theirs[3]));
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -1234,7 +1292,7 @@ void k_attn_tiles(AttnArgs a) {
         }
         sum *= 1.0f / lift;
         const long long out = (long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head;
-        const bool write = on && kw == 0;
+        const bool write = on && (PAIR || kw == 0);
         if (CELLS && a.splits > 1) {
             const long long at = (long long)split * a.n_tok * a.H * a.G + out;
             if (write) {
@@ -1242,7 +1300,7 @@ void k_attn_tiles(AttnArgs a) {
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
-                        const int col = 32 * d + 8 * y + 4 * hf;
+                        const int col = 32 * (d0 + d) + 8 * y + 4 * hf;
                         if (col < a.dv && t_lo < t_hi)
                             *reinterpret_cast<f4 *>(a.part_o + at * a.dv + col) =
                                 f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]} * (1.0f / lift);
@@ -1259,13 +1317,13 @@ void k_attn_tiles(AttnArgs a) {
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const int col = 32 * d + 8 * y + 4 * hf;
+                    const int col = 32 * (d0 + d) + 8 * y + 4 * hf;
                     if (col >= a.dv) continue;
                     const u2 v = {pack2<TYPE>(acc[d][4 * y] * inv, acc[d][4 * y + 1] * inv),
                                   pack2<TYPE>(acc[d][4 * y + 2] * inv, acc[d][4 * y + 3] * inv)};
                     *reinterpret_cast<u2 *>(o + 2 * col) = v;
                 }
-            if (a.lse && hf == 0)
+            if (a.lse && hf == 0 && kw == 0)
                 a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS ? mx : mx * scale) + logf(sum);
         }
         if (__builtin_expect(odd_lo < odd_hi, 0) && write && sum == sum) {
@@ -1275,7 +1333,7 @@ void k_attn_tiles(AttnArgs a) {
             Odd<TYPE, TYPE> o{a, q, h, tok, head};
             const float top = (mx == -INFINITY ? 0.0f : mx) * (CELLS ? 1.0f : scale);
 #pragma nounroll
-            for (int col = hf; col < a.dv; col += 2) {
+            for (int col = 32 * d0 + hf; col < a.dv && col < 32 * (d0 + DT); col += 2) {
                 float x = 0.0f;
 #pragma nounroll
                 for (int key = odd_lo * BK; key < odd_hi * BK && key < q.held; key++) x += o.term(key, col, top);
@@ -1289,7 +1347,7 @@ void k_attn_tiles(AttnArgs a) {
             }
         }
         __syncthreads();
-        if (KW == 2 && (long long)(tile + tile_step) * ROWS < rows) {
+        if (KW == 2 && !PAIR && (long long)(tile + tile_step) * ROWS < rows) {
             // (what was handed over stood on pieces that are to be zero)
             for (int i = threadIdx.x; i < BUFS * 2 * BK * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
             __syncthreads();
@@ -1410,7 +1468,7 @@ int row_tiles(int type, int d, bool careful, long long rows) {
 }
 
 template <int TYPE, bool CELLS, int RW> bool run_tiles(const AttnArgs & a, int d, long long blocks, hipStream_t st) {
-    const dim3 grid((unsigned)blocks), block(64 * RW * (CELLS ? 2 : 1));
+    const dim3 grid((unsigned)blocks), block(64 * RW * tile_halves(CELLS, d));
     if (d == 64) return launch(k_attn_tiles<TYPE, 64, CELLS, RW>, grid, block, st, a);
     if (d == 128) return launch(k_attn_tiles<TYPE, 128, CELLS, RW>, grid, block, st, a);
     if constexpr (CELLS && RW == 4) return false;   // (not asked for: eight waves' sums of 256 columns do not fit)

@@ -476,3 +476,18 @@ def test_nothing_announced(dll, typ, cache):
 def test_the_same_sequence_twice(dll, typ, cache):
     # (reads only: each entry sees the whole sequence)
     run_cells(dll, typ, cache, [90, 90, 50], [3, 3, 3], 1, 2, 64, 64, seed=28, seqs=[2, 2, 0])
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 136, 200, 256])
+@pytest.mark.parametrize("G", [1, 3])
+def test_longer_prompts(dll, typ, d, G):
+    # tiles that every row sees whole, then those with hidden keys; values that are not finite in both
+    def edit(q, k, v):
+        v[9, :, 5] = np.inf
+        v[260, 0, d - 1] = -np.inf
+        v[290, :, 7] = np.nan
+        v[400:, :, 3] = np.inf
+        k[299] = np.nan
+    run_prompt(dll, typ, [300, 333, 66], 2, G, d, d, seed=30 + d, edit=edit)
+    run_prompt(dll, typ, [300, 333, 66], 1, G, d, d, seed=31 + d, tail=2)
