@@ -926,7 +926,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // Over a cache HBM has to be kept busy: eight waves share four buffers (RW = 4:
 // 96 KB on their way), or two blocks of four waves two buffers each (RW = 2).
 // Eight sequences of up to 20000 F16 cells, 8 x 128, with 32 drafts of 32 heads
-// take 163 us, 2.6 TB/s; bound by the last blocks of ragged sequences and by a
+// take 157 us, 2.7 TB/s (163 with one loop for plain and masked tiles); bound by the last blocks of ragged sequences and by a
 // step's latency, 2.2 us where its loads alone would take 1.7.
 __device__ const unsigned zero_word = 0;
 __device__ const unsigned hidden_word = 0xff800000u;   // -inf
@@ -1100,15 +1100,18 @@ void k_attn_tiles(AttnArgs a) {
             }
             find_pages(t_lo + AHEAD < t_hi ? t_lo + AHEAD : t_hi - 1);
         }
-        // PLAIN: no key of the tile is hidden from a row of the block
-        auto step = [&](int t, auto kind) {
-            constexpr bool PLAIN = decltype(kind)::value;
-            const int buf = (t - t_lo) % BUFS;
+        // until tile t is there; the next loads go
+        auto arrive = [&](int t) {
             wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            fill(t + AHEAD, (buf + AHEAD) % BUFS);
+            fill(t + AHEAD, (t - t_lo + AHEAD) % BUFS);
             find_pages(t + AHEAD + 1 < t_hi ? t + AHEAD + 1 : t_hi - 1);
+        };
+        // PLAIN: no key of the wave's part of the tile is hidden from one of its rows (!CELLS: of the block's)
+        auto step = [&](int t, auto kind) {
+            constexpr bool PLAIN = decltype(kind)::value;
+            const int buf = (t - t_lo) % BUFS;
             const int part0 = 32 * SUB * kw, key0 = t * BK + part0;   // this wave's keys of the tile
             const char * kt = lds[buf][0] + part0 * ROWB;
             const char * vt = lds[buf][1] + (PAIR ? 0 : part0 * ROWB);
@@ -1126,7 +1129,7 @@ void k_attn_tiles(AttnArgs a) {
             }
             bool hidden = false;   // (uniform) a key that some row does not see
             if constexpr (CELLS) {
-                hidden = __ballot(cells[buf][part0 + (lane & (32 * SUB - 1))] == -INFINITY) != 0;
+                hidden = !PLAIN;
 #pragma unroll
                 for (int x = 0; x < SUB; x++)
 #pragma unroll
@@ -1135,7 +1138,7 @@ void k_attn_tiles(AttnArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) sc[x][4 * y + i] = sc[x][4 * y + i] * scale + b[i];
                     }
-                if (hidden) {   // (whatever the product was)
+                if (!PLAIN) {   // (whatever the product was)
 #pragma unroll
                     for (int x = 0; x < SUB; x++)
 #pragma unroll
@@ -1246,13 +1249,48 @@ void k_attn_tiles(AttnArgs a) {
                 odd_hi = t + 1;
             }
         };
+        // (Loops apart for the two kinds: a branch around each product would keep
+        // it behind its own load of V, two copies of the products in one loop
+        // would each want sums of their own.)
         int t = t_lo;
-        if constexpr (!CELLS) {
-            // (a branch around each product would keep it behind its own load of V)
+        if constexpr (CELLS) {
+            auto whole = [&](int t) {
+                const int part0 = 32 * SUB * kw;
+                return t * BK + part0 + 32 * SUB <= clear &&
+                       __ballot(cells[(t - t_lo) % BUFS][part0 + (lane & (32 * SUB - 1))] == -INFINITY) == 0;
+            };
+            bool plain = false;
+            if (t < t_hi) {
+                arrive(t);
+                plain = whole(t);
+            }
+            while (t < t_hi) {
+                while (t < t_hi && plain) {
+                    step(t, std::true_type{});
+                    if (++t < t_hi) {
+                        arrive(t);
+                        plain = whole(t);
+                    }
+                }
+                while (t < t_hi && !plain) {
+                    step(t, std::false_type{});
+                    if (++t < t_hi) {
+                        arrive(t);
+                        plain = whole(t);
+                    }
+                }
+            }
+        } else {
             const int plain = min((q.base + row0 / a.G + 1) / BK, t_hi);
-            for (; t < plain; t++) step(t, std::true_type{});
+            for (; t < plain; t++) {
+                arrive(t);
+                step(t, std::true_type{});
+            }
+            for (; t < t_hi; t++) {
+                arrive(t);
+                step(t, std::false_type{});
+            }
         }
-        for (; t < t_hi; t++) step(t, std::false_type{});
         wait_lds_loads<0>();   // (LDS is given up, or used again, with no load to it on its way)
         sum += __shfl_xor(sum, 32);
         if constexpr (PAIR) {
