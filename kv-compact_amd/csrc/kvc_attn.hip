@@ -277,6 +277,16 @@ __device__ __forceinline__ float byte_value(const unsigned * w, int i) {
 // (for fp16 results with the remainder as a second term), which is a half step
 // off at most while the scales are between 2^-14 and 2^8; a tile with others
 // multiplies in fp32 (16x16x4).
+//
+// Each key is read once for all rows of its head, straight into the registers
+// the products take it from, a tile ahead. One token of 64 sequences of up to
+// 16384 bf16 cells (8 x 128, 32 heads): 0.50 ms, 5.3 TB/s, HBM's rate. One
+// sequence of 4096 cells: 14 us with the join, two launches and two latencies;
+// of 20000 F32 cells with a bias: 48 us, 3.4 TB/s. Trees of 13 tokens
+// of 32 heads over 16 sequences of up to 32768 Q8_0 cells (8 x 128): 404 us,
+// bound by the instructions that decode codes and scale sums (264 us of issue;
+// four row tiles a wave decode a key once for all 52 rows, and leave one wave a
+// SIMD).
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 struct RowKernel {
     static constexpr int ES = TYPE == kF32 ? 4 : 2;          // bytes of a q element
