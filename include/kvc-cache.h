@@ -86,6 +86,14 @@ size_t kvc_cache_workspace(const kvc_cache * c, int n);
 int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * count, int * status,
                      void * ws, size_t ws_bytes, void * stream);
 
+/* The same, and granted (device int[n], NULL: not wanted) becomes seqs[i]
+ * where the request was done and -1 where it was refused. A step whose calls
+ * are queued behind the reservation without a look at its status gives
+ * kvc_cache_write and kvc_attn_cache this array as their seqs: rows of a
+ * refused request are then written nowhere, and its tokens see nothing. */
+int kvc_cache_extend_granted(const kvc_cache * c, int n, const int * seqs, const int * count, int * status,
+                             int * granted, void * ws, size_t ws_bytes, void * stream);
+
 /* Rows of the last cells of each sequence, layers layer .. layer+n_layers-1.
  * Sequence seqs[i] takes rows cu[i] .. cu[i+1]-1 (cu: device int[n+1]) into
  * its last cu[i+1]-cu[i] cells, oldest first; n_rows = cu[n], known on the
@@ -93,10 +101,13 @@ int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * c
  * becomes 0. K and V rows of src_type: a cache of the same type takes the
  * bytes, a Q8_0 cache also F32, F16 and BF16 rows, encoded as by
  * kv_quantize_row. Row r of layer layer+j at byte j*ld_layer + r*ld_row;
- * both strides multiples of 2 (F32: 4). n_rows <= 2^24.
- * The cells are those that the last kvc_cache_extend reserved: a sequence is
- * forked before it is extended or after its rows are written, not in between
- * (a write goes to the page as it is, and a shared page is another's too). */
+ * both strides multiples of 2 (F32: 4). n_rows <= 2^24. A sequence number
+ * that the cache does not have takes no rows; each other is named once.
+ * The cells are those that the last kvc_cache_extend reserved. Where it
+ * refused, the last cells are older ones, so that sequence is not named here
+ * (kvc_cache_extend_granted leaves it out). Pages that another sequence holds
+ * too are not written: a sequence is forked before it is extended or after
+ * its rows are written, not in between. */
 typedef struct kvc_rows {
     const void * data;
     long long ld_layer, ld_row;   /* bytes */

@@ -196,9 +196,10 @@ __global__ __launch_bounds__(256) void k_cache_reset(Pages c) {
 // Reserves cells. A request's new pages are table columns have-copied .. of
 // its sequence, where copied is 1 when the last page is partly filled and
 // shared; that page's cells become a move job (identity, the old page in
-// saved[job][0]).
+// saved[job][0]). granted (or nullptr) names the sequences whose request is
+// done, for the calls behind this one.
 __global__ __launch_bounds__(kPlan) void k_cache_extend(Pages c, int n, const int * seqs, const int * count,
-                                                        int * status, Job * jobs, int * saved, int * list) {
+                                                        int * status, int * granted, Job * jobs, int * saved, int * list) {
     __shared__ int lds[kWaves], ids[kPlan], slots[kPlan], r_col[kPlan], r_need[kPlan], r_at[kPlan];
     const int i = threadIdx.x;
     const int page = 1 << c.shift;
@@ -233,6 +234,7 @@ __global__ __launch_bounds__(kPlan) void k_cache_extend(Pages c, int n, const in
     ids[i] = seq;
     if (i < n) {
         status[i] = done ? 0 : (missing ? missing : KVC_REQ_BAD);
+        if (granted) granted[i] = done ? seq : -1;
         Job j{};
         if (done && copied) {
             j = Job{seq, old & ~(page - 1), old, 0, 0, old, 1};
@@ -539,7 +541,10 @@ __global__ __launch_bounds__(256) void k_cache_move(Pages c, const Job * jobs, c
 
 // Row r of the call's packed rows: its sequence's cell, as a row of the pool
 // (page * page_size + cell), or -1. All threads; the answer for the block's
-// rows r0 .. r0+rows-1 (kRows at most) in place[].
+// rows r0 .. r0+rows-1 (kRows at most) in place[]. The threads look for the
+// rows' sequences; then a thread a row follows its chain of loads. A page of
+// more than one sequence takes no rows: a reservation that was granted never
+// ends in one, so these would be cells that were there before.
 constexpr int kRows = 8;
 __device__ void new_row_places(const Pages & c, int n, const int * seqs, const int * cu, int r0, int rows, int n_rows, int * place) {
     if (threadIdx.x < kRows) place[threadIdx.x] = -1;
@@ -549,17 +554,21 @@ __device__ void new_row_places(const Pages & c, int n, const int * seqs, const i
         const int lo = a > r0 ? a : r0;
         int hi = b < r0 + rows ? b : r0 + rows;
         if (hi > n_rows) hi = n_rows;
-        if (lo >= hi) continue;
-        const int s = seqs[i];
-        if (s < 0 || s >= c.max_seqs) continue;
-        const int held = c.len[s];
-        if (held > (long long)c.max_pages << c.shift) continue;
-        for (int r = lo; r < hi; r++) {
-            const long long cell = (long long)held - b + r;
-            if (cell < 0 || cell >= held) continue;
-            const int p = c.table[(long long)s * c.max_pages + (cell >> c.shift)];
-            if (good_page(c, p)) place[r - r0] = (p << c.shift) + (int)(cell & ((1 << c.shift) - 1));
+        for (int r = lo; r < hi; r++) place[r - r0] = i;
+    }
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+        const int i = place[threadIdx.x], s = i >= 0 ? seqs[i] : -1;
+        int at = -1;
+        if (s >= 0 && s < c.max_seqs) {
+            const int held = c.len[s];
+            const long long cell = (long long)held - cu[i + 1] + r0 + threadIdx.x;
+            if (cell >= 0 && cell < held && held <= (long long)c.max_pages << c.shift) {
+                const int p = c.table[(long long)s * c.max_pages + (cell >> c.shift)];
+                if (good_page(c, p) && c.refs[p] <= 1) at = (p << c.shift) + (int)(cell & ((1 << c.shift) - 1));
+            }
         }
+        place[threadIdx.x] = at;
     }
     __syncthreads();
 }
@@ -812,8 +821,8 @@ size_t kvc_cache_workspace(const kvc_cache * c, int n) {
     return plan_work(c, n, nullptr).bytes;
 }
 
-int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * count, int * status, void * ws,
-                     size_t ws_bytes, void * stream) {
+int kvc_cache_extend_granted(const kvc_cache * c, int n, const int * seqs, const int * count, int * status,
+                             int * granted, void * ws, size_t ws_bytes, void * stream) {
     if (int rc = check_cache(c)) return rc;
     if (int rc = check_requests(n)) return rc;
     if (n == 0) return 0;
@@ -825,10 +834,16 @@ int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * c
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
     const Pages p = pages_of(c);
     // (whole pages are 16-byte aligned, rows of a page may not be)
-    if (!launch(k_cache_extend, dim3(1), dim3(kPlan), st, p, n, seqs, count, status, w.jobs, w.saved, w.list) ||
+    if (!launch(k_cache_extend, dim3(1), dim3(kPlan), st, p, n, seqs, count, status, granted, w.jobs, w.saved,
+                w.list) ||
         !launch_move(c, p, w, n, c->page_size, Move{}, unit_of({p.krow, p.vrow}), st))
         return KV_COMPACT_E_DEVICE;
     return 0;
+}
+
+int kvc_cache_extend(const kvc_cache * c, int n, const int * seqs, const int * count, int * status, void * ws,
+                     size_t ws_bytes, void * stream) {
+    return kvc_cache_extend_granted(c, n, seqs, count, status, nullptr, ws, ws_bytes, stream);
 }
 
 int kvc_cache_write(const kvc_cache * c, int layer, int n_layers, int n, const int * seqs, const int * cu, int n_rows,

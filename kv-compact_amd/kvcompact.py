@@ -463,6 +463,7 @@ def bind_cache(dll):
     for name, args in {
             "kvc_cache_reset": [P(KvCache), _vp],
             "kvc_cache_extend": [P(KvCache), _i, _vp, _vp, _vp, _vp, sz, _vp],
+            "kvc_cache_extend_granted": [P(KvCache), _i, _vp, _vp, _vp, _vp, _vp, sz, _vp],
             "kvc_cache_write": [P(KvCache), _i, _i, _i, _vp, _vp, _i, _i, P(Rows), P(Rows), _vp],
             "kvc_cache_fork": [P(KvCache), _i, _vp, _vp, _vp, _vp],
             "kvc_cache_free": [P(KvCache), _i, _vp, _vp],
