@@ -128,7 +128,8 @@ int kvc_cache_free(const kvc_cache * c, int n, const int * seqs, void * stream);
  * them; what follows is dropped (no indices: the sequence is cut to start[i]).
  * Layer l's indices are idx + l*ld_idx (ld_idx 0: the same cells in every
  * layer), ascending within a sequence, each at least k - cu[i] and inside the
- * sequence (a cell whose index is not is left unwritten). n_idx = cu[n],
+ * sequence (where one is not, its cell's K, V and bias keep what their place
+ * on the page held, also with v and beta). n_idx = cu[n],
  * known on the host: cells whose k is at or past it are left unwritten.
  * v (NULL: the kept cells' own rows) gives the V rows: head h of row k of
  * layer l at byte l*ld_layer + k*ld_row + h*ld_head, in the cache's type.

@@ -413,7 +413,8 @@ constexpr int kCells = 1024;   // cells whose places a block works out at a time
 constexpr int kBatch = 16;     // rows a thread loads before it stores them
 
 // Places of cells c0 .. c0+kCells-1 of a job (all threads; barriers inside).
-// A place is a row of the pool, page * page_size + cell, or -1: left out.
+// A place is a row of the pool, page * page_size + cell, or -1: left out (an
+// index that does not fit leaves out all of its cell, given values too).
 // from_caller: the kept cells' sources are rows of the caller's array, and
 // rows of the pool stand as -2 - place.
 __device__ void cell_places(const Pages & c, const Job & j, const int * saved, const int * idx, bool from_caller,
@@ -429,15 +430,15 @@ __device__ void cell_places(const Pages & c, const Job & j, const int * saved, c
             const int q = t[to >> c.shift];
             if (good_page(c, q)) b = (q << c.shift) + (to & mask);
             const bool kept = k >= lead;
+            int from = to;
+            if (kept) {
+                // (an index below its place would read a row that is already overwritten)
+                const int x = idx[j.k0 + k - lead];
+                from = x >= k - lead && x < j.end - j.start ? j.start + x : -1;
+            }
             if (kept && from_caller) {
-                a = k - lead;
+                if (from >= 0) a = k - lead;
             } else {
-                int from = to;
-                if (kept) {
-                    // (an index below its place would read a row that is already overwritten)
-                    const int x = idx[j.k0 + k - lead];
-                    from = x >= k - lead && x < j.end - j.start ? j.start + x : -1;
-                }
                 const int p = from >= 0 ? saved[(from >> c.shift) - col0] : -1;
                 if (p >= 0) a = ((p & ~kShared) << c.shift) + (from & mask);
                 if (a == b) a = -1;

@@ -8,7 +8,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from cache_model import BAD, F16, attend, decode, encode
+from cache_model import BAD, F16, Q8_0, attend, decode, encode
 from kvc_harness import kc
 from test_gpu_cache_attn import Strided, compare, wide
 from test_gpu_cache_pages import Cache, dev, dll   # noqa: F401 (the fixture)
@@ -125,3 +125,59 @@ def test_a_step_behind_a_refused_reservation(dll):   # noqa: F811
     hiprt.check(h.hipGraphExecDestroy(exe))
     hiprt.check(h.hipGraphDestroy(graph))
     hiprt.check(h.hipStreamDestroy(stream))
+
+class BadIndices(Cache):
+    """Compactions some of whose indices do not fit."""
+
+    def run(self, seqs, start, cu, idx, total, values=False, betas=False, bad=(), what=""):
+        """idx [L][cu[-1]] as handed over; total the n_idx of the call; bad: (layer, k) of cells to be left unwritten."""
+        m = self.m
+        cu, idx = np.int32(cu), np.int32(idx)
+        n = idx.shape[1]
+        good = idx.copy()
+        for l, k in bad:
+            i = np.searchsorted(cu[1:], k, side="right")
+            good[l, k] = k - cu[i]           # (what the model moves; put back below)
+        bufs = [dev(np.int32(seqs)), dev(np.int32(start)), dev(cu), dev(idx), dev(np.full(len(seqs), 77, np.int32))]
+        v = beta = pv = pb = None
+        if values:
+            v = self.rng.integers(0, 256, (m.L, n, m.V.shape[3]), np.uint8)
+            bufs.append(dev(v))
+            pv = kc.Values(bufs[-1].value, n * v.shape[2], v.shape[2], v.shape[2] // m.H)
+        if betas:
+            beta = self.rng.standard_normal((m.L, m.H, n), np.float32)
+            bufs.append(dev(beta))
+            pb = kc.Betas(bufs[-1].value, m.H * n, n)
+        before = m.K.copy(), m.V.copy(), None if m.bias is None else m.bias.copy()
+        # (a request whose indices pass the ones given is refused: it asks for more cells than there are)
+        ask = [int(s) if cu[i + 1] <= total else -1 for i, s in enumerate(seqs)]
+        want = m.compact(ask, start, cu, good, v, beta)
+        for l, k in bad:
+            i = int(np.searchsorted(cu[1:], k, side="right"))
+            p, x = m.spots(m.table[seqs[i]], [start[i] + k - cu[i]])
+            m.K[l, p, x], m.V[l, p, x] = before[0][l, p, x], before[1][l, p, x]
+            if m.bias is not None:
+                m.bias[l, p, :, x] = before[2][l, p, :, x]
+        rc = self.dll.kvc_cache_compact(self.c, len(seqs), bufs[0].value, bufs[1].value, bufs[2].value, total,
+                                        bufs[3].value, n, ctypes.byref(pv) if pv else None,
+                                        ctypes.byref(pb) if pb else None, bufs[4].value, *self.ws(len(seqs)), None)
+        self._status(rc, want, bufs[4], what)
+
+
+@pytest.mark.parametrize("values", [False, True])
+@pytest.mark.parametrize("betas", [False, True])
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("kt", [F16, Q8_0])
+def test_indices_that_do_not_fit(dll, kt, shared, betas, values):   # noqa: F811
+    # negative, past the end, below their place: the cell is left as it was, in place and on a fresh page
+    c = BadIndices(dll, seed=3, pages=24, page=16, max_pages=10, L=2, k_type=kt, v_type=kt)
+    c.extend([0], [100])
+    c.write([0], [100])
+    if shared:
+        c.fork([0], [1])
+    start = 5
+    idx = np.stack([np.sort(c.rng.choice(np.arange(1, 95), 40, replace=False)) for _ in range(2)])
+    bad = [(0, 3), (0, 39), (1, 0), (1, 17), (1, 38)]
+    for (l, k), x in zip(bad, (-1, 95, -(1 << 31), 16, (1 << 31) - 1)):
+        idx[l, k] = x
+    c.run([0], [start], [0, 40], idx, 40, values, betas, bad, f"shared={shared}")
