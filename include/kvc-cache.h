@@ -129,8 +129,9 @@ int kvc_cache_free(const kvc_cache * c, int n, const int * seqs, void * stream);
  * Layer l's indices are idx + l*ld_idx (ld_idx 0: the same cells in every
  * layer), ascending within a sequence, each at least k - cu[i] and inside the
  * sequence (where one is not, its cell's K, V and bias keep what their place
- * on the page held, also with v and beta). n_idx = cu[n],
- * known on the host: cells whose k is at or past it are left unwritten.
+ * on the page held, also with v and beta). n_idx = cu[n], known on the host: a
+ * request whose cu[i+1] is past it is refused (KVC_REQ_BAD), as is one that
+ * asks for more cells than the sequence has behind start[i].
  * v (NULL: the kept cells' own rows) gives the V rows: head h of row k of
  * layer l at byte l*ld_layer + k*ld_row + h*ld_head, in the cache's type.
  * beta (NULL: the kept cells' own bias) gives the bias:

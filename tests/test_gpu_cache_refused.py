@@ -181,3 +181,15 @@ def test_indices_that_do_not_fit(dll, kt, shared, betas, values):   # noqa: F811
     for (l, k), x in zip(bad, (-1, 95, -(1 << 31), 16, (1 << 31) - 1)):
         idx[l, k] = x
     c.run([0], [start], [0, 40], idx, 40, values, betas, bad, f"shared={shared}")
+
+
+def test_fewer_indices_than_asked_for(dll):   # noqa: F811
+    # a request whose last index is past n_idx is refused; the ones before it are done
+    c = BadIndices(dll, seed=4, pages=24, page=16, max_pages=10, L=2)
+    c.extend([0, 1, 2], [60, 50, 40])
+    c.write([0, 1, 2], [60, 50, 40])
+    cu = [0, 20, 35, 45]
+    idx = np.concatenate([np.stack([c.some(n, k) for _ in range(2)]) for n, k in ((60, 20), (50, 15), (40, 10))], 1)
+    c.run([0, 1, 2], [0, 0, 0], cu, idx, 34, what="34 of 45")
+    assert c.m.len.tolist()[:3] == [20, 50, 40]
+    c.run([1, 2], [0, 0], [0, 15, 25], idx[:, 20:], 25, True, True, what="all of them")
