@@ -51,7 +51,10 @@ extern "C" {
  *   len   [max_seqs]             cells held
  *   refs  [n_pages]              sequences that hold the page; 0: free
  * k_row bytes is kv_quant_row_bytes(k_type, n_head_kv * d_k), likewise V.
- * Types: F32, F16, BF16, Q8_0 (d_k and d_v multiples of 32).
+ * Types: F32, F16, BF16, Q8_0 (its head width a multiple of 32). Where k_type
+ * and v_type differ, kvc_cache_write and kvc_attn_cache return
+ * KV_COMPACT_E_UNSUPPORTED: the caller fills such a cache and reads it by
+ * kernels of its own, and these calls reserve, share, move and gather the rows.
  * page_size: a power of two from 16 to 1024. n_pages <= 2^20. d_k, d_v <= 256.
  * K, V and bias 16-byte aligned, the workspaces too (hipMalloc's are).
  * New pages are the lowest free ones, in request order, so that equal calls
@@ -133,7 +136,8 @@ int kvc_cache_free(const kvc_cache * c, int n, const int * seqs, void * stream);
  * request whose cu[i+1] is past it is refused (KVC_REQ_BAD), as is one that
  * asks for more cells than the sequence has behind start[i].
  * v (NULL: the kept cells' own rows) gives the V rows: head h of row k of
- * layer l at byte l*ld_layer + k*ld_row + h*ld_head, in the cache's type.
+ * layer l at byte l*ld_layer + k*ld_row + h*ld_head, in the cache's V type;
+ * address and strides multiples of 2 (F32: 4).
  * beta (NULL: the kept cells' own bias) gives the bias:
  * beta[l*ld_layer + h*ld_head + k]. The outputs of
  * kvc_compact_layers_device (C_v: ld_row 4*d_v, ld_head 4*t*d_v, ld_layer

@@ -924,8 +924,9 @@ int kvc_cache_compact(const kvc_cache * c, int n, const int * seqs, const int * 
         mv.v = static_cast<const char *>(v->data);
         mv.v_layer = v->ld_layer; mv.v_row = v->ld_row; mv.v_head = v->ld_head;
         mv.v_head_bytes = (int)(p.vrow / c->n_head_kv);
-        any |= reinterpret_cast<long long>(v->data) | v->ld_layer | v->ld_row | v->ld_head | mv.v_head_bytes;
-        if (any & (c->v_type == KV_TYPE_F32 ? 3 : 1)) return KV_COMPACT_E_UNSUPPORTED;
+        const long long given = reinterpret_cast<long long>(v->data) | v->ld_layer | v->ld_row | v->ld_head;
+        if (given & (c->v_type == KV_TYPE_F32 ? 3 : 1)) return KV_COMPACT_E_UNSUPPORTED;
+        any |= given | mv.v_head_bytes;
     }
     if (beta) {
         mv.beta = beta->data; mv.b_layer = beta->ld_layer; mv.b_head = beta->ld_head;

@@ -8,7 +8,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from cache_model import BAD, F16, Q8_0, attend, decode, encode
+from cache_model import BAD, BF16, F16, F32, Q8_0, attend, decode, encode
 from kvc_harness import kc
 from test_gpu_cache_attn import Strided, compare, wide
 from test_gpu_cache_pages import Cache, dev, dll   # noqa: F401 (the fixture)
@@ -193,3 +193,14 @@ def test_fewer_indices_than_asked_for(dll):   # noqa: F811
     c.run([0, 1, 2], [0, 0, 0], cu, idx, 34, what="34 of 45")
     assert c.m.len.tolist()[:3] == [20, 50, 40]
     c.run([1, 2], [0, 0], [0, 15, 25], idx[:, 20:], 25, True, True, what="all of them")
+
+
+@pytest.mark.parametrize("kt,H,dk,dv", [(F16, 1, 33, 5), (BF16, 3, 7, 9), (F16, 2, 32, 64), (Q8_0, 1, 32, 5), (Q8_0, 3, 96, 8)])
+def test_keys_and_values_of_different_types(dll, kt, H, dk, dv):   # noqa: F811
+    # rows of K whose bytes are no multiple of 4 beside F32 values
+    c = Cache(dll, seed=6, pages=40, page=16, max_pages=16, L=2, H=H, dk=dk, dv=dv, k_type=kt, v_type=F32)
+    c.extend([0, 1], [70, 90])
+    c.fork([1], [2])
+    kept = [c.some(70, 30) for _ in range(2)], [c.some(80, 31) for _ in range(2)]
+    c.compact([0, 2], [0, 10], kept, values=True, betas=True)
+    c.compact([1], [3], [[c.some(87, 40) for _ in range(2)]], values=True, heads_apart=True)
