@@ -1601,7 +1601,7 @@ int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, void * ws
     const CacheShape s = cache_shape(c, x);
     const size_t need = kvc_attn_cache_workspace(c, x);
     if (need && !ws) return -1;
-    if (reinterpret_cast<uintptr_t>(ws) & 15) return KV_COMPACT_E_UNSUPPORTED;
+    if (need && reinterpret_cast<uintptr_t>(ws) & 15) return KV_COMPACT_E_UNSUPPORTED;
     if (need > ws_bytes) return KVC_E_SCRATCH;
     const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);
     const long long vrow = (long long)kv_quant_row_bytes(c->v_type, c->n_head_kv * c->d_v);

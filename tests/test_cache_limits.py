@@ -47,3 +47,13 @@ def test_caches_of_two_types(dll):   # noqa: F811
     for typ in (F32, F16, BF16, Q8_0):
         assert dll.kvc_cache_write(c, 0, 1, 2, FAKE, FAKE, 4, typ, r, r, None) == -5
         assert dll.kvc_attn_cache(c, attn(type=typ), FAKE, size, None) == -5
+
+
+def test_workspace_that_is_not_needed(dll):   # noqa: F811
+    # any address will do where the call needs no workspace; where it does, 16-byte aligned ones
+    c, size = cache(), 1 << 30
+    short, long = attn(), attn(n_seq=1, n_tok=1, max_new=1, max_len=100000)
+    assert dll.kvc_attn_cache_workspace(c, short) == 0 and dll.kvc_attn_cache_workspace(c, long) > 0
+    for ws, code in ((None, -1), (FAKE + 4, -5), (FAKE + 8, -5), (FAKE + 16, kc.E_DEVICE)):
+        assert dll.kvc_attn_cache(c, short, ws, size, None) == kc.E_DEVICE
+        assert dll.kvc_attn_cache(c, long, ws, size, None) == code
