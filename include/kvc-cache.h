@@ -171,10 +171,15 @@ int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_
  * the fast ones. n_head is a multiple of n_head_kv: query heads h*g ..
  * h*g+g-1 read KV head h. d_k, d_v from 1 to 256. Sums and softmax statistics
  * are fp32; F16 and BF16 round the softmax weights to that type before the
- * product with V (a Q8_0 cache: to fp16), and the result once. At most 2^30
- * rows (n_tok * n_head) a call. o and lse overlap no input. A row that sees no cell gives zeros
- * and lse -inf. lse = log(sum exp(scale q.k + bias)), float [n_tok][n_head],
- * may be NULL. scale 0: 1/sqrt(d_k). */
+ * product with V (a Q8_0 cache: to fp16), and the result once. A call has at
+ * most 2^30 rows (n_tok * n_head), and a launch's blocks limit it: prompts to
+ *   n_head_kv * (ceil(n_tok * n_head / n_head_kv / R) + n_seq) < 2^23,
+ * R = 128 for F16 and BF16 whose q, k, v and o are all in aligned rows, else 32
+ * where q, k and v are and heads are up to 128 wide, else 16; a cache call to
+ *   n_head_kv * n_seq < 2^23.
+ * o and lse overlap no input. A row that sees no cell gives zeros and lse
+ * -inf. lse = log(sum exp(scale q.k + bias)), float [n_tok][n_head], may be
+ * NULL. scale 0: 1/sqrt(d_k). */
 typedef struct kvc_heads {
     void *    data;
     long long ld_tok, ld_head;   /* elements */

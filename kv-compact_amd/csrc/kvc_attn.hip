@@ -1530,10 +1530,11 @@ template <bool CELLS, int RW> bool run_tiles(const AttnArgs & a, int type, long 
 int esize(int type) { return type == kF32 ? 4 : 2; }
 
 // Row numbers stay clear of 2^31 with a tile added, and a launch has fewer than
-// 2^32 threads (blocks of 512 at most).
+// 2^32 threads (blocks of 512 at most). (Key ranges only multiply launches of
+// fewer than 4096 blocks, to less than twice that.)
 constexpr long long kMaxRows = 1 << 30, kMaxBlocks = (1 << 23) - 1;
 
-// Shape of a cache call's launch.
+// Shape of a cache call's launch (n_seq > 0).
 struct CacheShape {
     int rt, tiles, splits, range;
     bool careful;
@@ -1550,7 +1551,10 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
         s.whole = rows > 64 && c->d_k <= 128 && c->d_v <= 128 ? 4 : 2;
     const int block_rows = s.whole ? 32 * s.whole : 16 * s.rt;
     const long long tiles = (rows + block_rows - 1) / block_rows;
-    s.tiles = (int)(tiles < 1 ? 1 : tiles > 65536 ? 65536 : tiles);
+    // (a block that has no tile of its own goes on with those that the grid has no blocks for)
+    const long long room = kMaxBlocks / ((long long)a->n_seq * c->n_head_kv);
+    const long long most_tiles = room < 1 ? 1 : room > 65536 ? 65536 : room;
+    s.tiles = (int)(tiles < 1 ? 1 : tiles > most_tiles ? most_tiles : tiles);
     // Key ranges: enough blocks to fill the GPU, each with at least 8 tiles of
     // 32 keys. Ranges of the same size in all sequences; four row tiles a wave
     // (one block a CU, and its time goes with its keys) take the same number

@@ -57,3 +57,26 @@ def test_workspace_that_is_not_needed(dll):   # noqa: F811
     for ws, code in ((None, -1), (FAKE + 4, -5), (FAKE + 8, -5), (FAKE + 16, kc.E_DEVICE)):
         assert dll.kvc_attn_cache(c, short, ws, size, None) == kc.E_DEVICE
         assert dll.kvc_attn_cache(c, long, ws, size, None) == code
+
+
+def test_what_one_launch_takes(dll):   # noqa: F811
+    # a cache call shapes its launch to what there is: only sequences times KV heads are limited
+    c = cache(k_type=F32, v_type=F32, n_head_kv=8)
+    for kw, code in ((dict(n_seq=2048, max_new=32768), kc.E_DEVICE), (dict(n_seq=1 << 19, max_new=1 << 19), kc.E_DEVICE),
+                     (dict(n_seq=(1 << 20) - 1, max_new=1), kc.E_DEVICE), (dict(n_seq=1 << 20, max_new=1), -5)):
+        a = attn(type=F32, n_head=8, max_len=1 << 20, **kw)
+        assert dll.kvc_attn_cache_workspace(c, a) == 0 and dll.kvc_attn_cache(c, a, None, 0, None) == code, kw
+
+    # a prompt call: n_head_kv * (ceil(n_tok * n_head / n_head_kv / R) + n_seq) < 2^23
+    def prompt(typ, d, n_tok, n_seq=1, pad=0, G=2):
+        h = [kc.Heads(FAKE, x * d + pad, d) for x in (2 * G, 2, 2, 2 * G)]
+        return dll.kvc_attn_prompt(kc.PromptArgs(q=h[0], k=h[1], v=h[2], o=h[3], cu=FAKE, type=typ, n_seq=n_seq, n_tok=n_tok,
+                                                 n_head=2 * G, n_head_kv=2, d_k=d, d_v=d), None)
+    for typ, d, pad, R in ((F16, 64, 0, 128), (BF16, 256, 8, 128), (F32, 128, 0, 32), (F32, 256, 0, 16), (F32, 132, 4, 16),
+                           (F16, 64, 1, 16), (F16, 20, 0, 16), (F32, 64, 1, 16)):
+        for n_seq in (1, 1 << 20):
+            most = ((1 << 22) - 1 - n_seq) * R // 2      # tokens: G rows each, R rows a block
+            if most * 4 > 1 << 30:
+                continue
+            assert prompt(typ, d, most, n_seq, pad) == kc.E_DEVICE, (typ, d, pad)
+            assert prompt(typ, d, most + 1, n_seq, pad) == -5, (typ, d, pad)
