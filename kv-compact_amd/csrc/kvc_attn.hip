@@ -1559,12 +1559,13 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     // 32 keys. Ranges of the same size in all sequences; four row tiles a wave
     // (one block a CU, and its time goes with its keys) take the same number
     // of ranges of each sequence instead.
+    const int max_len = a->max_len < 1 << 30 ? a->max_len : 1 << 30;   // (no sequence has more; sums with it stay in range)
     const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles, blocks = s.whole || s.rt == 4 ? 1024 : 4096;
-    long long want = (blocks + units - 1) / units, most = a->max_len / 256;
+    long long want = (blocks + units - 1) / units, most = max_len / 256;
     want = want < most ? want : most;
     if ((long long)a->n_tok * a->n_head > 1 << 24) want = 1;   // (the join's launch: a block a row or four; so many need no ranges)
     s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
-    s.range = s.rt == 4 ? 0 : (a->max_len + s.splits - 1) / s.splits;
+    s.range = s.rt == 4 ? 0 : (max_len + s.splits - 1) / s.splits;
     return s;
 }
 
