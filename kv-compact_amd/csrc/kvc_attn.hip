@@ -231,13 +231,13 @@ __device__ __forceinline__ unsigned seen32(const AttnArgs & a, const Sequence & 
 // count these loads: wait_lds_loads() does.
 __device__ __forceinline__ void load_lds16(const char * from, unsigned offset, char * to) {
     const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to;
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "m0", "memory");
 }
 // (4 bytes, each from an address of its own)
 __device__ __forceinline__ void load_lds4(const char * from, char * to) {
     const unsigned at = __builtin_amdgcn_readfirstlane(
         (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "m0", "memory");
 }
 // until at most N of the wave's loads are on their way
 template <int N> __device__ __forceinline__ void wait_lds_loads() {
