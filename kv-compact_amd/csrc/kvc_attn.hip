@@ -310,6 +310,26 @@ struct RowKernel {
     static __device__ __forceinline__ int column(int m, int c) { return (c / VW) * 16 * VW + VW * m + c % VW; }
 };
 
+// Tiles of a block's key range that left out values which are not finite: a bit
+// for each of up to 64 stretches of 2^shift tiles.
+struct OddTiles {
+    int t_lo, t_hi, shift;
+    unsigned long long bits = 0;
+    __device__ __forceinline__ OddTiles(int lo, int hi) : t_lo(lo), t_hi(hi) {
+        shift = hi - lo > 64 ? 26 - __builtin_clz(hi - lo - 1) : 0;
+    }
+    __device__ __forceinline__ void add(int t) { bits |= 1ull << ((t - t_lo) >> shift); }
+    // f(first key, key past the last) of each stretch, tiles of `keys` keys
+    template <class F> __device__ __forceinline__ void each(int keys, int held, F f) const {
+#pragma nounroll
+        for (unsigned long long m = bits; m; m &= m - 1) {
+            const int t0 = t_lo + ((__ffsll((long long)m) - 1) << shift);
+            const int t1 = t0 + (1 << shift) < t_hi ? t0 + (1 << shift) : t_hi;
+            f(t0 * keys, t1 * keys < held ? t1 * keys : held);
+        }
+    }
+};
+
 // Values of V that are not finite, for the rows of tiles that left them out:
 // one by one, the scores computed again.
 template <int TYPE, int QT> struct Odd {
@@ -359,7 +379,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) float join[4][ROWS][LD];
     __shared__ float join_m[4][ROWS], join_l[4][ROWS];
-    __shared__ int join_odd[4][2];
+    __shared__ unsigned long long join_odd[4];
     // Q8_0 scales of a wave's tile, by block and key
     __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
     __shared__ __align__(16) _Float16 v_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
@@ -551,7 +571,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 
         int page[2], next[2], later[2];
         f4 sc[RT][2];
-        int odd_lo = 1 << 30, odd_hi = 0;   // tiles with values that are not finite (they are left out, and added at the end)
+        OddTiles odd_tiles(t_lo, t_hi);   // with values that are not finite (they are left out, and added at the end)
         // K of the next tile is loaded behind the first product, V behind the
         // second, page numbers a tile earlier: the loads run under the arithmetic
         pages_of(t_lo + wave, page);
@@ -800,10 +820,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                     }
                 }
             }
-            if (SPECIAL && __ballot(odd)) {
-                odd_lo = t < odd_lo ? t : odd_lo;
-                odd_hi = t + 1;
-            }
+            if (SPECIAL && __ballot(odd)) odd_tiles.add(t);
             if (t + 4 < t_hi) load_v(t + 4, next);
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -835,15 +852,9 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                             f4{acc[r][w * C::VW + y][i], acc[r][w * C::VW + y + 1][i], acc[r][w * C::VW + y + 2][i],
                                acc[r][w * C::VW + y + 3][i]};
         }
-        if (lane == 0) {
-            join_odd[wave][0] = odd_lo;
-            join_odd[wave][1] = odd_hi;
-        }
+        if (lane == 0) join_odd[wave] = odd_tiles.bits;
         __syncthreads();
-        for (int w = 0; w < 4; w++) {
-            odd_lo = min(odd_lo, join_odd[w][0]);
-            odd_hi = max(odd_hi, join_odd[w][1]);
-        }
+        for (int w = 0; w < 4; w++) odd_tiles.bits |= join_odd[w];
         for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
             const int r = e / (D / 4), col = e % (D / 4) * 4;
             const int row = row0 + r;
@@ -859,19 +870,21 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                 l += f * join_l[w][r];
                 x += f * *reinterpret_cast<const f4 *>(&join[w][r][col]);
             }
-            if (__builtin_expect(odd_lo < odd_hi, 0)) {
+            if (__builtin_expect(odd_tiles.bits != 0, 0)) {
                 // what was left out reaches the rows that see its key
                 Odd<TYPE, QT> o{a, sq, h, row / a.G, row % a.G};
+                odd_tiles.each(32, held, [&](int key, int end) {
 #pragma nounroll
-                for (int key = odd_lo * 32; key < odd_hi * 32 && key < held; key++)
+                    for (; key < end; key++)
 #pragma nounroll
-                    for (int y = 0; y < 4 && col + y < a.dv; y++) {
-                        const float add = o.term(key, col + y, zero);
-                        x[0] += y == 0 ? add : 0.0f;
-                        x[1] += y == 1 ? add : 0.0f;
-                        x[2] += y == 2 ? add : 0.0f;
-                        x[3] += y == 3 ? add : 0.0f;
-                    }
+                        for (int y = 0; y < 4 && col + y < a.dv; y++) {
+                            const float add = o.term(key, col + y, zero);
+                            x[0] += y == 0 ? add : 0.0f;
+                            x[1] += y == 1 ? add : 0.0f;
+                            x[2] += y == 2 ? add : 0.0f;
+                            x[3] += y == 3 ? add : 0.0f;
+                        }
+                });
             }
             const long long out = (long long)(tok0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
             if (a.splits > 1) {
@@ -1098,7 +1111,7 @@ void k_attn_tiles(AttnArgs a) {
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-        int odd_lo = 1 << 30, odd_hi = 0;   // tiles with values that are not finite and were left out (see below)
+        OddTiles odd_tiles(t_lo, t_hi);     // with values that are not finite and were left out (see below)
         float mx = -INFINITY, sum = 0.0f;   // (mx: in units of s, kept up to 2^5 below the true maximum)
         float mc = 0.0f;                    // mx, or 0 while nothing is seen
 
@@ -1254,10 +1267,7 @@ void k_attn_tiles(AttnArgs a) {
                         acc[d] = mfma32<TYPE>(vf, pf[x0][st], acc[d]);
                     }
                 }
-            if (!PLAIN && hidden && __ballot(odd)) {
-                odd_lo = t < odd_lo ? t : odd_lo;
-                odd_hi = t + 1;
-            }
+            if (!PLAIN && hidden && __ballot(odd)) odd_tiles.add(t);
         };
         // (Loops apart for the two kinds: a branch around each product would keep
         // it behind its own load of V, two copies of the products in one loop
@@ -1317,7 +1327,7 @@ void k_attn_tiles(AttnArgs a) {
 #pragma unroll
                     for (int y = 0; y < 4; y++)
                         over[(4 * d + y) * 64] = f4{acc[d][4 * y], acc[d][4 * y + 1], acc[d][4 * y + 2], acc[d][4 * y + 3]};
-                over[DT * 4 * 64] = f4{mx, sum, __int_as_float(odd_lo), __int_as_float(odd_hi)};
+                over[DT * 4 * 64] = f4{mx, sum, __uint_as_float((unsigned)odd_tiles.bits), __uint_as_float((unsigned)(odd_tiles.bits >> 32))};
             }
             __syncthreads();
             if (kw == 0) {
@@ -1326,8 +1336,7 @@ void k_attn_tiles(AttnArgs a) {
                 const float f = __builtin_amdgcn_exp2f((mx - use) * c), g = __builtin_amdgcn_exp2f((theirs[0] - use) * c);
                 mx = top;
                 sum = sum * f + theirs[1] * g;
-                odd_lo = min(odd_lo, __float_as_int(theirs[2]));
-                odd_hi = max(odd_hi, __float_as_int(theirs[3]));
+                odd_tiles.bits |= __float_as_uint(theirs[2]) | (unsigned long long)__float_as_uint(theirs[3]) << 32;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -1374,7 +1383,7 @@ void k_attn_tiles(AttnArgs a) {
             if (a.lse && hf == 0 && kw == 0)
                 a.lse[out] = sum == 0.0f ? -INFINITY : (CELLS ? mx : mx * scale) + logf(sum);
         }
-        if (__builtin_expect(odd_lo < odd_hi, 0) && write && sum == sum) {
+        if (__builtin_expect(odd_tiles.bits != 0, 0) && write && sum == sum) {
             // Values that are not finite were left out of tiles where a key is
             // hidden from some row. They decide every result they reach (of rows
             // that are not NaN by their scores): those are written again.
@@ -1383,8 +1392,10 @@ void k_attn_tiles(AttnArgs a) {
 #pragma nounroll
             for (int col = 32 * d0 + hf; col < a.dv && col < 32 * (d0 + DT); col += 2) {
                 float x = 0.0f;
+                odd_tiles.each(BK, q.held, [&](int key, int end) {
 #pragma nounroll
-                for (int key = odd_lo * BK; key < odd_hi * BK && key < q.held; key++) x += o.term(key, col, top);
+                    for (; key < end; key++) x += o.term(key, col, top);
+                });
                 if (x == 0.0f) continue;
                 if (CELLS && a.splits > 1)
                     a.part_o[((long long)split * a.n_tok * a.H * a.G + out) * a.dv + col] = x;
