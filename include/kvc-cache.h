@@ -171,7 +171,10 @@ int kvc_cache_read(const kvc_cache * c, int seq, int start, int count, void * K_
  * the fast ones. n_head is a multiple of n_head_kv: query heads h*g ..
  * h*g+g-1 read KV head h. d_k, d_v from 1 to 256. Sums and softmax statistics
  * are fp32; F16 and BF16 round the softmax weights to that type before the
- * product with V (a Q8_0 cache: to fp16), and the result once. A call has at
+ * product with V (a Q8_0 cache: to fp16), and the result once. Over a Q8_0
+ * cache scores take the blocks' codes exactly and their scales in fp32; BF16
+ * queries lose the bits of elements under 2^-28 of their row's largest; values
+ * of V are scale times code rounded to fp16 where the result is BF16. A call has at
  * most 2^30 rows (n_tok * n_head), and a launch's blocks limit it: prompts to
  *   n_head_kv * (ceil(n_tok * n_head / n_head_kv / R) + n_seq) < 2^23,
  * R = 128 for F16 and BF16 whose q, k, v and o are all in aligned rows, else 32

@@ -280,13 +280,13 @@ __device__ __forceinline__ float byte_value(const unsigned * w, int i) {
 //
 // Each key is read once for all rows of its head, straight into the registers
 // the products take it from, a tile ahead. One token of 64 sequences of up to
-// 16384 bf16 cells (8 x 128, 32 heads): 0.50 ms, 5.3 TB/s, HBM's rate. One
-// sequence of 4096 cells: 14 us with the join, two launches and two latencies;
-// of 20000 F32 cells with a bias: 48 us, 3.4 TB/s. Trees of 13 tokens
-// of 32 heads over 16 sequences of up to 32768 Q8_0 cells (8 x 128): 404 us,
-// bound by the instructions that decode codes and scale sums (264 us of issue;
-// four row tiles a wave decode a key once for all 52 rows, and leave one wave a
-// SIMD).
+// 16384 bf16 cells (8 x 128, 32 heads): 0.52 ms, 5.2 TB/s (a plain read: 6.8).
+// One sequence of 4096 cells: 14 us with the join, two launches and two
+// latencies; of 20000 F32 cells with a bias: 49 us, 3.4 TB/s. Trees of 13 tokens
+// of 32 heads over 16 sequences of up to 32768 Q8_0 cells (8 x 128): 409 us.
+// Four row tiles a wave decode a key once for all 52 rows and leave one wave a
+// SIMD: vector instructions are 47 % of its cycles, matrix instructions 9 %,
+// and most of the rest is loads that nothing else runs under.
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 struct RowKernel {
     static constexpr int ES = TYPE == kF32 ? 4 : 2;          // bytes of a q element
@@ -938,8 +938,10 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // A prompt's blocks are four waves, two of them on a CU: one's softmax runs
 // under the other's products, and K and V come from L2 (one tile ahead). They
 // are bound by what issues beside the products: 16384 tokens of 32 heads of 128
-// take 2.27 ms, 971 TFLOP/s (85 % of a large matrix product's rate; 2.36 ms
-// with one loop for plain and masked tiles), 12 prompts of as many in all 0.57 ms.
+// take 2.2 to 2.34 ms by card, 940 to 995 TFLOP/s (a large matrix product: 1130;
+// 4 % more with one loop for plain and masked tiles; matrix units busy 46 % of
+// the cycles, vector instructions 44 %), 12 prompts of as many in all 0.56 to
+// 0.59 ms (37 % and 43 %: the last blocks of ragged prompts).
 // At 256 columns a wave's sums and queries alone are 192 registers, which
 // leaves one wave a SIMD and a third of its instructions moves between the
 // halves of the file: 5003 tokens in three prompts of 8 heads took 132 us that
@@ -949,8 +951,9 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
 // Over a cache HBM has to be kept busy: eight waves share four buffers (RW = 4:
 // 96 KB on their way), or two blocks of four waves two buffers each (RW = 2).
 // Eight sequences of up to 20000 F16 cells, 8 x 128, with 32 drafts of 32 heads
-// take 157 us, 2.7 TB/s (163 with one loop for plain and masked tiles); bound by the last blocks of ragged sequences and by a
-// step's latency, 2.2 us where its loads alone would take 1.7.
+// take 157 us, 2.7 TB/s (163 with one loop for plain and masked tiles); bound by
+// the last blocks of ragged sequences and by a step's latency, 2.2 us where its
+// loads alone would take 1.7 (matrix units busy 14 %, vector instructions 27 %).
 __device__ const unsigned zero_word = 0;
 __device__ const unsigned hidden_word = 0xff800000u;   // -inf
 
@@ -1520,7 +1523,14 @@ bool run_rows(const AttnArgs & a, int type, int qt, int rt, bool careful, long l
 // Row tiles a wave holds: two where there are more than 16 rows, and over a
 // Q8_0 cache, whose rows cost more to decode than to multiply, four where
 // there are more than 32; at 256 wide heads more than one does not fit the
-// registers.
+// registers. Measured, us (8 KV heads of 128, trees; one, two and four tiles):
+//   8 sequences of up to 16384 cells, 32 rows   F16 141, 138; F32 311, 295
+//   the same, 20 rows                           F16 128, 127; F32 267, 280
+//   Q8_0, 16 sequences of up to 32768 cells: 24 rows 454, 414, 460; 36 rows
+//     569, 591, 466; 52 rows 797, 631, 471; 64 of up to 8192, 20 rows 491, 429
+//   Q8_0, 8 sequences of up to 16384 cells, 32 rows: 146, 195 (one would do
+//     better where the call is this small)
+//   F32 prompts of 2048 tokens in all, 32 heads: 354, 271
 int row_tiles(int type, int d, bool careful, long long rows) {
     if (rows <= 16 || careful || d == 256) return 1;
     return rows > 32 && type == kQ8 ? 4 : 2;
@@ -1558,6 +1568,14 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
     const long long rows = (long long)a->max_new * G;
     s.rt = row_tiles(c->k_type, head_tile(c->d_k, c->d_v), s.careful, rows);
+    // Tiles in LDS from 33 rows on: 8 sequences of up to 20000 F16 cells with a
+    // bias, k_attn_rows against two waves of rows: 36 rows 164 and 127 us, 64
+    // rows 190 and 133 (24 rows 152 and 121: it would pay earlier); one
+    // sequence of 20000: 32 rows 33 both, 36 rows 47 and 34. Four waves of rows
+    // from 65 on read a tile for twice as many rows; which is faster goes with
+    // the sequences' lengths: 128 rows 157 us against 170 with two, and with
+    // other lengths 190 against 183 and 183 against 175; 16 sequences of up to
+    // 16384 242 against 260; 64 of up to 4096, 80 rows, 268 against 227.
     if (rows > 32 && !s.careful && c->k_type != kF32 && c->k_type != kQ8 && vec_rows(a->o, es))
         s.whole = rows > 64 && c->d_k <= 128 && c->d_v <= 128 ? 4 : 2;
     const int block_rows = s.whole ? 32 * s.whole : 16 * s.rt;
@@ -1569,7 +1587,13 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a) {
     // Key ranges: enough blocks to fill the GPU, each with at least 8 tiles of
     // 32 keys. Ranges of the same size in all sequences; four row tiles a wave
     // (one block a CU, and its time goes with its keys) take the same number
-    // of ranges of each sequence instead.
+    // of ranges of each sequence instead (trees over Q8_0 471 us, 559 with
+    // ranges of one size). Measured, us, for 1024 and 4096 blocks: one token of
+    // 64 sequences of up to 16384 bf16 cells 559 and 509, Q8_0 642 and 542 (8192:
+    // 503 and 497; of 8 sequences 96 and 105); trees of 32 over F16 193 and 319
+    // (512: 171), of 13 over Q8_0 469 and 604. For one token of one sequence:
+    // 4096 cells in 8, 16 and 32 ranges 17.0, 14.1 and 13.3, 1024 cells in 2, 4
+    // and 8 15.2, 12.4 and 11.1. At most 64, the lanes of the join's wave.
     const int max_len = a->max_len < 1 << 30 ? a->max_len : 1 << 30;   // (no sequence has more; sums with it stay in range)
     const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles, blocks = s.whole || s.rt == 4 ? 1024 : 4096;
     long long want = (blocks + units - 1) / units, most = max_len / 256;
