@@ -143,7 +143,8 @@ int kvc_cache_free(const kvc_cache * c, int n, const int * seqs, void * stream);
  * kvc_compact_layers_device (C_v: ld_row 4*d_v, ld_head 4*t*d_v, ld_layer
  * 4*H*t*d_v; beta: ld_head t, ld_layer H*t) and of the quantized entry fit as
  * they are. Rows move within the sequence's pages; a page that is shared is
- * replaced by a free one. start[i] is the same in every layer. */
+ * replaced by a free one. start[i] is the same in every layer. v and beta
+ * overlap no array of the cache. */
 typedef struct kvc_values {
     const void * data;
     long long ld_layer, ld_row, ld_head;   /* bytes */
@@ -202,7 +203,7 @@ typedef struct kvc_prompt_args {
 int kvc_attn_prompt(const kvc_prompt_args * a, void * stream);
 
 /* Attention over one layer of a cache. Sequence seqs[s] (NULL: s) has tokens
- * cu[s] .. cu[s+1]-1, whose rows are the last cells of the sequence: n_new =
+ * cu[s] .. cu[s+1]-1 (cu: device int[n_seq+1], ascending), whose rows are the last cells of the sequence: n_new =
  * cu[s+1]-cu[s] of len. Every token sees the cells before those. Of the last
  * n_new, token i sees cell j when bit j % 64 of mask[i_row*mask_words + j/64]
  * is set (a tree of drafts: a token's ancestors and itself), without a mask

@@ -5,7 +5,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from cache_model import BF16, F16, F32, Q8_0
+from cache_model import BF16, F16, F32, Q8_0, encode
 from kvc_harness import kc
 from test_gpu_cache_attn import dev, dll, run_cells, typed   # noqa: F401 (the fixture)
 
@@ -96,3 +96,41 @@ def test_values_that_are_not_finite_in_a_long_range(dll, typ, cache, G):   # noq
         v[p, i, :, 13] = np.inf if cache != Q8_0 else 1.0
     run_cells(dll, typ, cache, [5010, 40], [2, 1], 2, G, 64, 64, page=64, bias=True, tree=True, seed=43, edit=edit, max_len=1,
               runs=2)
+
+
+@pytest.mark.parametrize("typ,cache", [(F32, F32), (F16, F16), (BF16, Q8_0)])
+@pytest.mark.parametrize("news,G", [([1, 1, 1], 2), ([20, 3, 9], 4), ([40, 1, 33], 4)])
+def test_tokens_around_the_sequences(dll, typ, cache, news, G):   # noqa: F811
+    # cu that begins behind 0 and ends before n_tok: the same results, bit for bit, and nothing else written
+    H, d, page, lens = 2, 64, 32, [1500, 40, 333]
+    rng = np.random.default_rng(44)
+    pages = [-(-m // page) for m in lens]
+    n_pages = sum(pages)
+    K, V = (dev(encode(rng.standard_normal((n_pages * page, H * d)).astype(np.float32), cache)) for _ in range(2))
+    table = np.full((3, max(pages)), -1, np.int32)
+    for s, p in enumerate(pages):
+        table[s, :p] = np.arange(p) + sum(pages[:s])
+    held = [dev(x) for x in (table, np.int32(lens), np.ones(n_pages, np.int32))]
+    c = kc.KvCache(n_layers=1, n_pages=n_pages, page_size=page, max_seqs=3, max_pages=max(pages), n_head_kv=H, d_k=d, d_v=d,
+                   k_type=cache, v_type=cache, K=K.value, V=V.value, table=held[0].value, len=held[1].value, refs=held[2].value)
+    n, Hq = sum(news), H * G
+    q = typed(rng.standard_normal((n, Hq, d)), typ)
+    out = []
+    for before, after in ((0, 0), (3, 5)):
+        m = before + n + after
+        all_q = np.zeros((m, Hq, d), q.dtype)
+        all_q[before:before + n] = q
+        dq, o, lse = dev(all_q), dev(typed(np.full((m, Hq, d), 7.0), typ)), dev(np.full((m, Hq), 9.0, np.float32))
+        cu = dev(np.int32(before + np.concatenate([[0], np.cumsum(news)])))
+        h = [kc.Heads(x.value, Hq * d, d) for x in (dq, o)]
+        a = kc.CacheAttnArgs(q=h[0], o=h[1], lse=lse.value, cu=cu.value, type=typ, n_seq=3, n_tok=m, n_head=Hq,
+                             max_new=max(news), max_len=1500)
+        size = dll.kvc_attn_cache_workspace(c, a)
+        assert size > 0
+        ws = dev(np.full(size, 0xFF, np.uint8))
+        assert dll.kvc_attn_cache(c, a, ws.value, size, None) == 0
+        x, l = o.download(q.dtype, m * Hq * d).reshape(m, Hq, d), lse.download(np.float32, m * Hq).reshape(m, Hq)
+        rest = np.r_[0:before, before + n:m]
+        assert (x[rest] == typed(np.full(1, 7.0), typ)[0]).all() and (l[rest] == 9.0).all()
+        out.append((x[before:before + n].tobytes(), l[before:before + n].tobytes()))
+    assert out[0] == out[1]

@@ -204,3 +204,19 @@ def test_keys_and_values_of_different_types(dll, kt, H, dk, dv):   # noqa: F811
     kept = [c.some(70, 30) for _ in range(2)], [c.some(80, 31) for _ in range(2)]
     c.compact([0, 2], [0, 10], kept, values=True, betas=True)
     c.compact([1], [3], [[c.some(87, 40) for _ in range(2)]], values=True, heads_apart=True)
+
+
+def test_rows_before_the_first_sequence(dll):   # noqa: F811
+    # cu need not begin at 0: rows and indices before it belong to no request
+    c = BadIndices(dll, seed=9, pages=24, page=16, max_pages=10, L=2)
+    c.extend([0, 1], [60, 50])
+    c.write([0, 1], [60, 50])
+    rows = [c.rng.integers(0, 256, (2, 12, 128), np.uint8) for _ in range(2)]
+    bufs = [dev(x) for x in rows]
+    a, cu = dev(np.int32([1, 0])), np.int32([4, 7, 10])
+    r, dcu = [kc.Rows(b.value, 12 * 128, 128) for b in bufs], dev(cu)
+    assert dll.kvc_cache_write(c.c, 0, 2, 2, a.value, dcu.value, 10, F16, *r, None) == 0
+    c.m.write(0, 2, [1, 0], cu, *rows)
+    c.check("write from row 4 on")
+    idx = np.concatenate([np.full((2, 5), -7), np.stack([c.some(60, 20) for _ in range(2)]), np.stack([c.some(50, 9) for _ in range(2)])], 1)
+    c.run([0, 1], [0, 0], [5, 25, 34], idx, 34, True, True, what="indices from the sixth on")
