@@ -228,6 +228,25 @@ typedef struct kvc_cache_attn_args {
 size_t kvc_attn_cache_workspace(const kvc_cache * c, const kvc_cache_attn_args * a);
 int kvc_attn_cache(const kvc_cache * c, const kvc_cache_attn_args * a, void * ws, size_t ws_bytes, void * stream);
 
+/* The same two with a sliding window: of the tokens (cells) that the calls
+ * above show a token, it sees the first `first` of its sequence and the last
+ * `last` up to and with itself (first >= 0, last >= 1; -2 otherwise). Over a
+ * cache with a mask, a token sees its drafted cells by the mask alone, and they
+ * count as its last: of the cells before the drafts it sees the first `first`
+ * and the last max(0, last - b), b the bits set in its mask below n_new. Work
+ * goes with first + last, not with the length: what no token of a tile sees is
+ * not read. Cells are counted as the cache holds them, so a window over a
+ * compacted sequence spans its kept cells. Workspaces are the window call's own:
+ * kvc_attn_cache_window_workspace with the same window. Limits, types and
+ * errors are those of the calls without one; a NULL window returns -1. */
+typedef struct kvc_window {
+    int first, last;
+} kvc_window;
+int kvc_attn_prompt_window(const kvc_prompt_args * a, const kvc_window * w, void * stream);
+size_t kvc_attn_cache_window_workspace(const kvc_cache * c, const kvc_cache_attn_args * a, const kvc_window * w);
+int kvc_attn_cache_window(const kvc_cache * c, const kvc_cache_attn_args * a, const kvc_window * w, void * ws,
+                          size_t ws_bytes, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

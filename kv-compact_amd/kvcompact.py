@@ -456,6 +456,11 @@ class CacheAttnArgs(ctypes.Structure):
         ("scale", _f)]
 
 
+class Window(ctypes.Structure):
+    """kvc_window."""
+    _fields_ = [("first", _i), ("last", _i)]
+
+
 def bind_cache(dll):
     """Declare the entry points of include/kvc-cache.h. Device arrays go in as addresses (int or None), structs by
     reference (a ctypes instance is passed as one)."""
@@ -470,10 +475,14 @@ def bind_cache(dll):
             "kvc_cache_compact": [P(KvCache), _i, _vp, _vp, _vp, _i, _vp, _ll, P(Values), P(Betas), _vp, _vp, sz, _vp],
             "kvc_cache_read": [P(KvCache), _i, _i, _i, _vp, _vp, _vp, _vp],
             "kvc_attn_prompt": [P(PromptArgs), _vp],
+            "kvc_attn_prompt_window": [P(PromptArgs), P(Window), _vp],
+            "kvc_attn_cache_window": [P(KvCache), P(CacheAttnArgs), P(Window), _vp, sz, _vp],
             "kvc_attn_cache": [P(KvCache), P(CacheAttnArgs), _vp, sz, _vp]}.items():
         f = getattr(dll, name)
         f.argtypes, f.restype = args, _i
     dll.kvc_cache_workspace.argtypes, dll.kvc_cache_workspace.restype = [P(KvCache), _i], sz
     dll.kvc_attn_cache_workspace.argtypes = [P(KvCache), P(CacheAttnArgs)]
     dll.kvc_attn_cache_workspace.restype = sz
+    dll.kvc_attn_cache_window_workspace.argtypes = [P(KvCache), P(CacheAttnArgs), P(Window)]
+    dll.kvc_attn_cache_window_workspace.restype = sz
     return dll
