@@ -247,6 +247,84 @@ size_t kvc_attn_cache_window_workspace(const kvc_cache * c, const kvc_cache_attn
 int kvc_attn_cache_window(const kvc_cache * c, const kvc_cache_attn_args * a, const kvc_window * w, void * ws,
                           size_t ws_bytes, void * stream);
 
+/* ---- a budget of cells ----------------------------------------------------
+ * What tokens attended to, gathered by cell, and the cells to keep by it. The
+ * caller owns
+ *   weight [n_layers][max_seqs][n_head_kv][max_pages * page_size] float
+ * by sequence and cell, not by page: sequences that share pages gather apart. */
+
+/* Adds to each cell of a layer the softmax weight that tokens gave it. a: the
+ * arguments of the attention call that computed those tokens, whose lse it
+ * wrote (o is not touched; lse may not be NULL); w: its window, or NULL. For
+ * cell j of sequence seqs[s], KV head h
+ *   weight = decay * weight + sum exp(scale q.k + bias - lse)
+ * over the sequence's tokens that see j and the query heads h*g .. h*g+g-1, in
+ * fp32 and in one order (two calls give the same bits). The last n_new cells,
+ * those of the tokens, begin at 0, and so do the last `fresh` ones, for a call
+ * that does not name every token that came since the last one; decay 0 begins
+ * all at 0: nothing is read then. decay is from 0 to 1. tail > 0: only the last
+ * `tail` tokens of each sequence are counted. Rows whose lse is -inf give
+ * nothing; cells of a bad page gather nothing. Weights at or past the
+ * sequence's end are left as they were, and so are sequences without tokens, of
+ * a bad number or with more tokens than cells. No sequence is named twice.
+ * Types and limits as of kvc_attn_cache. No workspace. */
+typedef struct kvc_weigh_args {
+    float * weight;
+    float decay;
+    int tail, fresh;
+} kvc_weigh_args;
+int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * a, const kvc_window * w, const kvc_weigh_args * x,
+                    void * stream);
+
+/* Picks the cells that sequence seqs[i] keeps behind its first start[i] ones
+ * (which stay, as in kvc_cache_compact): the last min(recent, keep[i]) of the
+ * sequence, and of the others those of the largest score, keep[i] in all or as
+ * many as there are; of equal scores those of the lower index. A cell's score is
+ * the sum of its heads' weights (KVC_HEADS_SUM: in 64 bits, heads ascending,
+ * rounded once to float) or the largest of them (KVC_HEADS_MAX, NaN passed
+ * over); a NaN score ranks below every other. Layer l's indices go to
+ * idx + l*ld_idx, ascending and counted from start[i], request i's at
+ * cu[i] .. cu[i+1]-1; ld_idx 0: one list for all layers, by the sum (the
+ * largest) over the layers too, layers before heads. cu (int[n+1]), granted and
+ * status (int[n]) are written: status 0 and granted seqs[i], or KVC_REQ_BAD and
+ * -1 where the sequence number, start or keep does not fit, the sequence has
+ * more than max_len cells, an earlier request names it, or the indices of the
+ * requests granted before leave too few of the n_idx places (a refused one has
+ * none). idx, cu and granted then go into kvc_cache_compact as they are: with
+ * granted for its seqs, a refused sequence keeps all its cells. ld_idx is 0 or
+ * at least n_idx. n_layers * n under 2^22 (ld_idx 0: n). weight 16-byte aligned.
+ * No array that is written overlaps another. */
+#define KVC_HEADS_SUM 0
+#define KVC_HEADS_MAX 1
+typedef struct kvc_pick_args {
+    const int *   seqs;
+    const int *   start;
+    const int *   keep;
+    const float * weight;
+    int *     idx;
+    long long ld_idx;
+    int * cu;
+    int * granted;
+    int * status;
+    int n_idx, recent, heads, max_len;
+} kvc_pick_args;
+size_t kvc_cache_pick_workspace(const kvc_cache * c, int n, const kvc_pick_args * a);
+int kvc_cache_pick(const kvc_cache * c, int n, const kvc_pick_args * a, void * ws, size_t ws_bytes, void * stream);
+
+/* Weights follow their cells, in all layers: sequence dst[i] takes those of
+ * src[i]. cu NULL: of the first len[dst[i]] cells, after a fork (start, idx,
+ * n_idx and ld_idx are not looked at). Otherwise as kvc_cache_compact moves
+ * cells: the first start[i], then those at start[i] + idx[k], k = cu[i] ..
+ * cu[i+1]-1, each index at least k - cu[i] (where one is not, or lies past the
+ * array, its place keeps what it held). src[i] may be dst[i], for a compaction
+ * in place; else no dst is the src of another request. No dst is named twice.
+ * status (NULL: all): only requests whose status is 0 move, so that those that a
+ * compaction or a fork refused keep their weights. A request whose sequence
+ * numbers, start or cu do not fit moves nothing. */
+int kvc_cache_take_weights(const kvc_cache * c, int n, const int * src, const int * dst, const int * start,
+                           const int * cu, int n_idx, const int * idx, long long ld_idx, const int * status,
+                           float * weight, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

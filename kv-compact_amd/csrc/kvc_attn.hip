@@ -148,12 +148,14 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a, const
     return s;
 }
 
-int check_window(const kvc_window * w) { return w && (w->first < 0 || w->last < 1) ? -2 : 0; }
-
 void set_window(AttnArgs & a, const kvc_window * w) {
     a.first = w->first < 1 << 30 ? w->first : 1 << 30;
     a.last = w->last < 1 << 30 ? w->last : 1 << 30;
 }
+
+}  // namespace
+
+int check_window(const kvc_window * w) { return w && (w->first < 0 || w->last < 1) ? -2 : 0; }
 
 int check_cache_attn(const kvc_cache * c, const kvc_cache_attn_args * a) {
     if (int rc = check_cache(c)) return rc;
@@ -167,6 +169,30 @@ int check_cache_attn(const kvc_cache * c, const kvc_cache_attn_args * a) {
     if (c->k_type == kQ8 ? a->type != kF16 && a->type != kBF16 : a->type != c->k_type) return KV_COMPACT_E_UNSUPPORTED;
     return 0;
 }
+
+int cache_args(const kvc_cache * c, const kvc_cache_attn_args * x, const kvc_window * w, AttnArgs & a) {
+    const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);
+    const long long vrow = (long long)kv_quant_row_bytes(c->v_type, c->n_head_kv * c->d_v);
+    const long long cells = (long long)c->n_pages * c->page_size;
+    if (krow >= 1 << 24 || vrow >= 1 << 24) return KV_COMPACT_E_UNSUPPORTED;
+    a = AttnArgs{};
+    a.k = RowsAt{static_cast<const char *>(c->K) + x->layer * cells * krow, krow / c->n_head_kv, (unsigned)krow};
+    a.v = RowsAt{static_cast<const char *>(c->V) + x->layer * cells * vrow, vrow / c->n_head_kv, (unsigned)vrow};
+    a.q = static_cast<const char *>(x->q.data);
+    a.o = static_cast<char *>(x->o.data);
+    a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;
+    a.lse = x->lse; a.cu = x->cu; a.seqs = x->seqs; a.len = c->len; a.table = c->table;
+    a.bias = c->bias ? c->bias + x->layer * cells * c->n_head_kv : nullptr;
+    a.mask = reinterpret_cast<const unsigned long long *>(x->mask);
+    a.mask_words = x->mask_words; a.n_seq = x->n_seq; a.n_tok = x->n_tok;
+    a.H = c->n_head_kv; a.G = x->n_head / c->n_head_kv; a.dk = c->d_k; a.dv = c->d_v;
+    a.shift = __builtin_ctz(c->page_size); a.n_pages = c->n_pages; a.max_seqs = c->max_seqs; a.max_pages = c->max_pages;
+    a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)c->d_k);
+    if (w) set_window(a, w);
+    return 0;
+}
+
+namespace {
 
 size_t cache_workspace(const kvc_cache * c, const kvc_cache_attn_args * a, const kvc_window * w) {
     if (check_cache_attn(c, a) || check_window(w) || a->n_seq == 0 || a->n_tok == 0) return 0;
@@ -188,24 +214,9 @@ int attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, const kvc_win
     if (need && !ws) return -1;
     if (need && reinterpret_cast<uintptr_t>(ws) & 15) return KV_COMPACT_E_UNSUPPORTED;
     if (need > ws_bytes) return KVC_E_SCRATCH;
-    const long long krow = (long long)kv_quant_row_bytes(c->k_type, c->n_head_kv * c->d_k);
-    const long long vrow = (long long)kv_quant_row_bytes(c->v_type, c->n_head_kv * c->d_v);
-    const long long cells = (long long)c->n_pages * c->page_size;
-    if (krow >= 1 << 24 || vrow >= 1 << 24) return KV_COMPACT_E_UNSUPPORTED;
-    AttnArgs a{};
-    a.k = RowsAt{static_cast<const char *>(c->K) + x->layer * cells * krow, krow / c->n_head_kv, (unsigned)krow};
-    a.v = RowsAt{static_cast<const char *>(c->V) + x->layer * cells * vrow, vrow / c->n_head_kv, (unsigned)vrow};
-    a.q = static_cast<const char *>(x->q.data);
-    a.o = static_cast<char *>(x->o.data);
-    a.q_tok = x->q.ld_tok; a.q_head = x->q.ld_head; a.o_tok = x->o.ld_tok; a.o_head = x->o.ld_head;
-    a.lse = x->lse; a.cu = x->cu; a.seqs = x->seqs; a.len = c->len; a.table = c->table;
-    a.bias = c->bias ? c->bias + x->layer * cells * c->n_head_kv : nullptr;
-    a.mask = reinterpret_cast<const unsigned long long *>(x->mask);
-    a.mask_words = x->mask_words; a.n_seq = x->n_seq; a.n_tok = x->n_tok;
-    a.H = c->n_head_kv; a.G = x->n_head / c->n_head_kv; a.dk = c->d_k; a.dv = c->d_v;
-    a.shift = __builtin_ctz(c->page_size); a.n_pages = c->n_pages; a.max_seqs = c->max_seqs; a.max_pages = c->max_pages;
+    AttnArgs a;
+    if (int rc = cache_args(c, x, w, a)) return rc;
     a.splits = s.splits; a.range = s.range; a.tiles = s.tiles;
-    a.scale = x->scale != 0.0f ? x->scale : 1.0f / sqrtf((float)c->d_k);
     a.part_o = static_cast<float *>(ws);
     a.part_ml = a.part_o + (size_t)s.splits * x->n_tok * x->n_head * c->d_v;
     const long long blocks = (long long)x->n_seq * s.tiles * s.splits * a.H;
@@ -213,7 +224,6 @@ int attn_cache(const kvc_cache * c, const kvc_cache_attn_args * x, const kvc_win
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
-    if (w) set_window(a, w);
     if (!(w ? run_attn_window(a, c->k_type, x->type, s.whole, s.rt, s.careful, blocks, st)
             : run_attn<false>(a, c->k_type, x->type, s.whole, s.rt, s.careful, blocks, st)))
         return KV_COMPACT_E_DEVICE;

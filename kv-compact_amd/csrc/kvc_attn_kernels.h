@@ -429,6 +429,34 @@ template <int TYPE, int QT, bool WINDOW> struct Odd {
     }
 };
 
+// A bf16 row over Q8_0 keys as fp16 times a power of two; scores are products times to_score times rest.
+template <int NK> __device__ __forceinline__ void bf16_row_to_f16(u4 (&q)[NK], float scale, float & to_score, float & rest) {
+    // the largest of the row to 2^14 (eight bits of it: exact; others from 2^-28 of it on)
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned lo = q[j][i] & 0x7fffu, hi = q[j][i] >> 16 & 0x7fffu;
+            top = lo > top ? lo : top;
+            top = hi > top ? hi : top;
+        }
+    top = max(top, (unsigned)__shfl_xor((int)top, 16));
+    top = max(top, (unsigned)__shfl_xor((int)top, 32));
+    int e = (int)(top >> 7) - 127;               // of the largest
+    if (top == 0 || top >= 0x7f80u) e = 14;      // nothing, or not finite: as it is
+    const int near = 14 - e > 100 ? 100 : 14 - e < -100 ? -100 : 14 - e;
+    const float up = __builtin_ldexpf(1.0f, near), more = __builtin_ldexpf(1.0f, 14 - e - near);
+#pragma unroll
+    for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            q[j][i] = pack2<kF16>(bf16_value((unsigned short)q[j][i]) * up * more,
+                                 bf16_value((unsigned short)(q[j][i] >> 16)) * up * more);
+    to_score = scale * __builtin_ldexpf(1.0f, -near);
+    rest = __builtin_ldexpf(1.0f, near - (14 - e));
+}
+
 template <int TYPE, int QT, int D, int RT, Columns COLS, bool WINDOW>
 __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D * RT > 128) ? 2 : 1) void k_attn_rows(AttnArgs a) {
     using C = RowKernel<TYPE, QT, D, RT, COLS>;
@@ -508,30 +536,7 @@ __global__ __launch_bounds__(256, D <= 128 && TYPE != kF32 && !(TYPE == kQ8 && D
                 }
             }
             if constexpr (Q8 && QT == kBF16) {
-                // the largest of the row to 2^14 (eight bits of it: exact; others from 2^-28 of it on)
-                unsigned top = 0;
-#pragma unroll
-                for (int j = 0; j < C::NK; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const unsigned lo = q[r][j][i] & 0x7fffu, hi = q[r][j][i] >> 16 & 0x7fffu;
-                        top = lo > top ? lo : top;
-                        top = hi > top ? hi : top;
-                    }
-                top = max(top, (unsigned)__shfl_xor((int)top, 16));
-                top = max(top, (unsigned)__shfl_xor((int)top, 32));
-                int e = (int)(top >> 7) - 127;               // of the largest
-                if (top == 0 || top >= 0x7f80u) e = 14;      // nothing, or not finite: as it is
-                const int near = 14 - e > 100 ? 100 : 14 - e < -100 ? -100 : 14 - e;
-                const float up = __builtin_ldexpf(1.0f, near), more = __builtin_ldexpf(1.0f, 14 - e - near);
-#pragma unroll
-                for (int j = 0; j < C::NK; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        q[r][j][i] = pack2<kF16>(bf16_value((unsigned short)q[r][j][i]) * up * more,
-                                                 bf16_value((unsigned short)(q[r][j][i] >> 16)) * up * more);
-                to_score[r] = a.scale * __builtin_ldexpf(1.0f, -near);
-                rest[r] = __builtin_ldexpf(1.0f, near - (14 - e));
+                bf16_row_to_f16(q[r], a.scale, to_score[r], rest[r]);
             }
         }
         f4 acc[RT][C::NC];
@@ -1575,6 +1580,12 @@ int esize(int type) { return type == kF32 ? 4 : 2; }
 constexpr long long kMaxRows = 1 << 30, kMaxBlocks = (1 << 23) - 1;
 
 }  // namespace
+
+// 0, or the error of a window (NULL: none), of a cache call's arguments.
+int check_window(const kvc_window * w);
+int check_cache_attn(const kvc_cache * c, const kvc_cache_attn_args * a);
+// A cache call's arguments as kernels take them, but for a launch's shape.
+int cache_args(const kvc_cache * c, const kvc_cache_attn_args * x, const kvc_window * w, AttnArgs & a);
 
 // The forms with a window (a file of their own: compiled beside the others).
 bool run_attn_window(const AttnArgs & a, int type, int qt, int whole, int rt, bool careful, long long blocks, hipStream_t st);

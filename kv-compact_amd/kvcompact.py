@@ -413,6 +413,7 @@ def state_compact(dll, prefix, blob: bytes, params: StateParams, t_max: int):
 
 # -- paged cache and its attention (include/kvc-cache.h) ------------------
 CACHE_MAX_REQUESTS, REQ_BAD = 1024, -2
+HEADS_SUM, HEADS_MAX = 0, 1
 _ll = ctypes.c_longlong
 _f = ctypes.c_float
 
@@ -461,6 +462,17 @@ class Window(ctypes.Structure):
     _fields_ = [("first", _i), ("last", _i)]
 
 
+class WeighArgs(ctypes.Structure):
+    """kvc_weigh_args."""
+    _fields_ = [("weight", _vp), ("decay", _f), ("tail", _i), ("fresh", _i)]
+
+
+class PickArgs(ctypes.Structure):
+    """kvc_pick_args."""
+    _fields_ = [("seqs", _vp), ("start", _vp), ("keep", _vp), ("weight", _vp), ("idx", _vp), ("ld_idx", _ll), ("cu", _vp),
+                ("granted", _vp), ("status", _vp)] + [(n, _i) for n in ("n_idx", "recent", "heads", "max_len")]
+
+
 def bind_cache(dll):
     """Declare the entry points of include/kvc-cache.h. Device arrays go in as addresses (int or None), structs by
     reference (a ctypes instance is passed as one)."""
@@ -477,12 +489,16 @@ def bind_cache(dll):
             "kvc_attn_prompt": [P(PromptArgs), _vp],
             "kvc_attn_prompt_window": [P(PromptArgs), P(Window), _vp],
             "kvc_attn_cache_window": [P(KvCache), P(CacheAttnArgs), P(Window), _vp, sz, _vp],
+            "kvc_cache_weigh": [P(KvCache), P(CacheAttnArgs), P(Window), P(WeighArgs), _vp],
+            "kvc_cache_pick": [P(KvCache), _i, P(PickArgs), _vp, sz, _vp],
+            "kvc_cache_take_weights": [P(KvCache), _i, _vp, _vp, _vp, _vp, _i, _vp, _ll, _vp, _vp, _vp],
             "kvc_attn_cache": [P(KvCache), P(CacheAttnArgs), _vp, sz, _vp]}.items():
         f = getattr(dll, name)
         f.argtypes, f.restype = args, _i
     dll.kvc_cache_workspace.argtypes, dll.kvc_cache_workspace.restype = [P(KvCache), _i], sz
     dll.kvc_attn_cache_workspace.argtypes = [P(KvCache), P(CacheAttnArgs)]
     dll.kvc_attn_cache_workspace.restype = sz
+    dll.kvc_cache_pick_workspace.argtypes, dll.kvc_cache_pick_workspace.restype = [P(KvCache), _i, P(PickArgs)], sz
     dll.kvc_attn_cache_window_workspace.argtypes = [P(KvCache), P(CacheAttnArgs), P(Window)]
     dll.kvc_attn_cache_window_workspace.restype = sz
     return dll
