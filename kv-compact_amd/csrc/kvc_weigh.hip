@@ -228,6 +228,223 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
     }
 }
 
+// More rows of 16-bit types: a wave keeps the keys of 32 SUB cells in registers,
+// two waves a block's cells, and two the one half of a tile of 64 rows each, two
+// the other. Rows reach LDS by direct loads, three tiles ahead, pieces of 16
+// bytes exchanged by row % 8 as keys are in k_attn_tiles, whose fragments these
+// are: a lane holds a row's scores of 16 of 32 cells. A tile is whole tokens:
+// its rows' places are the same in every tile, and rows that are left over (or
+// past the last token) repeat its last row with a log-sum-exp of +inf.
+//
+// Without a bias the scores go into the exponential by one multiply-add (scale
+// and log2 e in one factor: each rounded once, as the separate steps are).
+__device__ const float nothing_word = INFINITY;
+
+template <int TYPE, int D, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
+    constexpr int SUB = D == 256 ? 1 : 2, CELLS = 64 * SUB;   // 32-cell parts of a wave; cells of a block
+    constexpr int ROWS = 64, KS = D / 16, CH = D / 8, ROWB = 2 * D;
+    constexpr int NL = ROWS * CH / 256, RPL = 512 / D;        // direct loads of a wave and tile; rows of one
+    constexpr int BUFS = D == 256 ? 2 : 4, AHEAD = BUFS - 1, LOADS = NL + 1;
+    __shared__ __align__(16) char lds[BUFS][ROWS * ROWB];
+    __shared__ float row_lse[BUFS][ROWS];
+    __shared__ float join[2][64];
+
+    const AttnArgs & a = w.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cw = wave & 1, rw = wave >> 1, n = lane & 31, hf = lane >> 5;
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    const int first_tile = u % w.cell_tiles, s = u / w.cell_tiles;
+    Counted c;
+    if (!counted_of(w, s, c)) return;
+    const Sequence & q = c.q;
+    const int page_mask = (1 << a.shift) - 1;
+    const int T = ROWS / a.G;                                 // tokens of a tile
+    const float to_log2 = a.scale * kLog2e;
+    // places of a tile's rows: this lane's, and those it loads
+    const int my_row = 32 * rw + n < T * a.G ? 32 * rw + n : T * a.G - 1;
+    const int my_tok = my_row / a.G;
+    int load_tok[NL];
+    unsigned load_off[NL];
+    bool load_on[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int at = (i * 4 + wave) * RPL + lane / CH, row = at < T * a.G ? at : T * a.G - 1;
+        const int piece = (lane % CH) ^ (at & 7);
+        load_tok[i] = row / a.G;
+        load_off[i] = (unsigned)(row % a.G) * (unsigned)(2 * a.q_head) + 16 * piece;
+        load_on[i] = 8 * piece < a.dk;
+    }
+    const int lse_row = 16 * wave + (lane & 15);              // (lanes 0 .. 15)
+    const int lse_tok = lse_row / a.G, lse_head = lse_row % a.G;
+    const bool lse_on = lse_row < T * a.G;
+
+    for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
+        const int block0 = tile * CELLS, cell0 = block0 + 32 * SUB * cw;
+        int t0, t1;   // the block's tokens, and the wave's
+        tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
+        int wt0, wt1;
+        tokens_of(a, c, cell0, cell0 + 32 * SUB < q.held ? cell0 + 32 * SUB : q.held, wt0, wt1);
+        if (cell0 >= q.held) wt1 = wt0;
+
+        auto fill = [&](int tt, int buf) {
+            if (tt >= t1) tt = t0 + (t1 - 1 - t0) / T * T;   // (past the last: like the last, for the count of loads)
+            const char * from = a.q + 2 * ((long long)(q.tok0 + tt) * a.q_tok + (long long)(h * a.G) * a.q_head);
+            const int most = t1 - 1 - tt;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int tk = load_tok[i] < most ? load_tok[i] : most;
+                if (load_on[i]) load_lds16(from, load_off[i] + __umul24(tk, (unsigned)(2 * a.q_tok)), &lds[buf][(i * 4 + wave) * 1024]);
+            }
+            const char * l = lse_on && lse_tok <= most
+                                 ? reinterpret_cast<const char *>(a.lse + (long long)(q.tok0 + tt + lse_tok) * a.H * a.G + h * a.G + lse_head)
+                                 : reinterpret_cast<const char *>(&nothing_word);
+            if (lane < 16) load_lds4(l, reinterpret_cast<char *>(&row_lse[buf][16 * wave]));
+        };
+
+        __syncthreads();   // (LDS of the last tile of cells is read)
+        if (a.dk < D) {
+            for (int i = threadIdx.x; i < BUFS * ROWS * CH; i += 256) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+            __syncthreads();
+        }
+        u4 kf[SUB][KS];
+        f16x bias[BIAS ? SUB : 1], sum[SUB];
+        unsigned there[SUB];   // cells of this lane's registers that rows may see
+#pragma unroll
+        for (int x = 0; x < SUB; x++) {
+            const int cell = cell0 + 32 * x + (n & 16);
+            int page = cell < q.held ? q.table[cell >> a.shift] : -1;
+            const bool good = page >= 0 && page < a.n_pages;
+            if (!good) page = 0;
+            const unsigned long long row = ((unsigned)page << a.shift) + ((cell + (n & 15)) & page_mask);
+            const char * p = a.k.base + h * a.k.ld_head + row * a.k.ld_tok + 16 * hf;
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+                kf[x][j] = 16 * j + 8 * hf < a.dk ? *reinterpret_cast<const u4 *>(p + 32 * j) : u4{0, 0, 0, 0};
+            const int left = q.held - cell0 - 32 * x;
+            const unsigned long long ok = __ballot(good);   // (lanes 0 and 16: the two groups of 16 cells)
+            there[x] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+            there[x] &= (ok & 1 ? 0xffffu : 0u) | (ok >> 16 & 1 ? 0xffff0000u : 0u);
+            if constexpr (BIAS) {
+                const int pages[2] = {__shfl(page, 0), __shfl(page, 16)};
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int at = cell0 + 32 * x + 8 * y + 4 * hf;
+                    const f4 b = *reinterpret_cast<const f4 *>(a.bias + (((long long)pages[y >> 1] * a.H + h) << a.shift) + (at & page_mask));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        bias[x][4 * y + i] = b[i];
+                        if (b[i] == -INFINITY) there[x] &= ~(1u << (8 * y + 4 * hf + i));
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) sum[x][i] = 0.0f;
+        }
+        if (t0 < t1) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) fill(t0 + i * T, i);
+        }
+        auto arrive = [&](int tt, int buf) {
+            wait_lds_loads<(AHEAD - 1) * LOADS>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            fill(tt + AHEAD * T, (buf + AHEAD) % BUFS);
+        };
+        auto step = [&](int tt, int buf, auto kind) {
+            constexpr bool PLAIN = decltype(kind)::value;
+            f16x sc[SUB];
+#pragma unroll
+            for (int x = 0; x < SUB; x++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) sc[x][i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const u4 qf = *reinterpret_cast<const u4 *>(&lds[buf][(32 * rw + n) * ROWB + (((2 * j + hf) ^ (n & 7)) << 4)]);
+#pragma unroll
+                for (int x = 0; x < SUB; x++) sc[x] = mfma32<TYPE>(kf[x][j], qf, sc[x]);
+            }
+            float lse = row_lse[buf][32 * rw + n];
+            if (lse == -INFINITY) lse = INFINITY;   // (a row that saw nothing gives nothing)
+            const float l2 = lse * kLog2e;
+            unsigned see[SUB];
+            if constexpr (!PLAIN) {
+                const int tok = tt + my_tok < t1 ? tt + my_tok : t1 - 1;
+                const int from = window_from(a, q, tok);
+#pragma unroll
+                for (int x = 0; x < SUB; x++)
+                    see[x] = (seen32(a, q, tok, cell0 + 32 * x) & window32(a, from, cell0 + 32 * x)) >> (4 * hf);
+            }
+#pragma unroll
+            for (int x = 0; x < SUB; x++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    // (with a bias the difference first: a score may be the type's lowest value)
+                    float p = BIAS ? exp_of(__builtin_fmaf(sc[x][i], a.scale, bias[BIAS ? x : 0][i]) - lse)
+                                   : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], to_log2, -l2));
+                    if constexpr (!PLAIN) p = see[x] >> (8 * (i >> 2) + (i & 3)) & 1 ? p : 0.0f;
+                    sum[x][i] += p;
+                }
+        };
+        // what the rows of a tile see of this wave's cells: nothing, all, or some
+        auto idle = [&](int tt) { return tt + T <= wt0 || tt >= wt1; };
+        auto whole = [&](int tt) {
+            const int last = tt + T < t1 ? tt + T : t1;
+            if (cell0 + 32 * SUB > (a.mask ? q.base : q.base + tt + 1)) return false;
+            const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last - a.last;
+            return !(cell0 + 32 * SUB > a.first && cell0 < from);
+        };
+        int tt = t0, buf = 0;
+        auto next = [&] {
+            tt += T;
+            buf = (buf + 1) % BUFS;
+        };
+        while (tt < t1) {
+            for (; tt < t1 && (idle(tt) || !whole(tt)); next()) {
+                arrive(tt, buf);
+                if (!idle(tt)) step(tt, buf, std::false_type{});
+            }
+            for (; tt < t1 && !idle(tt) && whole(tt); next()) {
+                arrive(tt, buf);
+                step(tt, buf, std::true_type{});
+            }
+        }
+        wait_lds_loads<0>();
+        // over a half's 32 lanes: each step hands half of the sums to the lane across, until each holds one cell's
+        float v[16 * SUB];
+#pragma unroll
+        for (int x = 0; x < SUB; x++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[16 * x + i] = there[x] >> (8 * (i >> 2) + 4 * hf + (i & 3)) & 1 ? sum[x][i] : 0.0f;
+#pragma unroll
+        for (int m = 8 * SUB; m; m >>= 1)
+#pragma unroll
+            for (int i = 0; i < m; i++) {
+                const float mine = n & m ? v[m + i] : v[i], theirs = n & m ? v[i] : v[m + i];
+                v[i] = mine + __shfl_xor(theirs, m);
+            }
+        if constexpr (SUB == 1) v[0] += __shfl_xor(v[0], 16);
+        if (rw == 1) join[cw][lane] = v[0];
+        __syncthreads();
+        if (rw == 0 && (SUB == 2 || n < 16)) {
+            const int i = n & 15;
+            add_weight(w, c, h, cell0 + 32 * (n >> 4) + 8 * (i >> 2) + 4 * hf + (i & 3), v[0] + join[cw][lane]);
+        }
+    }
+}
+
+template <int TYPE, int D> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
+    return w.a.bias ? launch(k_weigh_tiles<TYPE, D, true>, dim3((unsigned)blocks), dim3(256), st, w)
+                    : launch(k_weigh_tiles<TYPE, D, false>, dim3((unsigned)blocks), dim3(256), st, w);
+}
+template <int TYPE> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
+    if (w.a.dk <= 64) return run_weigh_tiles<TYPE, 64>(w, blocks, st);
+    if (w.a.dk <= 128) return run_weigh_tiles<TYPE, 128>(w, blocks, st);
+    return run_weigh_tiles<TYPE, 256>(w, blocks, st);
+}
+
 template <int TYPE, int QT, int D> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
     const dim3 grid((unsigned)blocks), block(256);
     if constexpr (TYPE != kQ8)
@@ -269,7 +486,12 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     w.fresh = y->fresh;
     const int es = esize(x->type);
     const bool careful = c->k_type != kQ8 && (!vec_rows(x->q, es) || c->d_k * es % 16);
-    const long long want = (x->max_len + 127LL) / 128, most = kMaxBlocks / ((long long)x->n_seq * c->n_head_kv);
+    // Rows by tiles in LDS where there are more than 16; where strides are what direct loads take.
+    const long long rows = (long long)(y->tail > 0 && y->tail < x->max_new ? y->tail : x->max_new) * a.G;
+    const bool tiles = rows > 16 && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
+                       x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23;
+    const int cells = tiles && c->d_k > 128 ? 64 : 128;   // of a block
+    const long long want = ((long long)x->max_len + cells - 1) / cells, most = kMaxBlocks / ((long long)x->n_seq * c->n_head_kv);
     if (most < 1) return KV_COMPACT_E_UNSUPPORTED;
     w.cell_tiles = (int)(want < 1 ? 1 : want < most ? want : most);
     w.a = a;
@@ -278,7 +500,8 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
     bool ok;
-    if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, careful, blocks, st);
+    if (tiles) ok = c->k_type == kF16 ? run_weigh_tiles<kF16>(w, blocks, st) : run_weigh_tiles<kBF16>(w, blocks, st);
+    else if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, careful, blocks, st);
     else if (c->k_type == kF16) ok = run_weigh<kF16, kF16>(w, careful, blocks, st);
     else if (c->k_type == kBF16) ok = run_weigh<kBF16, kBF16>(w, careful, blocks, st);
     else if (x->type == kF16) ok = run_weigh<kQ8, kF16>(w, careful, blocks, st);
