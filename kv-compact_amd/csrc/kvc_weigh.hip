@@ -25,6 +25,7 @@ struct WeighArgs {
     float decay;
     int tail, fresh;
     int cell_tiles;        // blocks of a sequence's head
+    int range;             // k_weigh_few: groups of 32 cells of each, at least
 };
 
 // What a block of a call works on.
@@ -226,6 +227,296 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
             }
         if (m < 8) add_weight(w, c, h, cell0 + 16 * (m >> 2) + 4 * g + (m & 3), mine);
     }
+}
+
+// Few rows: 16 RT of them stay (RT = 1: in registers, more in LDS as the
+// fragments they are), and a block's waves go through a range of cells, 32 at a
+// time, the next ones' keys, biases and old weights on their way meanwhile.
+// (More rows than the launch was told of come in turns of as many; a cell's
+// weight is then added to by the lane that wrote it.)
+constexpr int kFewRows16 = 8, kFewRows32 = 4;   // row tiles of 16 that stay, of 16-bit and F32 rows
+
+// Sum over the 16 lanes of a row of v[m % 8] (lanes m and m ^ 8 alike): each
+// step hands half of the values to the lane across.
+__device__ __forceinline__ float sum_of_16(float (&v)[8], int m) {
+    auto dpp = [](float x, auto ctrl) {
+        constexpr int c = decltype(ctrl)::value;
+        return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), c, 0xf, 0xf, true));
+    };
+    using half_mirror = std::integral_constant<int, 0x141>;
+    using xor2 = std::integral_constant<int, 0x4e>;
+    using xor1 = std::integral_constant<int, 0xb1>;
+    using ror8 = std::integral_constant<int, 0x128>;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float mine = m & 4 ? v[4 + i] : v[i], theirs = m & 4 ? v[i] : v[4 + i];
+        v[i] = mine + dpp(theirs, half_mirror{});
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float mine = m & 2 ? v[2 + i] : v[i], theirs = m & 2 ? v[i] : v[2 + i];
+        v[i] = mine + dpp(theirs, xor2{});
+    }
+    const float mine = m & 1 ? v[1] : v[0], theirs = m & 1 ? v[0] : v[1];
+    const float x = mine + dpp(theirs, xor1{});
+    return x + dpp(x, ror8{});
+}
+
+template <int TYPE, int QT, int D, int RT, Columns COLS>
+__global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
+    using C = RowKernel<TYPE, QT, D, 1, COLS>;
+    constexpr bool Q8 = C::Q8;
+    constexpr int NS = Q8 ? (C::NB + 3) / 4 : 1;              // scales a lane loads of a group of 16 cells
+    constexpr bool AHEAD = 2 * C::NKL * C::WK <= 64;          // the next keys have registers of their own
+    __shared__ __align__(16) u4 rows_q[RT > 1 ? RT : 1][RT > 1 ? C::NK : 1][64];
+    __shared__ float rows_scale[RT > 1 && Q8 ? RT : 1][2][16];
+    __shared__ float rows_lse[RT > 1 ? RT : 1][16];
+    __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
+    const AttnArgs & a = w.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    const int split = u % w.cell_tiles, s = u / w.cell_tiles;
+    Counted c;
+    if (!counted_of(w, s, c)) return;
+    const Sequence & q = c.q;
+    const int page_mask = (1 << a.shift) - 1;
+    const int all_rows = (q.n_new - c.tok_from) * a.G;
+    const int n_groups = (q.held + 31) >> 5;
+    const int even = (n_groups + w.cell_tiles - 1) / w.cell_tiles, per = even > w.range ? even : w.range;
+    const int g_lo = split * per, g_hi = g_lo + per < n_groups ? g_lo + per : n_groups;
+    if (g_lo >= g_hi) return;
+
+    // row `row` of a turn's (those past the last repeat it, and give nothing)
+    int row_lo = 0, rows = 0;
+    auto load_row = [&](int row, u4 (&x)[C::NK], float & lse, float & scale, float & rest) {
+        const bool on = row < rows;
+        row = row_lo + (on ? row : rows - 1);
+        const int tok = c.tok_from + row / a.G, head = row % a.G;
+        const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
+#pragma unroll
+        for (int j = 0; j < C::NK; j++) {
+            const int col = 4 * C::KV * j + C::KV * g;
+            if constexpr (Q8) {
+                x[j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
+            } else {
+                unsigned y[4];
+                load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, y);
+                x[j] = u4{y[0], y[1], y[2], y[3]};
+            }
+        }
+        scale = a.scale;
+        rest = 1.0f;
+        if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(x, a.scale, scale, rest);
+        lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
+        lse = on && lse != -INFINITY ? lse : INFINITY;
+    };
+
+    unsigned kr[2][C::NKL][C::WK], next_kr[AHEAD ? 2 : 1][AHEAD ? C::NKL : 1][C::WK];
+    f4 bias[2], next_bias[2];
+    float old = 0.0f, next_old = 0.0f;
+    unsigned short scales[2][NS];
+    int page[2], next_page[2];
+    const int out_at = 16 * (m >> 2 & 1) + 4 * g + (m & 3);   // the cell of a group whose sum this lane (m < 8) gets
+    auto pages_of = [&](int t, int (&pg)[2]) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int cell = 32 * t + 16 * x;
+            pg[x] = t < g_hi && cell < q.held ? uniform_load(q.table + (cell >> a.shift)) : -1;
+        }
+    };
+    auto good = [&](int pg) { return pg >= 0 && pg < a.n_pages; };
+    auto load_keys = [&](int t, const int (&pg)[2], auto & to) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int cell = 32 * t + 16 * x, pg_x = good(pg[x]) ? pg[x] : 0;
+            const unsigned row0 = ((unsigned)pg_x << a.shift) + (cell & page_mask);
+            const char * p = a.k.base + h * a.k.ld_head + (unsigned long long)row0 * a.k.ld_tok;
+            const unsigned row = __umul24(m, a.k.ld_tok);
+#pragma unroll
+            for (int j = 0; j < C::NKL; j++) {
+                if constexpr (Q8)
+                    *reinterpret_cast<u2 *>(to[x][j]) =
+                        COLS == FULL || 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + (row + 34 * j + 2 + 8 * g)) : u2{0, 0};
+                else
+                    load_cols<C::KV, C::ES, COLS>(p, row, 4 * C::KV * j + C::KV * g, a.dk, to[x][j]);
+            }
+            if constexpr (Q8) {
+                // lane g * 16 + m: blocks g, g + 4, ... of cell m
+#pragma unroll
+                for (int b = 0; b < NS; b++) {
+                    const int at = 4 * b + g;
+                    scales[x][b] = at < C::NB && (COLS == FULL || 32 * at < a.dk) ? *reinterpret_cast<const unsigned short *>(p + row + 34 * at) : 0;
+                }
+            }
+            if (a.bias) next_bias[x] = *reinterpret_cast<const f4 *>(a.bias + (((long long)pg_x * a.H + h) << a.shift) + ((cell + 4 * g) & page_mask));
+        }
+        const int cell = 32 * t + out_at;
+        next_old = 0.0f;
+        if (m < 8 && (row_lo ? cell < q.held : w.decay != 0.0f && cell < c.old)) next_old = w.weight[c.seq * w.w_seq + h * w.room + cell];
+    };
+
+    for (; row_lo < all_rows; row_lo += 16 * RT) {
+        rows = all_rows - row_lo < 16 * RT ? all_rows - row_lo : 16 * RT;
+        const int row_tiles = (rows + 15) >> 4, t0 = g_lo + wave;
+        pages_of(t0, page);
+        pages_of(t0 + 4, next_page);
+        if constexpr (AHEAD)
+            if (t0 < g_hi) load_keys(t0, page, next_kr);
+        u4 q0[C::NK];
+        float lse0 = 0.0f, scale0 = 0.0f, rest0 = 0.0f;
+        if constexpr (RT == 1) {
+            load_row(m, q0, lse0, scale0, rest0);
+        } else {
+            if (row_lo) __syncthreads();   // (the rows before are read)
+            for (int r = wave; r < row_tiles; r += 4) {
+                load_row(16 * r + m, q0, lse0, scale0, rest0);
+#pragma unroll
+                for (int j = 0; j < C::NK; j++) rows_q[r][j][lane] = q0[j];
+                if (g == 0) {
+                    rows_lse[r][m] = lse0;
+                    if constexpr (Q8) {
+                        rows_scale[r][0][m] = scale0;
+                        rows_scale[r][1][m] = rest0;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+
+        for (int t = t0; t < g_hi; t += 4) {
+            const int cell0 = 32 * t;
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int j = 0; j < C::NKL; j++)
+#pragma unroll
+                        for (int y = 0; y < C::WK; y++) kr[x][j][y] = next_kr[x][j][y];
+            } else {
+                load_keys(t, page, kr);
+            }
+            unsigned there = 0;   // cells that rows may see
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                bias[x] = next_bias[x];
+                const int left = q.held - cell0 - 16 * x;
+                if (good(page[x])) there |= (left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1) << (16 * x);
+                if (a.bias)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (bias[x][i] == -INFINITY) there &= ~(1u << (16 * x + 4 * g + i));
+                if constexpr (Q8)
+#pragma unroll
+                    for (int b = 0; b < NS; b++)
+                        if (4 * b + g < C::NB) k_scale[wave][4 * b + g][16 * x + m] = f16_value(scales[x][b]);
+            }
+            old = next_old;
+            if constexpr (AHEAD) {
+                if (t + 4 < g_hi) load_keys(t + 4, next_page, next_kr);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) page[x] = next_page[x];
+            pages_of(t + 8, next_page);
+            if constexpr (Q8) {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            }
+            float sum[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum[i] = 0.0f;
+            for (int r = 0; r < (RT == 1 ? 1 : row_tiles); r++) {
+                const int row0 = 16 * r, last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
+                const int first_tok = c.tok_from + (row_lo + row0) / a.G, last_tok = c.tok_from + (row_lo + last_row) / a.G;
+                u4 qr[C::NK];
+                float lse = lse0, scale = scale0, rest = rest0;
+                if constexpr (RT > 1) {
+#pragma unroll
+                    for (int j = 0; j < C::NK; j++) qr[j] = rows_q[r][j][lane];
+                    lse = rows_lse[r][m];
+                    scale = a.scale;
+                    if constexpr (Q8) {
+                        scale = rows_scale[r][0][m];
+                        rest = rows_scale[r][1][m];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C::NK; j++) qr[j] = q0[j];
+                }
+                const int clear = a.mask ? q.base : q.base + first_tok + 1;
+                const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
+                const bool special = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
+                unsigned see = ~0u;
+                if (special) {
+                    const int row = row0 + m < rows ? row0 + m : rows - 1, tok = c.tok_from + (row_lo + row) / a.G;
+                    see = seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    f4 sc = {0, 0, 0, 0};
+                    if constexpr (TYPE == kF32) {
+                        f4 part[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) part[e] = f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < C::NKL; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][j][e]),
+                                                                               __uint_as_float(qr[j][e]), part[e], 0, 0, 0);
+                        sc = (part[0] + part[1]) + (part[2] + part[3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
+                        if constexpr (Q8) {
+                            unsigned y[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                y[e] = code_pair(kr[x][j][e >> 1], kr[x][j][e >> 1], e & 1 ? 0x0c030c02u : 0x0c010c00u);
+                            const f4 f = *reinterpret_cast<const f4 *>(&k_scale[wave][j][16 * x + 4 * g]);
+                            sc += f * mfma16<kF16>(u4{y[0], y[1], y[2], y[3]}, qr[j], f4{0, 0, 0, 0});
+                        } else {
+                            sc = mfma16<C::MT>(u4{kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]}, qr[j], sc);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
+                        float v = sc[i] * scale;
+                        if constexpr (Q8 && QT == kBF16) v *= rest;
+                        if (a.bias) v += bias[x][i];
+                        const float p = exp_of(v - lse);
+                        sum[4 * x + i] += see >> (16 * x + 4 * g + i) & 1 ? p : 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
+            const float all = sum_of_16(sum, m);
+            const int cell = cell0 + out_at;
+            if (m < 8 && cell < q.held) w.weight[c.seq * w.w_seq + h * w.room + cell] = (row_lo ? old : w.decay * old) + all;
+        }
+    }
+}
+
+template <int TYPE, int QT, int D, int RT> bool run_weigh_few(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks), block(256);
+    if constexpr (TYPE != kQ8)
+        if (careful) return launch(k_weigh_few<TYPE, QT, D, RT, ANY>, grid, block, st, w);
+    if (w.a.dk == D) return launch(k_weigh_few<TYPE, QT, D, RT, FULL>, grid, block, st, w);
+    return launch(k_weigh_few<TYPE, QT, D, RT, PART>, grid, block, st, w);
+}
+template <int TYPE, int QT, int RT> bool run_weigh_few(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
+    if (w.a.dk <= 64) return run_weigh_few<TYPE, QT, 64, RT>(w, careful, blocks, st);
+    if (w.a.dk <= 128) return run_weigh_few<TYPE, QT, 128, RT>(w, careful, blocks, st);
+    return run_weigh_few<TYPE, QT, 256, RT>(w, careful, blocks, st);
+}
+template <int TYPE, int QT> bool run_weigh_few(const WeighArgs & w, long long rows, bool careful, long long blocks, hipStream_t st) {
+    if (rows <= 16) return run_weigh_few<TYPE, QT, 1>(w, careful, blocks, st);
+    return run_weigh_few<TYPE, QT, TYPE == kF32 ? kFewRows32 : kFewRows16>(w, careful, blocks, st);
 }
 
 // More rows of 16-bit types: a wave keeps the keys of 32 SUB cells in registers,
@@ -486,22 +777,34 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     w.fresh = y->fresh;
     const int es = esize(x->type);
     const bool careful = c->k_type != kQ8 && (!vec_rows(x->q, es) || c->d_k * es % 16);
-    // Rows by tiles in LDS where there are more than 16; where strides are what direct loads take.
     const long long rows = (long long)(y->tail > 0 && y->tail < x->max_new ? y->tail : x->max_new) * a.G;
-    const bool tiles = rows > 16 && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
+    const bool few = rows <= 16 * (c->k_type == kF32 ? kFewRows32 : kFewRows16);
+    // (strides that direct loads take)
+    const bool tiles = !few && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
                        x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23;
     const int cells = tiles && c->d_k > 128 ? 64 : 128;   // of a block
-    const long long want = ((long long)x->max_len + cells - 1) / cells, most = kMaxBlocks / ((long long)x->n_seq * c->n_head_kv);
+    const long long units = (long long)x->n_seq * c->n_head_kv;
+    long long want = ((long long)x->max_len + cells - 1) / cells;
+    const long long most = kMaxBlocks / units;
     if (most < 1) return KV_COMPACT_E_UNSUPPORTED;
+    if (few && want > (4095 + units) / units) want = (4095 + units) / units;
     w.cell_tiles = (int)(want < 1 ? 1 : want < most ? want : most);
+    w.range = (int)(((long long)x->max_len + 32LL * w.cell_tiles - 1) / (32LL * w.cell_tiles));
     w.a = a;
-    const long long blocks = (long long)x->n_seq * c->n_head_kv * w.cell_tiles;
+    const long long blocks = units * w.cell_tiles;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
     bool ok;
-    if (tiles) ok = c->k_type == kF16 ? run_weigh_tiles<kF16>(w, blocks, st) : run_weigh_tiles<kBF16>(w, blocks, st);
-    else if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, careful, blocks, st);
+    if (few) {
+        if (c->k_type == kF32) ok = run_weigh_few<kF32, kF32>(w, rows, careful, blocks, st);
+        else if (c->k_type == kF16) ok = run_weigh_few<kF16, kF16>(w, rows, careful, blocks, st);
+        else if (c->k_type == kBF16) ok = run_weigh_few<kBF16, kBF16>(w, rows, careful, blocks, st);
+        else if (x->type == kF16) ok = run_weigh_few<kQ8, kF16>(w, rows, careful, blocks, st);
+        else ok = run_weigh_few<kQ8, kBF16>(w, rows, careful, blocks, st);
+    } else if (tiles) {
+        ok = c->k_type == kF16 ? run_weigh_tiles<kF16>(w, blocks, st) : run_weigh_tiles<kBF16>(w, blocks, st);
+    } else if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, careful, blocks, st);
     else if (c->k_type == kF16) ok = run_weigh<kF16, kF16>(w, careful, blocks, st);
     else if (c->k_type == kBF16) ok = run_weigh<kBF16, kBF16>(w, careful, blocks, st);
     else if (x->type == kF16) ok = run_weigh<kQ8, kF16>(w, careful, blocks, st);
