@@ -30,7 +30,8 @@ struct PickArgs {
     int * cu;
     int * granted;
     int * status;
-    unsigned * keys;       // [groups][n][max_len]
+    unsigned * keys;       // [groups][n][stride]
+    long long stride;      // max_len, in whole fours
     int n, n_idx, recent, max_len, max_seqs, H, n_layers, groups, most;
     int parts;             // blocks of a unit's keys
     long long room;        // cells of a row of weights
@@ -44,46 +45,73 @@ __device__ __forceinline__ int cells_of(const PickArgs & p, int i) {
     return start < 0 || start > len || len > p.max_len || len > p.room || p.keep[i] < 0 ? -1 : len - start;
 }
 
+// (0 is left for what is no cell of the choice)
 __device__ __forceinline__ unsigned key_of(float x) {
-    if (x != x) return 0;
+    if (x != x) return 1;
     const unsigned u = __float_as_uint(x + 0.0f);   // (-0 is 0)
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Four cells a thread.
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// A request's cells as a unit works on them.
+struct Unit {
+    int seq, start, len, stay;   // cells at or past `stay` are kept whatever they gathered
+    int l0, l1;                  // layers
+    const float * weight;        // layer l0's, head 0
+};
+__device__ __forceinline__ Unit unit_of(const PickArgs & p, int i, int group, int kept) {
+    Unit u;
+    u.seq = p.seqs[i];
+    u.start = p.start[i];
+    u.len = p.len[u.seq];
+    u.stay = u.len - (p.recent < kept ? p.recent : kept);
+    u.l0 = p.groups == 1 ? 0 : group;
+    u.l1 = p.groups == 1 ? p.n_layers : group + 1;
+    u.weight = p.weight + ((long long)u.l0 * p.max_seqs + u.seq) * p.H * p.room;
+    return u;
+}
+
+// Keys of cells c .. c+3 (c a multiple of 4, below the length).
+__device__ __forceinline__ u4 keys_at(const PickArgs & p, const Unit & u, int c) {
+    u4 k = {0, 0, 0, 0};
+    if (c + 4 <= u.start) return k;
+    double sum[4] = {0, 0, 0, 0};
+    f4 top = {NAN, NAN, NAN, NAN};
+    for (int l = u.l0; l < u.l1; l++) {
+        // (a row is whole pages: four cells at a time)
+        const float * w = u.weight + (long long)(l - u.l0) * p.max_seqs * p.H * p.room + c;
+        if (p.most) {
+#pragma unroll 8
+            for (int h = 0; h < p.H; h++) {
+                const f4 x = *reinterpret_cast<const f4 *>(w + h * p.room);
+#pragma unroll
+                for (int j = 0; j < 4; j++) top[j] = fmaxf(top[j], x[j]);
+            }
+        } else {
+#pragma unroll 8
+            for (int h = 0; h < p.H; h++) {
+                const f4 x = *reinterpret_cast<const f4 *>(w + h * p.room);
+#pragma unroll
+                for (int j = 0; j < 4; j++) sum[j] += x[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (c + j >= u.start && c + j < u.len) k[j] = c + j >= u.stay ? kAlways : key_of(p.most ? top[j] : (float)sum[j]);
+    return k;
+}
+
+// The keys by themselves, for few units of many cells. Four cells a thread.
 __global__ __launch_bounds__(256) void k_cell_keys(PickArgs p) {
     const int part = blockIdx.x % p.parts, i = blockIdx.x / p.parts % p.n, group = blockIdx.x / p.parts / p.n;
     const int cells = cells_of(p, i);
     if (cells <= 0) return;
-    const int seq = p.seqs[i], start = p.start[i], len = start + cells;
-    const int kept = p.keep[i] < cells ? p.keep[i] : cells;
-    const int stay = len - (p.recent < kept ? p.recent : kept);
-    const int l0 = p.groups == 1 ? 0 : group, l1 = p.groups == 1 ? p.n_layers : group + 1;
-    for (int c = (part * 256 + (int)threadIdx.x) * 4; c < len; c += p.parts * 1024) {
-        if (c + 4 <= start) continue;
-        double sum[4] = {0, 0, 0, 0};
-        float top[4] = {NAN, NAN, NAN, NAN};
-        for (int l = l0; l < l1; l++) {
-            const float * w = p.weight + ((long long)l * p.max_seqs + seq) * p.H * p.room + c;
-            for (int h = 0; h < p.H; h++) {
-                const float4 x = *reinterpret_cast<const float4 *>(w + h * p.room);   // (a row is whole pages)
-                if (p.most) {
-                    top[0] = fmaxf(top[0], x.x);
-                    top[1] = fmaxf(top[1], x.y);
-                    top[2] = fmaxf(top[2], x.z);
-                    top[3] = fmaxf(top[3], x.w);
-                } else {
-                    sum[0] += x.x;
-                    sum[1] += x.y;
-                    sum[2] += x.z;
-                    sum[3] += x.w;
-                }
-            }
-        }
-        unsigned * out = p.keys + ((long long)group * p.n + i) * p.max_len;
-        for (int j = 0; j < 4; j++)
-            if (c + j < len) out[c + j] = c + j >= stay ? kAlways : key_of(p.most ? top[j] : (float)sum[j]);
-    }
+    const Unit u = unit_of(p, i, group, p.keep[i] < cells ? p.keep[i] : cells);
+    u4 * out = reinterpret_cast<u4 *>(p.keys + ((long long)group * p.n + i) * p.stride);
+    for (int c = (part * 256 + (int)threadIdx.x) * 4; c < u.len; c += p.parts * 1024) out[c >> 2] = keys_at(p, u, c);
 }
 
 // Sum of v over the block's threads before this one; *total the whole sum.
@@ -106,26 +134,54 @@ template <class T> __device__ T pick_scan(T v, T * lds, T * total) {
     return before + x - v;
 }
 
-// A block per request and group of layers.
-__global__ __launch_bounds__(kPick) void k_pick(PickArgs p) {
-    __shared__ int lds[kWaves], kept_of[kPick], first[kPick], bins[256];
+// What request i keeps (-1: it is refused) and where its indices begin, from
+// all requests of the call. Up to 64 by each wave by itself.
+__device__ void plan_of(const PickArgs & p, int i, int & k, int & to) {
     __shared__ long long sums[kWaves];
-    __shared__ int found[2];
-    const int t = threadIdx.x, i = blockIdx.x % p.n, group = blockIdx.x / p.n;
-    // every block goes through the requests: what they keep (-1: refused), and where their indices begin
-    int kept = -1;
+    __shared__ int ids[kPick], kept_of[kPick], first[kPick];
+    const int t = p.n <= 64 ? threadIdx.x & 63 : threadIdx.x;
+    int kept = -1, seq = -1;
     if (t < p.n) {
         const int cells = cells_of(p, t);
+        seq = p.seqs[t];
         kept = cells < 0 ? -1 : p.keep[t] < cells ? p.keep[t] : cells;
         if (kept > p.n_idx) kept = -1;
-        for (int j = 0; j < t && kept >= 0; j++)
-            if (p.seqs[j] == p.seqs[t]) kept = -1;
     }
+    if (p.n <= 64) {
+        for (int j = 0; j < p.n; j++) {
+            const int other = __shfl(seq, j);   // (all lanes)
+            if (j < t && other == seq) kept = -1;
+        }
+        long long at = kept > 0 ? kept : 0;
+        const long long mine = at;
+        for (int o = 1; o < 64; o <<= 1) {
+            const long long y = __shfl_up(at, o);
+            if (t >= o) at += y;
+        }
+        if (__shfl(at, 63) <= p.n_idx) {
+            k = __shfl(kept, i);
+            to = (int)__shfl(at - mine, i);
+            return;
+        }
+        // (rare) in order, each that still fits
+        int used = 0;
+        for (int j = 0; j <= i; j++) {
+            k = __shfl(kept, j);
+            to = used;
+            if (k > p.n_idx - used) k = -1;
+            if (k > 0) used += k;
+        }
+        return;
+    }
+    ids[t] = seq;
+    __syncthreads();
+    for (int j = 0; j < t && kept >= 0; j++)
+        if (ids[j] == seq) kept = -1;
     long long total;
     first[t] = (int)pick_scan((long long)(kept > 0 ? kept : 0), sums, &total);
     kept_of[t] = kept;
     __syncthreads();
-    if (total > p.n_idx) {   // (rare) in order, each that still fits
+    if (total > p.n_idx) {
         if (t == 0) {
             int used = 0;
             for (int j = 0; j < p.n; j++) {
@@ -136,7 +192,24 @@ __global__ __launch_bounds__(kPick) void k_pick(PickArgs p) {
         }
         __syncthreads();
     }
-    const int k = kept_of[i], to = first[i];
+    k = kept_of[i];
+    to = first[i];
+}
+
+// A block per request and group of layers. Its waves have neighbouring
+// stretches of the cells, a thread four cells at a time, the same ones in every
+// pass: what it writes it alone reads again. FUSED: the keys are worked out on
+// the way of the first pass.
+//
+// The k-th largest key by its bits from the top, 11, 11 and 10 of them: the
+// first 11 are sign, exponent and two bits more, which keeps the lanes of a wave
+// in different places of the histogram where eight bits would not.
+template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArgs p) {
+    __shared__ int lds[kWaves], bins[2048], found[2], above[kWaves], same[kWaves];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int i = blockIdx.x % p.n, group = blockIdx.x / p.n;
+    int k, to;
+    plan_of(p, i, k, to);
     if (group == 0 && t == 0) {
         p.status[i] = k < 0 ? KVC_REQ_BAD : 0;
         p.granted[i] = k < 0 ? -1 : p.seqs[i];
@@ -144,43 +217,103 @@ __global__ __launch_bounds__(kPick) void k_pick(PickArgs p) {
         if (i == 0) p.cu[0] = 0;
     }
     if (k <= 0) return;
-    const int start = p.start[i], len = p.len[p.seqs[i]];
-    const unsigned * keys = p.keys + ((long long)group * p.n + i) * p.max_len;
-    // the k-th largest key, a byte at a time
+    const Unit u = unit_of(p, i, group, k);
+    const int turns = (u.len + 4 * kPick - 1) / (4 * kPick);   // of 256 cells a wave
+    const int c0 = wave * turns * 256 + 4 * lane;
+    u4 * keys = reinterpret_cast<u4 *>(p.keys + ((long long)group * p.n + i) * p.stride);
+
     unsigned top = 0;
-    int left = k;   // of the keys that begin with top's bytes, how many are kept
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) bins[t] = 0;
+    int left = k;   // of the keys that begin with top's bits, how many are kept
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        bins[t] = 0;
+        bins[t + kPick] = 0;
         __syncthreads();
-        for (int c = start + t; c < len; c += kPick) {
-            const unsigned u = keys[c];
-            if (shift == 24 || u >> (shift + 8) == top >> (shift + 8)) atomicAdd(&bins[u >> shift & 255], 1);
+        for (int y = 0; y < turns; y++) {
+            const int c = c0 + 256 * y;
+            if (c >= u.len) break;
+            u4 x;
+            if (FUSED && pass == 0) {
+                x = keys_at(p, u, c);
+                keys[c >> 2] = x;
+            } else {
+                x = keys[c >> 2];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool in = x[j] != 0 && (pass == 0 || x[j] >> (shift + bits) == top >> (shift + bits));
+                const int b = x[j] >> shift & ((1 << bits) - 1);
+                // (many alike: one addition for the lanes that agree with the first)
+                const unsigned long long who = __ballot(in);
+                if (!who) continue;
+                const int lead = __ffsll((long long)who) - 1, b0 = __shfl(b, lead);
+                const unsigned long long with = __ballot(in && b == b0);
+                if (lane == lead) atomicAdd(&bins[b0], __popcll(with));
+                if (in && b != b0) atomicAdd(&bins[b], 1);
+            }
         }
         __syncthreads();
-        if (t == 0) {
-            int b = 255, more = left;
-            while (more > bins[b]) more -= bins[b--];
-            found[0] = b;
-            found[1] = more;
+        // from the top: thread t has places 2 t and 2 t + 1
+        const int n0 = bins[2047 - 2 * t], n1 = bins[2046 - 2 * t];
+        int all;
+        const int before = pick_scan(n0 + n1, lds, &all);
+        if (before < left && left <= before + n0 + n1) {
+            const bool second = left > before + n0;
+            found[0] = 2047 - 2 * t - second;
+            found[1] = left - before - (second ? n0 : 0);
         }
         __syncthreads();
         top |= (unsigned)found[0] << shift;
         left = found[1];
         __syncthreads();
     }
+    // how many of each wave are above it, and equal to it
+    int n_above = 0, n_same = 0;
+    for (int y = 0; y < turns; y++) {
+        const int c = c0 + 256 * y;
+        const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            n_above += __popcll(__ballot(x[j] > top));
+            n_same += __popcll(__ballot(x[j] == top));
+        }
+    }
+    if (lane == 0) {
+        above[wave] = n_above;
+        same[wave] = n_same;
+    }
+    __syncthreads();
+    int done = 0, equal = 0;   // kept, and equal to top, before this wave's cells
+    for (int j = 0; j < wave; j++) {
+        done += above[j];
+        equal += same[j];
+    }
+    done += equal < left ? equal : left;
     int * out = p.idx + group * p.ld_idx + to;
-    int done = 0, equal = 0;
-    for (int c0 = start; c0 < len; c0 += kPick) {
-        const int c = c0 + t;
-        const unsigned u = c < len ? keys[c] : 0;
-        const int same = c < len && u == top;
-        int all;
-        const int nth = equal + pick_scan(same, lds, &all);
-        equal += all;
-        const int stays = c < len && (u > top || (same && nth < left));
-        const int where = done + pick_scan(stays, lds, &all);
-        done += all;
-        if (stays) out[where] = c - start;
+    const unsigned long long before = (1ull << lane) - 1;
+    for (int y = 0; y < turns; y++) {
+        const int c = c0 + 256 * y;
+        const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+        int nth = equal, where = done;
+        unsigned long long alike[4], kept[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            alike[j] = __ballot(x[j] == top);
+            nth += __popcll(alike[j] & before);
+            equal += __popcll(alike[j]);
+        }
+        bool stays[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            stays[j] = x[j] > top || (x[j] == top && nth < left);
+            nth += x[j] == top;
+            kept[j] = __ballot(stays[j]);
+            where += __popcll(kept[j] & before);
+            done += __popcll(kept[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (stays[j]) out[where++] = c + j - u.start;
     }
 }
 
@@ -274,7 +407,7 @@ extern "C" {
 
 size_t kvc_cache_pick_workspace(const kvc_cache * c, int n, const kvc_pick_args * a) {
     if (check_pick(c, n, a) || n == 0) return 0;
-    return sizeof(unsigned) * (size_t)(a->ld_idx ? c->n_layers : 1) * n * pick_cells(c, a);
+    return sizeof(unsigned) * (size_t)(a->ld_idx ? c->n_layers : 1) * n * ((pick_cells(c, a) + 3LL) & ~3LL);
 }
 
 int kvc_cache_pick(const kvc_cache * c, int n, const kvc_pick_args * a, void * ws, size_t ws_bytes, void * stream) {
@@ -290,17 +423,20 @@ int kvc_cache_pick(const kvc_cache * c, int n, const kvc_pick_args * a, void * w
     p.seqs = a->seqs; p.start = a->start; p.keep = a->keep; p.len = c->len; p.weight = a->weight;
     p.idx = a->idx; p.ld_idx = a->ld_idx; p.cu = a->cu; p.granted = a->granted; p.status = a->status;
     p.keys = static_cast<unsigned *>(ws);
+    p.stride = (pick_cells(c, a) + 3LL) & ~3LL;
     p.n = n; p.n_idx = a->n_idx; p.recent = a->recent; p.max_len = pick_cells(c, a); p.max_seqs = c->max_seqs;
     p.H = c->n_head_kv; p.n_layers = c->n_layers; p.groups = a->ld_idx ? c->n_layers : 1; p.most = a->heads == KVC_HEADS_MAX;
     p.room = (long long)c->max_pages * c->page_size;
     const int units = p.groups * n;
-    const int want = p.max_len / 1024 + 1, most = (1 << 22) / units;
-    p.parts = want < most ? want : most;
+    const long long want = p.max_len / 1024 + 1, most = (1 << 22) / units;
+    p.parts = (int)(want < most ? want : most);
+    const bool fused = units >= 32;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
+    if (fused) return launch(k_pick<true>, dim3((unsigned)units), dim3(kPick), st, p) ? 0 : KV_COMPACT_E_DEVICE;
     if (!launch(k_cell_keys, dim3((unsigned)(units * p.parts)), dim3(256), st, p) ||
-        !launch(k_pick, dim3((unsigned)units), dim3(kPick), st, p))
+        !launch(k_pick<false>, dim3((unsigned)units), dim3(kPick), st, p))
         return KV_COMPACT_E_DEVICE;
     return 0;
 }
