@@ -61,11 +61,11 @@ struct Unit {
     int l0, l1;                  // layers
     const float * weight;        // layer l0's, head 0
 };
-__device__ __forceinline__ Unit unit_of(const PickArgs & p, int i, int group, int kept) {
+__device__ __forceinline__ Unit unit_of(const PickArgs & p, int seq, int start, int len, int group, int kept) {
     Unit u;
-    u.seq = p.seqs[i];
-    u.start = p.start[i];
-    u.len = p.len[u.seq];
+    u.seq = seq;
+    u.start = start;
+    u.len = len;
     u.stay = u.len - (p.recent < kept ? p.recent : kept);
     u.l0 = p.groups == 1 ? 0 : group;
     u.l1 = p.groups == 1 ? p.n_layers : group + 1;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void k_cell_keys(PickArgs p) {
     const int part = blockIdx.x % p.parts, i = blockIdx.x / p.parts % p.n, group = blockIdx.x / p.parts / p.n;
     const int cells = cells_of(p, i);
     if (cells <= 0) return;
-    const Unit u = unit_of(p, i, group, p.keep[i] < cells ? p.keep[i] : cells);
+    const Unit u = unit_of(p, p.seqs[i], p.start[i], p.start[i] + cells, group, p.keep[i] < cells ? p.keep[i] : cells);
     u4 * out = reinterpret_cast<u4 *>(p.keys + ((long long)group * p.n + i) * p.stride);
     for (int c = (part * 256 + (int)threadIdx.x) * 4; c < u.len; c += p.parts * 1024) out[c >> 2] = keys_at(p, u, c);
 }
@@ -134,20 +134,25 @@ template <class T> __device__ T pick_scan(T v, T * lds, T * total) {
     return before + x - v;
 }
 
-// What request i keeps (-1: it is refused) and where its indices begin, from
-// all requests of the call. Up to 64 by each wave by itself.
-__device__ void plan_of(const PickArgs & p, int i, int & k, int & to) {
+// Request i: what it keeps (-1: it is refused) and where its indices begin, from
+// all requests of the call, and its sequence's cells. Up to 64 by each wave by
+// itself.
+__device__ void plan_of(const PickArgs & p, int i, int & k, int & to, int & seq_i, int & start, int & len) {
     __shared__ long long sums[kWaves];
     __shared__ int ids[kPick], kept_of[kPick], first[kPick];
     const int t = p.n <= 64 ? threadIdx.x & 63 : threadIdx.x;
-    int kept = -1, seq = -1;
+    int kept = -1, seq = -1, from = 0, cells = 0;
     if (t < p.n) {
-        const int cells = cells_of(p, t);
         seq = p.seqs[t];
+        from = p.start[t];
+        cells = cells_of(p, t);
         kept = cells < 0 ? -1 : p.keep[t] < cells ? p.keep[t] : cells;
         if (kept > p.n_idx) kept = -1;
     }
     if (p.n <= 64) {
+        seq_i = __shfl(seq, i);
+        start = __shfl(from, i);
+        len = start + __shfl(cells, i);
         for (int j = 0; j < p.n; j++) {
             const int other = __shfl(seq, j);   // (all lanes)
             if (j < t && other == seq) kept = -1;
@@ -194,6 +199,9 @@ __device__ void plan_of(const PickArgs & p, int i, int & k, int & to) {
     }
     k = kept_of[i];
     to = first[i];
+    seq_i = ids[i];
+    start = p.start[i];
+    len = k < 0 ? 0 : p.len[seq_i];
 }
 
 // A block per request and group of layers. Its waves have neighbouring
@@ -201,57 +209,52 @@ __device__ void plan_of(const PickArgs & p, int i, int & k, int & to) {
 // pass: what it writes it alone reads again. FUSED: the keys are worked out on
 // the way of the first pass.
 //
-// The k-th largest key by its bits from the top, 11, 11 and 10 of them: the
-// first 11 are sign, exponent and two bits more, which keeps the lanes of a wave
-// in different places of the histogram where eight bits would not.
+// The k-th largest key by its bits from the top. The first 11, sign, exponent
+// and two bits more, spread the lanes of a wave over a histogram in LDS where
+// eight bits would not. The keys that share those of the k-th one, mostly a few
+// hundred, are then listed in LDS with their wave, and the other 21 bits and each
+// wave's counts come from the list: three passes over the cells in all. Where
+// they are too many for the list, the passes go on over all cells.
+constexpr int kList = 4096;
+
 template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArgs p) {
-    __shared__ int lds[kWaves], bins[2048], found[2], above[kWaves], same[kWaves];
+    __shared__ int lds[kWaves], bins[2048], found[2], above[kWaves], same[kWaves], listed;
+    __shared__ unsigned list[kList];   // low 21 bits of a key, and the wave
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int i = blockIdx.x % p.n, group = blockIdx.x / p.n;
-    int k, to;
-    plan_of(p, i, k, to);
+    int k, to, seq, start, len;
+    plan_of(p, i, k, to, seq, start, len);
     if (group == 0 && t == 0) {
         p.status[i] = k < 0 ? KVC_REQ_BAD : 0;
-        p.granted[i] = k < 0 ? -1 : p.seqs[i];
+        p.granted[i] = k < 0 ? -1 : seq;
         p.cu[i + 1] = to + (k < 0 ? 0 : k);
         if (i == 0) p.cu[0] = 0;
     }
     if (k <= 0) return;
-    const Unit u = unit_of(p, i, group, k);
+    const Unit u = unit_of(p, seq, start, len, group, k);
     const int turns = (u.len + 4 * kPick - 1) / (4 * kPick);   // of 256 cells a wave
     const int c0 = wave * turns * 256 + 4 * lane;
     u4 * keys = reinterpret_cast<u4 *>(p.keys + ((long long)group * p.n + i) * p.stride);
 
-    unsigned top = 0;
-    int left = k;   // of the keys that begin with top's bits, how many are kept
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    // one more in place b of the histogram, of the lanes that are `in` (all lanes call)
+    auto count = [&](bool in, int b) {
+        // (many alike: one addition for the lanes that agree with the first)
+        const unsigned long long who = __ballot(in);
+        if (!who) return;
+        const int lead = __ffsll((long long)who) - 1, b0 = __builtin_amdgcn_readlane(b, lead);
+        const unsigned long long with = __ballot(in && b == b0);
+        if (lane == lead) atomicAdd(&bins[b0], __popcll(with));
+        if (in && b != b0) atomicAdd(&bins[b], 1);
+    };
+    auto clear = [&] {
         bins[t] = 0;
         bins[t + kPick] = 0;
         __syncthreads();
-        for (int y = 0; y < turns; y++) {
-            const int c = c0 + 256 * y;
-            if (c >= u.len) break;
-            u4 x;
-            if (FUSED && pass == 0) {
-                x = keys_at(p, u, c);
-                keys[c >> 2] = x;
-            } else {
-                x = keys[c >> 2];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = x[j] != 0 && (pass == 0 || x[j] >> (shift + bits) == top >> (shift + bits));
-                const int b = x[j] >> shift & ((1 << bits) - 1);
-                // (many alike: one addition for the lanes that agree with the first)
-                const unsigned long long who = __ballot(in);
-                if (!who) continue;
-                const int lead = __ffsll((long long)who) - 1, b0 = __shfl(b, lead);
-                const unsigned long long with = __ballot(in && b == b0);
-                if (lane == lead) atomicAdd(&bins[b0], __popcll(with));
-                if (in && b != b0) atomicAdd(&bins[b], 1);
-            }
-        }
+    };
+    unsigned top = 0;
+    int left = k;   // of the keys that begin with top's bits, how many are kept
+    // the place of the histogram that the left-th largest is in; how many are in it
+    auto find = [&](int shift) {
         __syncthreads();
         // from the top: thread t has places 2 t and 2 t + 1
         const int n0 = bins[2047 - 2 * t], n1 = bins[2046 - 2 * t];
@@ -265,22 +268,85 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
         __syncthreads();
         top |= (unsigned)found[0] << shift;
         left = found[1];
-        __syncthreads();
-    }
-    // how many of each wave are above it, and equal to it
-    int n_above = 0, n_same = 0;
+        return bins[found[0]];
+    };
+    if (t == 0) listed = 0;
+    if (t < kWaves) above[t] = same[t] = 0;
+    clear();
     for (int y = 0; y < turns; y++) {
         const int c = c0 + 256 * y;
-        const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            n_above += __popcll(__ballot(x[j] > top));
-            n_same += __popcll(__ballot(x[j] == top));
+        u4 x = {0, 0, 0, 0};
+        if (c < u.len) {
+            if constexpr (FUSED) {
+                x = keys_at(p, u, c);
+                keys[c >> 2] = x;
+            } else {
+                x = keys[c >> 2];
+            }
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++) count(x[j] != 0, x[j] >> 21);
     }
-    if (lane == 0) {
-        above[wave] = n_above;
-        same[wave] = n_same;
+    const int near = find(21);   // (uniform) keys that begin like the k-th
+    int n_above = 0, n_same = 0;
+    if (near <= kList) {
+        for (int y = 0; y < turns; y++) {
+            const int c = c0 + 256 * y;
+            const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                n_above += __popcll(__ballot(x[j] >> 21 > top >> 21));
+                const bool in = x[j] != 0 && x[j] >> 21 == top >> 21;
+                const unsigned long long who = __ballot(in);
+                if (!who) continue;
+                const int lead = __ffsll((long long)who) - 1;
+                int at = 0;
+                if (lane == lead) at = atomicAdd(&listed, __popcll(who));
+                at = __builtin_amdgcn_readlane(at, lead);
+                if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = (x[j] & 0x1fffff) | (unsigned)wave << 21;
+            }
+        }
+        for (int pass = 1; pass < 3; pass++) {
+            const int shift = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10;
+            clear();
+            for (int e = t; e < kList; e += kPick) {
+                const unsigned x = e < near ? list[e] & 0x1fffff : 0;
+                count(e < near && x >> (shift + bits) == (top & 0x1fffff) >> (shift + bits), x >> shift & ((1 << bits) - 1));
+            }
+            find(shift);
+        }
+        for (int e = t; e < near; e += kPick) {
+            const unsigned x = list[e] & 0x1fffff;
+            if (x > (top & 0x1fffff)) atomicAdd(&above[list[e] >> 21], 1);
+            if (x == (top & 0x1fffff)) atomicAdd(&same[list[e] >> 21], 1);
+        }
+        if (lane == 0) atomicAdd(&above[wave], n_above);
+    } else {
+        for (int pass = 1; pass < 3; pass++) {
+            const int shift = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10;
+            clear();
+            for (int y = 0; y < turns; y++) {
+                const int c = c0 + 256 * y;
+                const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    count(x[j] != 0 && x[j] >> (shift + bits) == top >> (shift + bits), x[j] >> shift & ((1 << bits) - 1));
+            }
+            find(shift);
+        }
+        for (int y = 0; y < turns; y++) {
+            const int c = c0 + 256 * y;
+            const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                n_above += __popcll(__ballot(x[j] > top));
+                n_same += __popcll(__ballot(x[j] == top));
+            }
+        }
+        if (lane == 0) {
+            above[wave] = n_above;
+            same[wave] = n_same;
+        }
     }
     __syncthreads();
     int done = 0, equal = 0;   // kept, and equal to top, before this wave's cells
@@ -295,21 +361,20 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
         const int c = c0 + 256 * y;
         const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
         int nth = equal, where = done;
-        unsigned long long alike[4], kept[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            alike[j] = __ballot(x[j] == top);
-            nth += __popcll(alike[j] & before);
-            equal += __popcll(alike[j]);
+            const unsigned long long alike = __ballot(x[j] == top);
+            nth += __popcll(alike & before);
+            equal += __popcll(alike);
         }
         bool stays[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             stays[j] = x[j] > top || (x[j] == top && nth < left);
             nth += x[j] == top;
-            kept[j] = __ballot(stays[j]);
-            where += __popcll(kept[j] & before);
-            done += __popcll(kept[j]);
+            const unsigned long long kept = __ballot(stays[j]);
+            where += __popcll(kept & before);
+            done += __popcll(kept);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -333,9 +398,10 @@ struct TakeArgs {
 
 // A block per request, layer and head. Places are filled in ascending order and
 // no cell moves down, so that a row can be moved within itself: what a step of
-// the block reads is at or behind what it writes.
+// the block reads is at or behind what it writes. A step is 16 cells a thread:
+// two rounds of loads in all for most budgets.
 __global__ __launch_bounds__(256) void k_take_weights(TakeArgs p) {
-    constexpr int STEP = 1024;
+    constexpr int STEP = 4096;
     for (long long u = blockIdx.x; u < (long long)p.n * p.n_layers * p.H; u += gridDim.x) {
         const int h = (int)(u % p.H), l = (int)(u / p.H % p.n_layers), i = (int)(u / p.H / p.n_layers);
         const int src = p.src[i], dst = p.dst[i];
@@ -358,18 +424,22 @@ __global__ __launch_bounds__(256) void k_take_weights(TakeArgs p) {
         const int * idx = p.idx + l * p.ld_idx + k0;
         for (int c0 = 0; c0 < kept; c0 += STEP) {
             float x[STEP / 256];
-            bool ok[STEP / 256];
+            int at[STEP / 256];
 #pragma unroll
             for (int j = 0; j < STEP / 256; j++) {
                 const int c = c0 + 256 * j + (int)threadIdx.x;
-                const int a = c < kept ? idx[c] : -1;
-                ok[j] = a >= c && (long long)lead + a < p.room;
-                x[j] = ok[j] ? from[lead + a] : 0.0f;
+                at[j] = c < kept ? idx[c] : -1;
             }
-            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < STEP / 256; j++) {
+                const int c = c0 + 256 * j + (int)threadIdx.x;
+                if (at[j] < c || (long long)lead + at[j] >= p.room) at[j] = -1;
+                x[j] = at[j] >= 0 ? from[lead + at[j]] : 0.0f;
+            }
+            if (src == dst) __syncthreads();
 #pragma unroll
             for (int j = 0; j < STEP / 256; j++)
-                if (ok[j]) to[lead + c0 + 256 * j + (int)threadIdx.x] = x[j];
+                if (at[j] >= 0) to[lead + c0 + 256 * j + (int)threadIdx.x] = x[j];
         }
         __syncthreads();
     }
