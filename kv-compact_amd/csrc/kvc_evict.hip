@@ -134,6 +134,17 @@ template <class T> __device__ T pick_scan(T v, T * lds, T * total) {
     return before + x - v;
 }
 
+// Sum of v over the wave's lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // Request i: what it keeps (-1: it is refused) and where its indices begin, from
 // all requests of the call, and its sequence's cells. Up to 64 by each wave by
 // itself.
@@ -221,7 +232,8 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
     __shared__ int lds[kWaves], bins[2048], found[2], above[kWaves], same[kWaves], listed;
     __shared__ unsigned list[kList];   // low 21 bits of a key, and the wave
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int i = blockIdx.x % p.n, group = blockIdx.x / p.n;
+    // (a request's blocks on different dies and CUs: requests differ in length)
+    const int group = blockIdx.x / p.n, i = (blockIdx.x % p.n + group + group / 8) % p.n;
     int k, to, seq, start, len;
     plan_of(p, i, k, to, seq, start, len);
     if (group == 0 && t == 0) {
@@ -258,8 +270,12 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
         __syncthreads();
         // from the top: thread t has places 2 t and 2 t + 1
         const int n0 = bins[2047 - 2 * t], n1 = bins[2046 - 2 * t];
-        int all;
-        const int before = pick_scan(n0 + n1, lds, &all);
+        const int incl = wave_scan(n0 + n1);
+        if (lane == 63) lds[wave] = incl;
+        __syncthreads();
+        int before = incl - n0 - n1;
+#pragma unroll
+        for (int j = 0; j < kWaves; j++) before += j < wave ? lds[j] : 0;
         if (before < left && left <= before + n0 + n1) {
             const bool second = left > before + n0;
             found[0] = 2047 - 2 * t - second;
@@ -270,6 +286,19 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
         left = found[1];
         return bins[found[0]];
     };
+    // f(four keys, their first cell) in ascending order (all lanes), the next four on their way
+    auto each = [&](auto f) {
+        u4 next = {0, 0, 0, 0};
+        if (c0 < u.len) next = keys[c0 >> 2];
+        for (int y = 0; y < turns; y++) {
+            const u4 x = next;
+            const int c = c0 + 256 * y;
+            next = u4{0, 0, 0, 0};
+            if (y + 1 < turns && c + 256 < u.len) next = keys[(c + 256) >> 2];
+            f(x, c);
+        }
+    };
+    const unsigned long long before_me = (1ull << lane) - 1;
     if (t == 0) listed = 0;
     if (t < kWaves) above[t] = same[t] = 0;
     clear();
@@ -290,22 +319,27 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
     const int near = find(21);   // (uniform) keys that begin like the k-th
     int n_above = 0, n_same = 0;
     if (near <= kList) {
-        for (int y = 0; y < turns; y++) {
-            const int c = c0 + 256 * y;
-            const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+        each([&](u4 x, int) {
+            bool in[4];
+            unsigned long long who[4];
+            int n = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 n_above += __popcll(__ballot(x[j] >> 21 > top >> 21));
-                const bool in = x[j] != 0 && x[j] >> 21 == top >> 21;
-                const unsigned long long who = __ballot(in);
-                if (!who) continue;
-                const int lead = __ffsll((long long)who) - 1;
-                int at = 0;
-                if (lane == lead) at = atomicAdd(&listed, __popcll(who));
-                at = __builtin_amdgcn_readlane(at, lead);
-                if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = (x[j] & 0x1fffff) | (unsigned)wave << 21;
+                in[j] = x[j] != 0 && x[j] >> 21 == top >> 21;
+                who[j] = __ballot(in[j]);
+                n += __popcll(who[j]);
             }
-        }
+            if (!n) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&listed, n);
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (in[j]) list[at + __popcll(who[j] & before_me)] = (x[j] & 0x1fffff) | (unsigned)wave << 21;
+                at += __popcll(who[j]);
+            }
+        });
         for (int pass = 1; pass < 3; pass++) {
             const int shift = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10;
             clear();
@@ -325,24 +359,20 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
         for (int pass = 1; pass < 3; pass++) {
             const int shift = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10;
             clear();
-            for (int y = 0; y < turns; y++) {
-                const int c = c0 + 256 * y;
-                const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+            each([&](u4 x, int) {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     count(x[j] != 0 && x[j] >> (shift + bits) == top >> (shift + bits), x[j] >> shift & ((1 << bits) - 1));
-            }
+            });
             find(shift);
         }
-        for (int y = 0; y < turns; y++) {
-            const int c = c0 + 256 * y;
-            const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+        each([&](u4 x, int) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 n_above += __popcll(__ballot(x[j] > top));
                 n_same += __popcll(__ballot(x[j] == top));
             }
-        }
+        });
         if (lane == 0) {
             above[wave] = n_above;
             same[wave] = n_same;
@@ -356,15 +386,12 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
     }
     done += equal < left ? equal : left;
     int * out = p.idx + group * p.ld_idx + to;
-    const unsigned long long before = (1ull << lane) - 1;
-    for (int y = 0; y < turns; y++) {
-        const int c = c0 + 256 * y;
-        const u4 x = c < u.len ? keys[c >> 2] : u4{0, 0, 0, 0};
+    each([&](u4 x, int c) {
         int nth = equal, where = done;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const unsigned long long alike = __ballot(x[j] == top);
-            nth += __popcll(alike & before);
+            nth += __popcll(alike & before_me);
             equal += __popcll(alike);
         }
         bool stays[4];
@@ -373,13 +400,13 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
             stays[j] = x[j] > top || (x[j] == top && nth < left);
             nth += x[j] == top;
             const unsigned long long kept = __ballot(stays[j]);
-            where += __popcll(kept & before);
+            where += __popcll(kept & before_me);
             done += __popcll(kept);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (stays[j]) out[where++] = c + j - u.start;
-    }
+    });
 }
 
 struct TakeArgs {
