@@ -107,7 +107,22 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a, const
     // a cache's pages are 16-byte aligned: its rows are where a head is whole 16-byte pieces
     s.careful = c->k_type != kQ8 && (!vec_rows(a->q, es) || c->d_k * es % 16 || c->d_v * es % 16);
     const long long rows = (long long)a->max_new * G;
+    int max_len = a->max_len < 1 << 30 ? a->max_len : 1 << 30;   // (no sequence has more; sums with it stay in range)
+    if (w) {   // (what lies between the first cells and the window is not gone through)
+        const long long seen = (long long)w->first + w->last + a->max_new;
+        max_len = seen < max_len ? (int)seen : max_len;
+    }
     s.rt = row_tiles(c->k_type, head_tile(c->d_k, c->d_v), s.careful, rows);
+    // Under a window a call over Q8_0 may be small: row tiles by the keys of all
+    // heads. 13 drafts of 32 heads, us with one, two and four tiles a wave, 8 KV
+    // heads: 2 sequences that see 512 cells 19, 23 and 33, 2048 23, 24 and 34,
+    // 8192 47, 38 and 46; 8 sequences: 20, 25 and 35; 44, 39 and 45; 140, 94 and
+    // 90; 16 and 2048: 71, 55 and 64; 32: 53, 53 and 46; 132, 108 and 91; 566, 351
+    // and 288.
+    if (w && s.rt > 1 && c->k_type == kQ8) {
+        const long long keys = (long long)max_len * a->n_seq * c->n_head_kv;
+        s.rt = keys < 1 << 16 ? 1 : keys < 400000 || s.rt == 2 ? 2 : 4;
+    }
     // Tiles in LDS from 33 rows on: 8 sequences of up to 20000 F16 cells with a
     // bias, k_attn_rows against two waves of rows: 36 rows 164 and 127 us, 64
     // rows 190 and 133 (24 rows 152 and 121: it would pay earlier); one
@@ -134,13 +149,16 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a, const
     // (512: 171), of 13 over Q8_0 469 and 604. For one token of one sequence:
     // 4096 cells in 8, 16 and 32 ranges 17.0, 14.1 and 13.3, 1024 cells in 2, 4
     // and 8 15.2, 12.4 and 11.1. At most 64, the lanes of the join's wave.
-    int max_len = a->max_len < 1 << 30 ? a->max_len : 1 << 30;   // (no sequence has more; sums with it stay in range)
-    if (w) {   // (what lies between the first cells and the window is not gone through)
-        const long long seen = (long long)w->first + w->last + a->max_new;
-        max_len = seen < max_len ? (int)seen : max_len;
-    }
-    const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles, blocks = s.whole || s.rt == 4 ? 1024 : 4096;
-    long long want = (blocks + units - 1) / units, most = max_len / 256;
+    // Under a window every long sequence has as many keys as the others, so that
+    // one block a CU is enough and more only cost their beginnings and the join:
+    // one token of 8, 32 and 64 sequences that see 2048 keys, for 256, 1024 and
+    // 4096 blocks 21, 23 and 23; 48, 55 and 61 us; 64 of 4096 keys 196, 206 and
+    // 216; trees of 32 over F16, 32 sequences of 4096 keys 150, 219 and 391. The
+    // least keys of a range are two tiles: 2 sequences of 512 keys 12.5 us, 15.2
+    // with eight; of 2048 14.9 and 15.3.
+    const long long units = (long long)a->n_seq * c->n_head_kv * s.tiles;
+    const long long blocks = w ? 256 : s.whole || s.rt == 4 ? 1024 : 4096;
+    long long want = (blocks + units - 1) / units, most = max_len / (w ? 64 : 256);
     want = want < most ? want : most;
     if ((long long)a->n_tok * a->n_head > 1 << 24) want = 1;   // (the join's launch: a block a row or four; so many need no ranges)
     s.splits = (int)(want < 1 ? 1 : want > 64 ? 64 : want);

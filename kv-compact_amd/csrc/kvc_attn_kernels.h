@@ -1105,7 +1105,9 @@ void k_attn_tiles(AttnArgs a) {
     const bool k_piece = (int)(8 * k_col) < a.dk, v_piece = (int)(8 * v_col) < a.dv;
     const char * k_head = a.k.base + h * a.k.ld_head;
     const char * v_head = a.v.base + h * a.v.ld_head;
-    for (int i = threadIdx.x; i < BUFS * 2 * BK * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+    // (whole heads leave nothing unwritten but rows past the end, which are hidden)
+    if (!WINDOW || a.dk < D || a.dv < D)
+        for (int i = threadIdx.x; i < BUFS * 2 * BK * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
     __syncthreads();
 
     for (; (long long)tile * ROWS < rows; tile += tile_step) {
@@ -1310,11 +1312,25 @@ void k_attn_tiles(AttnArgs a) {
                 pf[1][1] = swap[other][1][lane];
             }
             bool odd = false;
+            // Values of V that are not finite do not get into products where a key is hidden.
+            auto drop_odd = [&](u4 & vf, int key) {
+                constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const bool lo = (vf[y] & e) == e, hi = (vf[y] >> 16 & e) == e;
+                    // (cells that no row sees, past the end among them, are nothing)
+                    const int kk = key + 8 * (y >> 1) + 2 * (y & 1);
+                    if (lo) odd |= CELLS ? cells[buf][part0 + kk] != -INFINITY : (PAIR ? tile0 : key0) + kk < q.held;
+                    if (hi) odd |= CELLS ? cells[buf][part0 + kk + 1] != -INFINITY : (PAIR ? tile0 : key0) + kk + 1 < q.held;
+                    vf[y] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                }
+            };
 #pragma unroll
             for (int x0 = 0; x0 < PV; x0++)
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
                     const int x = PAIR ? x0 ^ kw : x0;
+                    u4 vs[DT];
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
                         u2 half[2];
@@ -1328,19 +1344,28 @@ void k_attn_tiles(AttnArgs a) {
                                                                  (__attribute__((address_space(3))) s4 *)at));
                         }
                         u4 vf = {half[0].x, half[0].y, half[1].x, half[1].y};
-                        if (!PLAIN && hidden) {
-                            constexpr unsigned e = TYPE == kF16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-                            for (int y = 0; y < 4; y++) {
-                                const bool lo = (vf[y] & e) == e, hi = (vf[y] >> 16 & e) == e;
-                                // (cells that no row sees, past the end among them, are nothing)
-                                const int kk = 32 * x + 16 * st + 8 * (y >> 1) + 4 * hf + 2 * (y & 1);
-                                if (lo) odd |= CELLS ? cells[buf][part0 + kk] != -INFINITY : (PAIR ? tile0 : key0) + kk < q.held;
-                                if (hi) odd |= CELLS ? cells[buf][part0 + kk + 1] != -INFINITY : (PAIR ? tile0 : key0) + kk + 1 < q.held;
-                                vf[y] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-                            }
+                        if constexpr (WINDOW && !PLAIN) {
+                            vs[d] = vf;
+                        } else {
+                            if (!PLAIN && hidden) drop_odd(vf, 32 * x + 16 * st + 4 * hf);
+                            acc[d] = mfma32<TYPE>(vf, pf[x0][st], acc[d]);
                         }
-                        acc[d] = mfma32<TYPE>(vf, pf[x0][st], acc[d]);
+                    }
+                    if constexpr (WINDOW && !PLAIN) {
+                        // (a window has such tiles at both ends: first whether there is such a value at all.
+                        // An exponent of all ones carries into the sign's place.)
+                        constexpr unsigned one = TYPE == kF16 ? 0x04000400u : 0x00800080u;
+                        unsigned any = 0;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) any |= (vs[d][y] & 0x7fff7fffu) + one;
+                        if (hidden && __ballot((any & 0x80008000u) != 0)) {
+#pragma unroll
+                            for (int d = 0; d < DT; d++) drop_odd(vs[d], 32 * x + 16 * st + 4 * hf);
+                        }
+#pragma unroll
+                        for (int d = 0; d < DT; d++) acc[d] = mfma32<TYPE>(vs[d], pf[x0][st], acc[d]);
                     }
                 }
             if (!PLAIN && hidden && __ballot(odd)) odd_tiles.add(t);
