@@ -519,31 +519,31 @@ template <int TYPE, int QT> bool run_weigh_few(const WeighArgs & w, long long ro
     return run_weigh_few<TYPE, QT, TYPE == kF32 ? kFewRows32 : kFewRows16>(w, careful, blocks, st);
 }
 
-// More rows of 16-bit types: a wave keeps the keys of 32 SUB cells in registers,
-// two waves a block's cells, and two the one half of a tile of 64 rows each, two
-// the other. Rows reach LDS by direct loads, three tiles ahead, pieces of 16
-// bytes exchanged by row % 8 as keys are in k_attn_tiles, whose fragments these
-// are: a lane holds a row's scores of 16 of 32 cells. A tile is whole tokens:
-// its rows' places are the same in every tile, and rows that are left over (or
-// past the last token) repeat its last row with a log-sum-exp of +inf.
+// More rows of 16-bit types: each of a block's four waves keeps the keys of 32
+// cells in registers and goes over all rows, tiles of 64 in LDS. Rows reach LDS
+// by direct loads, two tiles ahead, pieces of 16 bytes exchanged by the row's
+// number so that the lanes of a read are on different banks; the fragments are
+// those of k_attn_tiles: a lane holds a row's scores of 16 of 32 cells. A tile is
+// whole tokens: its rows' places are the same in every tile, and rows that are
+// left over (or past the last token) repeat its last row with a log-sum-exp of
+// +inf.
 //
 // Without a bias the scores go into the exponential by one multiply-add (scale
 // and log2 e in one factor: each rounded once, as the separate steps are).
 __device__ const float nothing_word = INFINITY;
 
 template <int TYPE, int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
-    constexpr int SUB = D == 256 ? 1 : 2, CELLS = 64 * SUB;   // 32-cell parts of a wave; cells of a block
-    constexpr int ROWS = 64, KS = D / 16, CH = D / 8, ROWB = 2 * D;
+__global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
+    constexpr int CELLS = 128, ROWS = 64, KS = D / 16, CH = D / 8, ROWB = 2 * D;
+    constexpr int SWAP = CH < 16 ? 7 : 15;                    // bits of a row's number that its pieces are exchanged by
     constexpr int NL = ROWS * CH / 256, RPL = 512 / D;        // direct loads of a wave and tile; rows of one
-    constexpr int BUFS = D == 256 ? 2 : 4, AHEAD = BUFS - 1, LOADS = NL + 1;
+    constexpr int BUFS = D == 256 ? 2 : 3, AHEAD = BUFS - 1, LOADS = NL + 1;
     __shared__ __align__(16) char lds[BUFS][ROWS * ROWB];
     __shared__ float row_lse[BUFS][ROWS];
-    __shared__ float join[2][64];
 
     const AttnArgs & a = w.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cw = wave & 1, rw = wave >> 1, n = lane & 31, hf = lane >> 5;
+    const int n = lane & 31, hf = lane >> 5;
     int u = blockIdx.x;
     const int h = u % a.H;
     u /= a.H;
@@ -554,16 +554,17 @@ __global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
     const int page_mask = (1 << a.shift) - 1;
     const int T = ROWS / a.G;                                 // tokens of a tile
     const float to_log2 = a.scale * kLog2e;
-    // places of a tile's rows: this lane's, and those it loads
-    const int my_row = 32 * rw + n < T * a.G ? 32 * rw + n : T * a.G - 1;
-    const int my_tok = my_row / a.G;
+    // places of a tile's rows: this lane's two, and those it loads
+    int my_tok[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) my_tok[r] = (32 * r + n < T * a.G ? 32 * r + n : T * a.G - 1) / a.G;
     int load_tok[NL];
     unsigned load_off[NL];
     bool load_on[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
         const int at = (i * 4 + wave) * RPL + lane / CH, row = at < T * a.G ? at : T * a.G - 1;
-        const int piece = (lane % CH) ^ (at & 7);
+        const int piece = (lane % CH) ^ (at & SWAP);
         load_tok[i] = row / a.G;
         load_off[i] = (unsigned)(row % a.G) * (unsigned)(2 * a.q_head) + 16 * piece;
         load_on[i] = 8 * piece < a.dk;
@@ -573,11 +574,11 @@ __global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
     const bool lse_on = lse_row < T * a.G;
 
     for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
-        const int block0 = tile * CELLS, cell0 = block0 + 32 * SUB * cw;
+        const int block0 = tile * CELLS, cell0 = block0 + 32 * wave;
         int t0, t1;   // the block's tokens, and the wave's
         tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
         int wt0, wt1;
-        tokens_of(a, c, cell0, cell0 + 32 * SUB < q.held ? cell0 + 32 * SUB : q.held, wt0, wt1);
+        tokens_of(a, c, cell0, cell0 + 32 < q.held ? cell0 + 32 : q.held, wt0, wt1);
         if (cell0 >= q.held) wt1 = wt0;
 
         auto fill = [&](int tt, int buf) {
@@ -600,44 +601,51 @@ __global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
             for (int i = threadIdx.x; i < BUFS * ROWS * CH; i += 256) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
             __syncthreads();
         }
-        u4 kf[SUB][KS];
-        f16x bias[BIAS ? SUB : 1], sum[SUB];
-        unsigned there[SUB];   // cells of this lane's registers that rows may see
-#pragma unroll
-        for (int x = 0; x < SUB; x++) {
-            const int cell = cell0 + 32 * x + (n & 16);
+        u4 kf[KS];
+        f16x bias, sum;
+        unsigned there;   // cells of this lane's registers that rows may see
+        {
+            const int cell = cell0 + (n & 16);
             int page = cell < q.held ? q.table[cell >> a.shift] : -1;
             const bool good = page >= 0 && page < a.n_pages;
             if (!good) page = 0;
             const unsigned long long row = ((unsigned)page << a.shift) + ((cell + (n & 15)) & page_mask);
             const char * p = a.k.base + h * a.k.ld_head + row * a.k.ld_tok + 16 * hf;
+            if (a.dk == D) {
 #pragma unroll
-            for (int j = 0; j < KS; j++)
-                kf[x][j] = 16 * j + 8 * hf < a.dk ? *reinterpret_cast<const u4 *>(p + 32 * j) : u4{0, 0, 0, 0};
-            const int left = q.held - cell0 - 32 * x;
+                for (int j = 0; j < KS; j++) kf[j] = *reinterpret_cast<const u4 *>(p + 32 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < KS; j++)
+                    kf[j] = 16 * j + 8 * hf < a.dk ? *reinterpret_cast<const u4 *>(p + 32 * j) : u4{0, 0, 0, 0};
+            }
+            const int left = q.held - cell0;
             const unsigned long long ok = __ballot(good);   // (lanes 0 and 16: the two groups of 16 cells)
-            there[x] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-            there[x] &= (ok & 1 ? 0xffffu : 0u) | (ok >> 16 & 1 ? 0xffff0000u : 0u);
+            there = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+            there &= (ok & 1 ? 0xffffu : 0u) | (ok >> 16 & 1 ? 0xffff0000u : 0u);
             if constexpr (BIAS) {
                 const int pages[2] = {__shfl(page, 0), __shfl(page, 16)};
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const int at = cell0 + 32 * x + 8 * y + 4 * hf;
+                    const int at = cell0 + 8 * y + 4 * hf;
                     const f4 b = *reinterpret_cast<const f4 *>(a.bias + (((long long)pages[y >> 1] * a.H + h) << a.shift) + (at & page_mask));
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        bias[x][4 * y + i] = b[i];
-                        if (b[i] == -INFINITY) there[x] &= ~(1u << (8 * y + 4 * hf + i));
+                        bias[4 * y + i] = b[i];
+                        if (b[i] == -INFINITY) there &= ~(1u << (8 * y + 4 * hf + i));
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) sum[x][i] = 0.0f;
+            for (int i = 0; i < 16; i++) sum[i] = 0.0f;
         }
         if (t0 < t1) {
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) fill(t0 + i * T, i);
         }
+        // (the keys are waited for here: a wait in the loop would be one for the rows on their way too)
+#pragma unroll
+        for (int j = 0; j < KS; j++) asm volatile("" : "+v"(kf[j]));
         auto arrive = [&](int tt, int buf) {
             wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
@@ -646,46 +654,79 @@ __global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
         };
         auto step = [&](int tt, int buf, auto kind) {
             constexpr bool PLAIN = decltype(kind)::value;
-            f16x sc[SUB];
+            f16x sc[2];
+            float l2[2];   // (with a bias the log-sum-exp itself)
+            unsigned see[2];
 #pragma unroll
-            for (int x = 0; x < SUB; x++)
+            for (int r = 0; r < 2; r++) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) sc[x][i] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < KS; j++) {
-                const u4 qf = *reinterpret_cast<const u4 *>(&lds[buf][(32 * rw + n) * ROWB + (((2 * j + hf) ^ (n & 7)) << 4)]);
-#pragma unroll
-                for (int x = 0; x < SUB; x++) sc[x] = mfma32<TYPE>(kf[x][j], qf, sc[x]);
-            }
-            float lse = row_lse[buf][32 * rw + n];
-            if (lse == -INFINITY) lse = INFINITY;   // (a row that saw nothing gives nothing)
-            const float l2 = lse * kLog2e;
-            unsigned see[SUB];
-            if constexpr (!PLAIN) {
-                const int tok = tt + my_tok < t1 ? tt + my_tok : t1 - 1;
-                const int from = window_from(a, q, tok);
-#pragma unroll
-                for (int x = 0; x < SUB; x++)
-                    see[x] = (seen32(a, q, tok, cell0 + 32 * x) & window32(a, from, cell0 + 32 * x)) >> (4 * hf);
-            }
-#pragma unroll
-            for (int x = 0; x < SUB; x++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    // (with a bias the difference first: a score may be the type's lowest value)
-                    float p = BIAS ? exp_of(__builtin_fmaf(sc[x][i], a.scale, bias[BIAS ? x : 0][i]) - lse)
-                                   : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], to_log2, -l2));
-                    if constexpr (!PLAIN) p = see[x] >> (8 * (i >> 2) + (i & 3)) & 1 ? p : 0.0f;
-                    sum[x][i] += p;
+                for (int i = 0; i < 16; i++) sc[r][i] = 0.0f;
+                const float lse = row_lse[buf][32 * r + n];
+                l2[r] = lse == -INFINITY ? INFINITY : BIAS ? lse : lse * kLog2e;   // (a row that saw nothing gives nothing)
+                if constexpr (!PLAIN) {
+                    const int tok = tt + my_tok[r] < t1 ? tt + my_tok[r] : t1 - 1;
+                    see[r] = (seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0)) >> (4 * hf);
                 }
+            }
+            // four of a row's scores to weights (PLAIN: exponentials side by side, with products around them)
+            auto weights = [&](int r, int y) {
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    // (with a bias the difference first: a score may be the type's lowest value)
+                    p[i] = BIAS ? exp_of(__builtin_fmaf(sc[r][4 * y + i], a.scale, bias[4 * y + i]) - l2[r])
+                                : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][4 * y + i], to_log2, -l2[r]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (!PLAIN) p[i] = see[r] >> (8 * y + i) & 1 ? p[i] : 0.0f;
+                    sum[4 * y + i] += p[i];
+                }
+            };
+            auto row_part = [&](int r, int j) {
+                return *reinterpret_cast<const u4 *>(&lds[buf][(32 * r + n) * ROWB + (((2 * j + hf) ^ (n & SWAP)) << 4)]);
+            };
+            constexpr int PART = KS < 8 ? KS : 8;   // reads of LDS ahead of their products
+            u4 qf[PART];
+#pragma unroll
+            for (int j0 = 0; j0 < KS; j0 += PART) {
+#pragma unroll
+                for (int j = 0; j < PART; j++) qf[j] = row_part(0, j0 + j);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < PART; j++) sc[0] = mfma32<TYPE>(kf[j0 + j], qf[j], sc[0]);
+            }
+#pragma unroll
+            for (int j = 0; j < PART; j++) qf[j] = row_part(1, j);
+            __builtin_amdgcn_sched_barrier(0);
+            // the second rows' products run under the first ones' exponentials
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+#pragma unroll
+                for (int j = y * PART / 4; j < (y + 1) * PART / 4; j++) sc[1] = mfma32<TYPE>(kf[j], qf[j], sc[1]);
+                weights(0, y);
+                if constexpr (PLAIN) __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j0 = PART; j0 < KS; j0 += PART) {
+#pragma unroll
+                for (int j = 0; j < PART; j++) qf[j] = row_part(1, j0 + j);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < PART; j++) sc[1] = mfma32<TYPE>(kf[j0 + j], qf[j], sc[1]);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                weights(1, y);
+                if constexpr (PLAIN) __builtin_amdgcn_sched_barrier(0);
+            }
         };
         // what the rows of a tile see of this wave's cells: nothing, all, or some
         auto idle = [&](int tt) { return tt + T <= wt0 || tt >= wt1; };
         auto whole = [&](int tt) {
             const int last = tt + T < t1 ? tt + T : t1;
-            if (cell0 + 32 * SUB > (a.mask ? q.base : q.base + tt + 1)) return false;
+            if (cell0 + 32 > (a.mask ? q.base : q.base + tt + 1)) return false;
             const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last - a.last;
-            return !(cell0 + 32 * SUB > a.first && cell0 < from);
+            return !(cell0 + 32 > a.first && cell0 < from);
         };
         int tt = t0, buf = 0;
         auto next = [&] {
@@ -704,25 +745,18 @@ __global__ __launch_bounds__(256, 2) void k_weigh_tiles(WeighArgs w) {
         }
         wait_lds_loads<0>();
         // over a half's 32 lanes: each step hands half of the sums to the lane across, until each holds one cell's
-        float v[16 * SUB];
+        float v[16];
 #pragma unroll
-        for (int x = 0; x < SUB; x++)
+        for (int i = 0; i < 16; i++) v[i] = there >> (8 * (i >> 2) + 4 * hf + (i & 3)) & 1 ? sum[i] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[16 * x + i] = there[x] >> (8 * (i >> 2) + 4 * hf + (i & 3)) & 1 ? sum[x][i] : 0.0f;
-#pragma unroll
-        for (int m = 8 * SUB; m; m >>= 1)
+        for (int m = 8; m; m >>= 1)
 #pragma unroll
             for (int i = 0; i < m; i++) {
                 const float mine = n & m ? v[m + i] : v[i], theirs = n & m ? v[i] : v[m + i];
                 v[i] = mine + __shfl_xor(theirs, m);
             }
-        if constexpr (SUB == 1) v[0] += __shfl_xor(v[0], 16);
-        if (rw == 1) join[cw][lane] = v[0];
-        __syncthreads();
-        if (rw == 0 && (SUB == 2 || n < 16)) {
-            const int i = n & 15;
-            add_weight(w, c, h, cell0 + 32 * (n >> 4) + 8 * (i >> 2) + 4 * hf + (i & 3), v[0] + join[cw][lane]);
-        }
+        v[0] += __shfl_xor(v[0], 16);
+        if (n < 16) add_weight(w, c, h, cell0 + 8 * (n >> 2) + 4 * hf + (n & 3), v[0]);
     }
 }
 
@@ -782,9 +816,8 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     // (strides that direct loads take)
     const bool tiles = !few && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
                        x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23;
-    const int cells = tiles && c->d_k > 128 ? 64 : 128;   // of a block
     const long long units = (long long)x->n_seq * c->n_head_kv;
-    long long want = ((long long)x->max_len + cells - 1) / cells;
+    long long want = ((long long)x->max_len + 127) / 128;   // (128 cells are a block's)
     const long long most = kMaxBlocks / units;
     if (most < 1) return KV_COMPACT_E_UNSUPPORTED;
     if (few && want > (4095 + units) / units) want = (4095 + units) / units;
