@@ -521,29 +521,36 @@ template <int TYPE, int QT> bool run_weigh_few(const WeighArgs & w, long long ro
 
 // More rows of 16-bit types: each of a block's four waves keeps the keys of 32
 // cells in registers and goes over all rows, tiles of 64 in LDS. Rows reach LDS
-// by direct loads, two tiles ahead, pieces of 16 bytes exchanged by the row's
+// by direct loads, two tiles ahead (256-wide heads: one), pieces of 16 bytes exchanged by the row's
 // number so that the lanes of a read are on different banks; the fragments are
 // those of k_attn_tiles: a lane holds a row's scores of 16 of 32 cells. A tile is
 // whole tokens: its rows' places are the same in every tile, and rows that are
 // left over (or past the last token) repeat its last row with a log-sum-exp of
-// +inf.
+// +inf. RW = 2, for few blocks: eight waves, two a cell tile, over tiles of 128
+// rows; they join in LDS.
 //
 // Without a bias the scores go into the exponential by one multiply-add (scale
 // and log2 e in one factor: each rounded once, as the separate steps are).
-__device__ const float nothing_word = INFINITY;
+// (4 bytes a lane, lanes' to side by side)
+__device__ __forceinline__ void load_lds4(const char * from, unsigned offset, char * to) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(from), "s"(at) : "m0", "memory");
+}
 
-template <int TYPE, int D, bool BIAS>
-__global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
-    constexpr int CELLS = 128, ROWS = 64, KS = D / 16, CH = D / 8, ROWB = 2 * D;
+template <int TYPE, int D, bool BIAS, int RW>
+__global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
+    constexpr int CELLS = 128, ROWS = 64 * RW, KS = D / 16, CH = D / 8, ROWB = 2 * D;
     constexpr int SWAP = CH < 16 ? 7 : 15;                    // bits of a row's number that its pieces are exchanged by
-    constexpr int NL = ROWS * CH / 256, RPL = 512 / D;        // direct loads of a wave and tile; rows of one
+    constexpr int WAVES = 4 * RW, NL = ROWS * CH / (64 * WAVES), RPL = 512 / D;   // direct loads of a wave and tile; rows of one
     constexpr int BUFS = D == 256 ? 2 : 3, AHEAD = BUFS - 1, LOADS = NL + 1;
+    static_assert(BUFS * ROWS * ROWB <= 128 * 1024, "a block fits a CU");
     __shared__ __align__(16) char lds[BUFS][ROWS * ROWB];
     __shared__ float row_lse[BUFS][ROWS];
+    __shared__ float join[RW == 2 ? 4 : 1][16][2];
 
     const AttnArgs & a = w.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 31, hf = lane >> 5;
+    const int cw = wave & 3, rw = wave >> 2, n = lane & 31, hf = lane >> 5;
     int u = blockIdx.x;
     const int h = u % a.H;
     u /= a.H;
@@ -556,49 +563,62 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
     const float to_log2 = a.scale * kLog2e;
     // places of a tile's rows: this lane's two, and those it loads
     int my_tok[2];
+    bool my_on[2];
 #pragma unroll
-    for (int r = 0; r < 2; r++) my_tok[r] = (32 * r + n < T * a.G ? 32 * r + n : T * a.G - 1) / a.G;
+    for (int r = 0; r < 2; r++) {
+        const int row = 64 * rw + 32 * r + n;
+        my_on[r] = row < T * a.G;
+        my_tok[r] = (my_on[r] ? row : T * a.G - 1) / a.G;
+    }
     int load_tok[NL];
     unsigned load_off[NL];
     bool load_on[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-        const int at = (i * 4 + wave) * RPL + lane / CH, row = at < T * a.G ? at : T * a.G - 1;
+        const int at = (i * WAVES + wave) * RPL + lane / CH, row = at < T * a.G ? at : T * a.G - 1;
         const int piece = (lane % CH) ^ (at & SWAP);
         load_tok[i] = row / a.G;
         load_off[i] = (unsigned)(row % a.G) * (unsigned)(2 * a.q_head) + 16 * piece;
         load_on[i] = 8 * piece < a.dk;
     }
-    const int lse_row = 16 * wave + (lane & 15);              // (lanes 0 .. 15)
-    const int lse_tok = lse_row / a.G, lse_head = lse_row % a.G;
-    const bool lse_on = lse_row < T * a.G;
+    const int lse_at = 16 * wave + (lane & 15), lse_row = lse_at < T * a.G ? lse_at : T * a.G - 1;   // (lanes 0 .. 15)
+    const int lse_tok = lse_row / a.G;
+    const unsigned lse_off = 4 * (unsigned)(lse_row % a.G), lse_step = 4 * (unsigned)(a.H * a.G);
 
     for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
-        const int block0 = tile * CELLS, cell0 = block0 + 32 * wave;
+        const int block0 = tile * CELLS, cell0 = block0 + 32 * cw;
         int t0, t1;   // the block's tokens, and the wave's
         tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
         int wt0, wt1;
         tokens_of(a, c, cell0, cell0 + 32 < q.held ? cell0 + 32 : q.held, wt0, wt1);
         if (cell0 >= q.held) wt1 = wt0;
 
-        auto fill = [&](int tt, int buf) {
-            if (tt >= t1) tt = t0 + (t1 - 1 - t0) / T * T;   // (past the last: like the last, for the count of loads)
-            const char * from = a.q + 2 * ((long long)(q.tok0 + tt) * a.q_tok + (long long)(h * a.G) * a.q_head);
-            const int most = t1 - 1 - tt;
+        // the next tile to load: its first token, its place, its rows and log-sum-exps
+        int load_tt = t0, load_buf = 0;
+        const char * load_q = a.q + 2 * ((long long)(q.tok0 + t0) * a.q_tok + (long long)(h * a.G) * a.q_head);
+        const char * load_l = reinterpret_cast<const char *>(a.lse + (long long)(q.tok0 + t0) * a.H * a.G + h * a.G);
+        const long long q_step = 2 * T * a.q_tok, l_step = 4LL * T * a.H * a.G;
+        auto fill = [&] {
+            const int most = t1 - 1 - load_tt;
+            char * to = lds[load_buf];
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int tk = load_tok[i] < most ? load_tok[i] : most;
-                if (load_on[i]) load_lds16(from, load_off[i] + __umul24(tk, (unsigned)(2 * a.q_tok)), &lds[buf][(i * 4 + wave) * 1024]);
+                if (load_on[i]) load_lds16(load_q, load_off[i] + __umul24(tk, (unsigned)(2 * a.q_tok)), to + (i * WAVES + wave) * 1024);
             }
-            const char * l = lse_on && lse_tok <= most
-                                 ? reinterpret_cast<const char *>(a.lse + (long long)(q.tok0 + tt + lse_tok) * a.H * a.G + h * a.G + lse_head)
-                                 : reinterpret_cast<const char *>(&nothing_word);
-            if (lane < 16) load_lds4(l, reinterpret_cast<char *>(&row_lse[buf][16 * wave]));
+            if (lane < 16)
+                load_lds4(load_l, lse_off + __umul24(lse_tok < most ? lse_tok : most, lse_step), reinterpret_cast<char *>(&row_lse[load_buf][16 * wave]));
+            load_buf = load_buf + 1 < BUFS ? load_buf + 1 : 0;
+            if (load_tt + T < t1) {   // (past the last tile: the last again, for the count of loads)
+                load_tt += T;
+                load_q += q_step;
+                load_l += l_step;
+            }
         };
 
         __syncthreads();   // (LDS of the last tile of cells is read)
         if (a.dk < D) {
-            for (int i = threadIdx.x; i < BUFS * ROWS * CH; i += 256) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+            for (int i = threadIdx.x; i < BUFS * ROWS * CH; i += 64 * WAVES) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
             __syncthreads();
         }
         u4 kf[KS];
@@ -641,16 +661,16 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
         }
         if (t0 < t1) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) fill(t0 + i * T, i);
+            for (int i = 0; i < AHEAD; i++) fill();
         }
         // (the keys are waited for here: a wait in the loop would be one for the rows on their way too)
 #pragma unroll
         for (int j = 0; j < KS; j++) asm volatile("" : "+v"(kf[j]));
-        auto arrive = [&](int tt, int buf) {
+        auto arrive = [&] {
             wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            fill(tt + AHEAD * T, (buf + AHEAD) % BUFS);
+            fill();
         };
         auto step = [&](int tt, int buf, auto kind) {
             constexpr bool PLAIN = decltype(kind)::value;
@@ -661,8 +681,9 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
             for (int r = 0; r < 2; r++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) sc[r][i] = 0.0f;
-                const float lse = row_lse[buf][32 * r + n];
-                l2[r] = lse == -INFINITY ? INFINITY : BIAS ? lse : lse * kLog2e;   // (a row that saw nothing gives nothing)
+                const float lse = row_lse[buf][64 * rw + 32 * r + n];
+                // (a row that saw nothing gives nothing, nor does one past the last)
+                l2[r] = lse == -INFINITY || !my_on[r] || tt + my_tok[r] >= t1 ? INFINITY : BIAS ? lse : lse * kLog2e;
                 if constexpr (!PLAIN) {
                     const int tok = tt + my_tok[r] < t1 ? tt + my_tok[r] : t1 - 1;
                     see[r] = (seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0)) >> (4 * hf);
@@ -683,7 +704,7 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
                 }
             };
             auto row_part = [&](int r, int j) {
-                return *reinterpret_cast<const u4 *>(&lds[buf][(32 * r + n) * ROWB + (((2 * j + hf) ^ (n & SWAP)) << 4)]);
+                return *reinterpret_cast<const u4 *>(&lds[buf][(64 * rw + 32 * r + n) * ROWB + (((2 * j + hf) ^ (n & SWAP)) << 4)]);
             };
             constexpr int PART = KS < 8 ? KS : 8;   // reads of LDS ahead of their products
             u4 qf[PART];
@@ -720,27 +741,34 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
                 if constexpr (PLAIN) __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // what the rows of a tile see of this wave's cells: nothing, all, or some
-        auto idle = [&](int tt) { return tt + T <= wt0 || tt >= wt1; };
-        auto whole = [&](int tt) {
-            const int last = tt + T < t1 ? tt + T : t1;
-            if (cell0 + 32 > (a.mask ? q.base : q.base + tt + 1)) return false;
-            const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last - a.last;
-            return !(cell0 + 32 > a.first && cell0 < from);
-        };
+        // Tiles whose rows all see all of this wave's cells begin at tokens w_lo .. w_hi - 1. (A
+        // last tile of fewer tokens may be taken for one that does not.)
+        int w_lo, w_hi;
+        if (a.mask) {
+            const int from = q.base - (q.n_new < a.last ? a.last - q.n_new : 0);
+            w_lo = t0;
+            w_hi = cell0 + 32 <= q.base && !(cell0 + 32 > a.first && cell0 < from) ? t1 : t0;
+        } else {
+            w_lo = cell0 + 31 - q.base;
+            w_hi = cell0 + 32 > a.first && cell0 - q.base + a.last - T + 1 < t1 ? cell0 - q.base + a.last - T + 1 : t1;
+        }
+        if (w_hi <= w_lo) w_lo = w_hi = t1;
         int tt = t0, buf = 0;
         auto next = [&] {
             tt += T;
-            buf = (buf + 1) % BUFS;
+            buf = buf + 1 < BUFS ? buf + 1 : 0;
         };
         while (tt < t1) {
-            for (; tt < t1 && (idle(tt) || !whole(tt)); next()) {
-                arrive(tt, buf);
-                if (!idle(tt)) step(tt, buf, std::false_type{});
+            const int stop = tt >= w_hi ? t1 : w_lo < t1 ? w_lo : t1;
+            while (tt < stop) {
+                arrive();
+                if (tt + T > wt0 && tt < wt1) step(tt, buf, std::false_type{});
+                next();
             }
-            for (; tt < t1 && !idle(tt) && whole(tt); next()) {
-                arrive(tt, buf);
+            while (tt < w_hi && tt < t1) {
+                arrive();
                 step(tt, buf, std::true_type{});
+                next();
             }
         }
         wait_lds_loads<0>();
@@ -756,18 +784,27 @@ __global__ __launch_bounds__(256, D == 256 || BIAS ? 2 : 3) void k_weigh_tiles(W
                 v[i] = mine + __shfl_xor(theirs, m);
             }
         v[0] += __shfl_xor(v[0], 16);
-        if (n < 16) add_weight(w, c, h, cell0 + 8 * (n >> 2) + 4 * hf + (n & 3), v[0]);
+        if constexpr (RW == 2) {
+            if (rw == 1 && n < 16) join[cw][n][hf] = v[0];
+            __syncthreads();
+            if (rw == 0 && n < 16) v[0] += join[cw][n][hf];
+        }
+        if (rw == 0 && n < 16) add_weight(w, c, h, cell0 + 8 * (n >> 2) + 4 * hf + (n & 3), v[0]);
     }
 }
 
-template <int TYPE, int D> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
-    return w.a.bias ? launch(k_weigh_tiles<TYPE, D, true>, dim3((unsigned)blocks), dim3(256), st, w)
-                    : launch(k_weigh_tiles<TYPE, D, false>, dim3((unsigned)blocks), dim3(256), st, w);
+template <int TYPE, int D, int RW> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks), block(256 * RW);
+    return w.a.bias ? launch(k_weigh_tiles<TYPE, D, true, RW>, grid, block, st, w)
+                    : launch(k_weigh_tiles<TYPE, D, false, RW>, grid, block, st, w);
+}
+template <int TYPE, int RW> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
+    if (w.a.dk <= 64) return run_weigh_tiles<TYPE, 64, RW>(w, blocks, st);
+    if (w.a.dk <= 128) return run_weigh_tiles<TYPE, 128, RW>(w, blocks, st);
+    return run_weigh_tiles<TYPE, 256, RW>(w, blocks, st);
 }
 template <int TYPE> bool run_weigh_tiles(const WeighArgs & w, long long blocks, hipStream_t st) {
-    if (w.a.dk <= 64) return run_weigh_tiles<TYPE, 64>(w, blocks, st);
-    if (w.a.dk <= 128) return run_weigh_tiles<TYPE, 128>(w, blocks, st);
-    return run_weigh_tiles<TYPE, 256>(w, blocks, st);
+    return blocks <= 512 ? run_weigh_tiles<TYPE, 2>(w, blocks, st) : run_weigh_tiles<TYPE, 1>(w, blocks, st);
 }
 
 template <int TYPE, int QT, int D> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
@@ -815,7 +852,7 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     const bool few = rows <= 16 * (c->k_type == kF32 ? kFewRows32 : kFewRows16);
     // (strides that direct loads take)
     const bool tiles = !few && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
-                       x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23;
+                       x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23 && x->n_head < 1 << 20;
     const long long units = (long long)x->n_seq * c->n_head_kv;
     long long want = ((long long)x->max_len + 127) / 128;   // (128 cells are a block's)
     const long long most = kMaxBlocks / units;
