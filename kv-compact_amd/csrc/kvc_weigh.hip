@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     };
 
     unsigned kr[2][C::NKL][C::WK], next_kr[AHEAD ? 2 : 1][AHEAD ? C::NKL : 1][C::WK];
-    f4 bias[2], next_bias[2];
+    f4 bias[2], next_bias[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float old = 0.0f, next_old = 0.0f;
     unsigned short scales[2][NS];
     int page[2], next_page[2];
@@ -457,6 +457,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     f4 sc = {0, 0, 0, 0};
+                    float p[4];
                     if constexpr (TYPE == kF32) {
                         f4 part[4];
 #pragma unroll
@@ -485,12 +486,16 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
-                        float v = sc[i] * scale;
+                        float v = sc[i];
                         if constexpr (Q8 && QT == kBF16) v *= rest;
-                        if (a.bias) v += bias[x][i];
-                        const float p = exp_of(v - lse);
-                        sum[4 * x + i] += see >> (16 * x + 4 * g + i) & 1 ? p : 0.0f;
+                        p[i] = exp_of(__builtin_fmaf(v, scale, bias[x][i]) - lse);
                     }
+                    if (special) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) p[i] = see >> (16 * x + 4 * g + i) & 1 ? p[i] : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
                 }
             }
 #pragma unroll
