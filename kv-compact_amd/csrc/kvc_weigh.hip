@@ -25,7 +25,7 @@ struct WeighArgs {
     float decay;
     int tail, fresh;
     int cell_tiles;        // blocks of a sequence's head
-    int range;             // k_weigh_few: groups of 32 cells of each, at least
+    int range;             // k_weigh_few, k_weigh_ring: groups of 32 or 64 cells of each, at least
 };
 
 // What a block of a call works on.
@@ -524,6 +524,187 @@ template <int TYPE, int QT> bool run_weigh_few(const WeighArgs & w, long long ro
     return run_weigh_few<TYPE, QT, TYPE == kF32 ? kFewRows32 : kFewRows16>(w, careful, blocks, st);
 }
 
+// (4 bytes a lane, lanes' to side by side)
+__device__ __forceinline__ void load_lds4(const char * from, unsigned offset, char * to) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(from), "s"(at) : "m0", "memory");
+}
+
+// Up to 16 rows of aligned types: bound by the read of the keys. Each wave has a
+// ring of its own in LDS, 16 cells a place, filled by direct loads of 1 KB (whole
+// rows of a head; loads to registers in the products' layout take a row in four
+// pieces of 64 bytes), and no barrier. It goes through 64 cells at a time: their
+// biases and old weights are one load each, their sums one store.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
+    using C = RowKernel<TYPE, TYPE, D, 1, FULL>;
+    constexpr int ROWB = D * C::ES, PR = ROWB / 16;                  // bytes and pieces of a row
+    constexpr int RPL = 1024 / ROWB, NL = 16 / RPL;                   // rows of a direct load; loads of 16 cells
+    constexpr int BUFS = ROWB <= 128 ? 8 : ROWB <= 512 ? 4 : 2, AHEAD = BUFS - 1;   // (two blocks a CU, one from 512 bytes on)
+    constexpr int SWAP = PR < 16 ? PR - 1 : 15;                       // bits of a cell's number that its pieces are exchanged by
+    constexpr int GB = BUFS / 4 + 2;                                  // groups whose biases and weights are on their way or in use
+    __shared__ __align__(16) char ring[4][BUFS][16 * ROWB];
+    __shared__ __align__(16) float cell_bias[4][GB][64], cell_old[4][GB][64];
+    const AttnArgs & a = w.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    const int split = u % w.cell_tiles, s = u / w.cell_tiles;
+    Counted c;
+    if (!counted_of(w, s, c)) return;
+    const Sequence & q = c.q;
+    const int page_mask = (1 << a.shift) - 1;
+    const int all_rows = (q.n_new - c.tok_from) * a.G;
+    const int n_groups = (q.held + 63) >> 6;
+    const int even = (n_groups + w.cell_tiles - 1) / w.cell_tiles, per = even > w.range ? even : w.range;
+    const int g_lo = split * per, g_hi = g_lo + per < n_groups ? g_lo + per : n_groups;
+    const int groups = (g_hi - g_lo - wave + 3) >> 2;                 // of this wave: g_lo + wave, every fourth
+    if (g_lo + wave >= g_hi) return;
+    const int out_at = 16 * (m >> 2) + 4 * g + (m & 3);               // the cell of 64 whose sum this lane gets
+
+    unsigned load_off[NL];
+    bool load_on[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int row = i * RPL + lane / PR, piece = (lane % PR) ^ (row & SWAP);
+        load_off[i] = __umul24(row, a.k.ld_tok) + 16 * piece;
+        load_on[i] = piece * C::KV < a.dk;
+    }
+    if (a.dk < D)
+        for (int i = lane; i < BUFS * 16 * PR; i += 64) reinterpret_cast<u4 *>(ring[wave])[i] = u4{0, 0, 0, 0};
+
+    for (int row_lo = 0; row_lo < all_rows; row_lo += 16) {           // (more rows than the launch was told of: in turns)
+        const int rows = all_rows - row_lo < 16 ? all_rows - row_lo : 16;
+        // places of 16 cells in this wave's order
+        const int places = 4 * groups;
+        auto cell_of = [&](int t) { return 64 * (g_lo + wave + 4 * (t >> 2)) + 16 * (t & 3); };
+        auto page_of = [&](int t) {
+            const int cell = cell_of(t);
+            return t < places && cell < q.held ? uniform_load(q.table + (cell >> a.shift)) : -1;
+        };
+        int load_t = 0, load_buf = 0, load_page = page_of(0);
+        // (past the last place: page 0 again, for the count of loads; at least NL of each place)
+        auto fill = [&] {
+            const int cell = cell_of(load_t), page = load_page >= 0 && load_page < a.n_pages ? load_page : 0;
+            const unsigned row = ((unsigned)page << a.shift) + (cell & page_mask);
+            const char * from = a.k.base + h * a.k.ld_head + (unsigned long long)row * a.k.ld_tok;
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                if (load_on[i]) load_lds16(from, load_off[i], &ring[wave][load_buf][i * 1024]);
+            if ((load_t & 3) == 0 && load_t < places) {
+                // biases (-inf: not there) and old weights of 64 cells, a lane each
+                const int at = cell + lane, b = (load_t >> 2) % GB;
+                // (by scalar loads: the wait for a vector one would be one for the keys on their way)
+                const int pages[4] = {load_page, page_of(load_t + 1), page_of(load_t + 2), page_of(load_t + 3)};
+                int pg = lane < 32 ? (lane < 16 ? pages[0] : pages[1]) : lane < 48 ? pages[2] : pages[3];
+                if (at >= q.held) pg = -1;
+                const char * from_b = reinterpret_cast<const char *>(&hidden_word);
+                if (pg >= 0 && pg < a.n_pages)
+                    from_b = a.bias ? reinterpret_cast<const char *>(a.bias + (((long long)pg * a.H + h) << a.shift) + (at & page_mask))
+                                    : reinterpret_cast<const char *>(&zero_word);
+                load_lds4(from_b, reinterpret_cast<char *>(cell_bias[wave][b]));
+                const bool kept = row_lo ? at < q.held : w.decay != 0.0f && at < c.old;
+                load_lds4(kept ? reinterpret_cast<const char *>(w.weight + c.seq * w.w_seq + h * w.room + at)
+                               : reinterpret_cast<const char *>(&zero_word),
+                          reinterpret_cast<char *>(cell_old[wave][b]));
+            }
+            load_t++;
+            load_buf = load_buf + 1 < BUFS ? load_buf + 1 : 0;
+            load_page = page_of(load_t);
+        };
+        // this lane's row (those past the last repeat it, and give nothing)
+        const bool on = m < rows;
+        const int row = row_lo + (on ? m : rows - 1), tok = c.tok_from + row / a.G, head = row % a.G;
+        u4 qf[C::NK];
+        {
+            const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
+#pragma unroll
+            for (int j = 0; j < C::NK; j++) {
+                const int col = 4 * C::KV * j + C::KV * g;
+                qf[j] = col < a.dk ? *reinterpret_cast<const u4 *>(p + col * C::ES) : u4{0, 0, 0, 0};
+            }
+        }
+        float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
+        lse = on && lse != -INFINITY ? lse : INFINITY;
+        const int first_tok = c.tok_from + row_lo / a.G, last_tok = c.tok_from + (row_lo + rows - 1) / a.G;
+        const int clear = a.mask ? q.base : q.base + first_tok + 1;
+        const int cut = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
+        const int from = window_from(a, q, tok);
+        // (waited for here: a wait in the loop would be one for the keys on their way too)
+#pragma unroll
+        for (int j = 0; j < C::NK; j++) asm volatile("" : "+v"(qf[j]));
+        asm volatile("" : "+v"(lse));
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) fill();
+
+        float mine = 0.0f;
+        int buf = 0;
+        for (int t = 0; t < places; t++) {
+            wait_lds_loads<(AHEAD - 1) * NL>();
+            __builtin_amdgcn_wave_barrier();
+            const int cell0 = cell_of(t), b = (t >> 2) % GB;
+            f4 part[TYPE == kF32 ? 4 : 1];
+#pragma unroll
+            for (int e = 0; e < (TYPE == kF32 ? 4 : 1); e++) part[e] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < C::NK; j++) {
+                const u4 kf = *reinterpret_cast<const u4 *>(&ring[wave][buf][m * ROWB + (((4 * j + g) ^ (m & SWAP)) << 4)]);
+                if constexpr (TYPE == kF32) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]), __uint_as_float(qf[j][e]), part[e], 0, 0, 0);
+                } else {
+                    part[0] = mfma16<TYPE>(kf, qf[j], part[0]);
+                }
+            }
+            f4 sc = part[0];
+            if constexpr (TYPE == kF32) sc = (part[0] + part[1]) + (part[2] + part[3]);
+            const f4 bias = *reinterpret_cast<const f4 *>(&cell_bias[wave][b][16 * (t & 3) + 4 * g]);
+            float p[4];
+            // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = exp_of(__builtin_fmaf(sc[i], a.scale, bias[i]) - lse);
+            if (cell0 + 16 > clear || (cell0 + 16 > a.first && cell0 < cut)) {
+                const unsigned see = seen32(a, q, tok, cell0) & window32(a, from, cell0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[i] = see >> (4 * g + i) & 1 ? p[i] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = bias[i] == -INFINITY ? 0.0f : p[i];
+            // over the rows: lane m of the 16 gets cell m % 4's
+            auto dpp = [](float x, auto ctrl) {
+                return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, true));
+            };
+            const float p0 = (m & 2 ? p[2] : p[0]) + dpp(m & 2 ? p[0] : p[2], std::integral_constant<int, 0x4e>{});
+            const float p1 = (m & 2 ? p[3] : p[1]) + dpp(m & 2 ? p[1] : p[3], std::integral_constant<int, 0x4e>{});
+            float x = (m & 1 ? p1 : p0) + dpp(m & 1 ? p0 : p1, std::integral_constant<int, 0xb1>{});
+            x += dpp(x, std::integral_constant<int, 0x124>{});   // (rotations by four and eight lanes)
+            x += dpp(x, std::integral_constant<int, 0x128>{});
+            mine = m >> 2 == (t & 3) ? x : mine;
+            if ((t & 3) == 3) {
+                const int cell = cell0 - 48 + out_at;
+                const float old = cell_old[wave][b][out_at];
+                if (cell < q.held) w.weight[c.seq * w.w_seq + h * w.room + cell] = (row_lo ? old : w.decay * old) + mine;
+            }
+            // (what was read of this place is in registers: it may be filled again)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+            fill();
+            buf = buf + 1 < BUFS ? buf + 1 : 0;
+        }
+        wait_lds_loads<0>();
+    }
+}
+
+template <int TYPE> bool run_weigh_ring(const WeighArgs & w, long long blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks), block(256);
+    if (w.a.dk <= 64) return launch(k_weigh_ring<TYPE, 64>, grid, block, st, w);
+    if (w.a.dk <= 128) return launch(k_weigh_ring<TYPE, 128>, grid, block, st, w);
+    return launch(k_weigh_ring<TYPE, 256>, grid, block, st, w);
+}
+
 // More rows of 16-bit types: each of a block's four waves keeps the keys of 32
 // cells in registers and goes over all rows, tiles of 64 in LDS. Rows reach LDS
 // by direct loads, two tiles ahead (256-wide heads: one), pieces of 16 bytes exchanged by the row's
@@ -536,12 +717,6 @@ template <int TYPE, int QT> bool run_weigh_few(const WeighArgs & w, long long ro
 //
 // Without a bias the scores go into the exponential by one multiply-add (scale
 // and log2 e in one factor: each rounded once, as the separate steps are).
-// (4 bytes a lane, lanes' to side by side)
-__device__ __forceinline__ void load_lds4(const char * from, unsigned offset, char * to) {
-    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)to;
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(from), "s"(at) : "m0", "memory");
-}
-
 template <int TYPE, int D, bool BIAS, int RW>
 __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
     constexpr int CELLS = 128, ROWS = 64 * RW, KS = D / 16, CH = D / 8, ROWB = 2 * D;
@@ -855,6 +1030,7 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     const bool careful = c->k_type != kQ8 && (!vec_rows(x->q, es) || c->d_k * es % 16);
     const long long rows = (long long)(y->tail > 0 && y->tail < x->max_new ? y->tail : x->max_new) * a.G;
     const bool few = rows <= 16 * (c->k_type == kF32 ? kFewRows32 : kFewRows16);
+    const bool ring = rows <= 16 && !careful && c->k_type != kQ8;
     // (strides that direct loads take)
     const bool tiles = !few && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
                        x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23 && x->n_head < 1 << 20;
@@ -864,14 +1040,19 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     if (most < 1) return KV_COMPACT_E_UNSUPPORTED;
     if (few && want > (4095 + units) / units) want = (4095 + units) / units;
     w.cell_tiles = (int)(want < 1 ? 1 : want < most ? want : most);
-    w.range = (int)(((long long)x->max_len + 32LL * w.cell_tiles - 1) / (32LL * w.cell_tiles));
+    const int group = ring ? 64 : 32;
+    w.range = (int)(((long long)x->max_len + (long long)group * w.cell_tiles - 1) / ((long long)group * w.cell_tiles));
     w.a = a;
     const long long blocks = units * w.cell_tiles;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;
     bool ok;
-    if (few) {
+    if (ring) {
+        ok = c->k_type == kF32 ? run_weigh_ring<kF32>(w, blocks, st)
+             : c->k_type == kF16 ? run_weigh_ring<kF16>(w, blocks, st)
+                                 : run_weigh_ring<kBF16>(w, blocks, st);
+    } else if (few) {
         if (c->k_type == kF32) ok = run_weigh_few<kF32, kF32>(w, rows, careful, blocks, st);
         else if (c->k_type == kF16) ok = run_weigh_few<kF16, kF16>(w, rows, careful, blocks, st);
         else if (c->k_type == kBF16) ok = run_weigh_few<kBF16, kBF16>(w, rows, careful, blocks, st);
