@@ -1035,10 +1035,25 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     const bool tiles = !few && a.G <= 64 && !careful && (c->k_type == kF16 || c->k_type == kBF16) && x->q.ld_tok >= 0 &&
                        x->q.ld_tok < 1 << 23 && x->q.ld_head >= 0 && x->q.ld_head < 1 << 23 && x->n_head < 1 << 20;
     const long long units = (long long)x->n_seq * c->n_head_kv;
-    long long want = ((long long)x->max_len + 127) / 128;   // (128 cells are a block's)
     const long long most = kMaxBlocks / units;
     if (most < 1) return KV_COMPACT_E_UNSUPPORTED;
-    if (few && want > (4095 + units) / units) want = (4095 + units) / units;
+    // Blocks: 128 cells each where rows come by tiles or 16 at a time. Otherwise
+    // ranges of at least 512 cells (up to 16 rows; 256 above), or half of that
+    // where it leaves fewer than 512 blocks, and not more than fill the GPU many
+    // times. Measured, us (8 x 128, bf16; one token, ranges of 128, 256 and 512):
+    // one sequence of 2000 cells 6.5, 6.6 and 8.7, of 20000 15.9, 12.7 and 12.6;
+    // 16 of 2000 18.8, 13.8 and 11.4; 64 of up to 16384, 4096, 8192 and 16384
+    // blocks: 278, 266 and 262. 32 tokens, ranges of 128 and 256: one of 20000
+    // 24.5 and 21.6, 4 of 4096 15.4 and 17.4; 2048 and 4096 blocks: 8 of up to
+    // 20000 63.7 and 65, 32 of up to 16384 202 and 178.
+    long long want = ((long long)x->max_len + 127) / 128;
+    if (few) {
+        const int least = ring ? 512 : 256, fill = ring ? 16384 : 4096;
+        want = ((long long)x->max_len + least - 1) / least;
+        if (want * units < 512) want = ((long long)x->max_len + least / 2 - 1) / (least / 2);
+        const long long enough = (fill + units - 1) / units;
+        want = want < enough ? want : enough;
+    }
     w.cell_tiles = (int)(want < 1 ? 1 : want < most ? want : most);
     const int group = ring ? 64 : 32;
     w.range = (int)(((long long)x->max_len + (long long)group * w.cell_tiles - 1) / ((long long)group * w.cell_tiles));
