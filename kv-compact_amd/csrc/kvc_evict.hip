@@ -527,7 +527,12 @@ int kvc_cache_pick(const kvc_cache * c, int n, const kvc_pick_args * a, void * w
     const int units = p.groups * n;
     const long long want = p.max_len / 1024 + 1, most = (1 << 22) / units;
     p.parts = (int)(want < most ? want : most);
-    const bool fused = units >= 32;
+    // Keys by the picking blocks themselves, or by a launch of their own where
+    // those blocks are few and long: 32 layers, 20 % of one sequence kept and its
+    // weights moved, us (own launch, picking blocks): 5120 cells 20.6 and 20.0,
+    // 16384 30.6 and 36.7, 32768 48.6 and 63.9; 4 of up to 32768 79 both, 8 103
+    // both, 16 of up to 8192 62.3 and 54.1.
+    const bool fused = units >= 256 || p.max_len <= 8192;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;

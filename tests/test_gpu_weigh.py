@@ -246,3 +246,36 @@ def test_large_groups(dll, typ, cache, G):   # noqa: F811
 def test_many_sequences(dll, typ, cache):   # noqa: F811
     run_weigh(dll, typ, cache, [1 + 11 * i % 60 for i in range(150)], [1 + i % 2 if 1 + 11 * i % 60 > 1 else 1 for i in range(150)],
               1, 2, 64, seed=24, bias=True)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16])
+@pytest.mark.parametrize("G", [1, 5, 33, 64, 65])
+@pytest.mark.parametrize("announced", [None, 1 << 20])
+def test_groups_of_many_rows(dll, typ, G, announced):   # noqa: F811
+    # tiles of whole tokens with rows left over; four waves a block and (more cells announced: more blocks) eight
+    run_weigh(dll, typ, typ, [300, 90], [140, 90], 1, G, 64, page=32, window=(5, 100) if G == 5 else None, decay=1.0, seed=G,
+              max_len=announced)
+
+
+@pytest.mark.parametrize("d", [32, 72, 96, 128, 136, 256])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("announced", [None, 1 << 20])
+def test_head_widths_of_many_rows(dll, d, bias, announced):   # noqa: F811
+    run_weigh(dll, BF16, BF16, [290, 77], [200, 77], 2, 2, d, page=16, bias=bias, window=(20, 150), decay=0.5, tail=0, seed=d,
+              max_len=announced, runs=2)
+    run_weigh(dll, F16, F16, [290, 200], [200, 150], 1, 2, d, page=16, bias=bias, tree=True, words=3, decay=1.0, tail=150, seed=d,
+              max_len=announced)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("G", [1, 4])
+def test_bad_cells_under_many_rows(dll, typ, G):   # noqa: F811
+    # bad pages, keys that are not finite where nothing sees them, cells that the bias hides; one row and many
+    def edit(k, v, b, cell):
+        for j in (40, 41, 170):
+            p, c = cell(0, j)
+            k[p, c] = np.nan
+            b[p, :, c] = -np.inf
+    for news in ([1, 1], [200, 40]):
+        run_weigh(dll, typ, typ, [400, 300], news, 2, G, 128, page=16, bias=True, seed=G, edit=edit, decay=0.5,
+                  bad_pages=[(0, 4, -1), (0, 20, 1 << 30), (1, 0, -5)])
