@@ -63,177 +63,6 @@ __device__ __forceinline__ void add_weight(const WeighArgs & w, const Counted & 
     *at = (cell < c.old && w.decay != 0.0f ? w.decay * *at : 0.0f) + sum;
 }
 
-// Four waves of a block, 32 cells each; rows 16 at a time.
-template <int TYPE, int QT, int D, Columns COLS>
-__global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
-    using C = RowKernel<TYPE, QT, D, 1, COLS>;
-    constexpr bool Q8 = C::Q8;
-    __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
-    const AttnArgs & a = w.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m = lane & 15, g = lane >> 4;
-    int u = blockIdx.x;
-    const int h = u % a.H;
-    u /= a.H;
-    const int first_tile = u % w.cell_tiles, s = u / w.cell_tiles;
-    Counted c;
-    if (!counted_of(w, s, c)) return;
-    const Sequence & q = c.q;
-    const int page_mask = (1 << a.shift) - 1;
-
-    for (int tile = first_tile; tile * 128LL < q.held; tile += w.cell_tiles) {
-        const int cell0 = tile * 128 + 32 * wave;
-        if (cell0 >= q.held) continue;
-        int t0, t1;
-        tokens_of(a, c, cell0, cell0 + 32 < q.held ? cell0 + 32 : q.held, t0, t1);
-        float sum[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sum[x][i] = 0.0f;
-        if (t0 < t1) {
-            // keys, and the cells that are not to be read (bad pages; past the end)
-            unsigned kr[2][C::NKL][C::WK];
-            unsigned there = 0;
-            f4 bias[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int cell = cell0 + 16 * x;
-                int page = cell < q.held ? uniform_load(q.table + (cell >> a.shift)) : -1;
-                if (page >= 0 && page < a.n_pages)
-                    there |= (q.held - cell >= 16 ? 0xffffu : (1u << (q.held - cell)) - 1) << (16 * x);
-                else
-                    page = 0;
-                const unsigned row0 = ((unsigned)page << a.shift) + (cell & page_mask);
-                const char * p = a.k.base + h * a.k.ld_head + (unsigned long long)row0 * a.k.ld_tok;
-                const unsigned row = __umul24(m, a.k.ld_tok);
-#pragma unroll
-                for (int j = 0; j < C::NKL; j++) {
-                    if constexpr (Q8)
-                        *reinterpret_cast<u2 *>(kr[x][j]) =
-                            COLS == FULL || 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + (row + 34 * j + 2 + 8 * g)) : u2{0, 0};
-                    else
-                        load_cols<C::KV, C::ES, COLS>(p, row, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
-                }
-                if (a.bias)
-                    bias[x] = *reinterpret_cast<const f4 *>(a.bias + (((long long)page * a.H + h) << a.shift) + ((cell + 4 * g) & page_mask));
-                if constexpr (Q8) {
-                    // scales: lane g * 16 + m takes cell m's blocks g, g + 4, ...
-#pragma unroll
-                    for (int b = 0; b < (C::NB + 3) / 4; b++) {
-                        const int at = 4 * b + g;
-                        if (at < C::NB)
-                            k_scale[wave][at][16 * x + m] =
-                                COLS == FULL || 32 * at < a.dk ? f16_value(*reinterpret_cast<const unsigned short *>(p + row + 34 * at)) : 0.0f;
-                    }
-                }
-            }
-            bool hidden = there != ~0u;   // (uniform) a cell that no row sees
-            if (a.bias) {
-                unsigned off = 0;
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) off |= bias[x][i] == -INFINITY ? 1u << (16 * x + 4 * g + i) : 0;
-                there &= ~off;
-                hidden |= __ballot(off != 0) != 0;
-            }
-            if constexpr (Q8) {
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            }
-            const int row_end = t1 * a.G;
-            for (int row0 = t0 * a.G; row0 < row_end; row0 += 16) {
-                const int row = row0 + m;
-                const bool on = row < row_end;
-                const int tok = (on ? row : row0) / a.G, head = (on ? row : row0) % a.G;
-                u4 qf[C::NK];
-                const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
-#pragma unroll
-                for (int j = 0; j < C::NK; j++) {
-                    const int col = 4 * C::KV * j + C::KV * g;
-                    if constexpr (Q8) {
-                        qf[j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
-                    } else {
-                        unsigned x[4];
-                        load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, x);
-                        qf[j] = u4{x[0], x[1], x[2], x[3]};
-                    }
-                }
-                float scale = a.scale, rest = 1.0f;
-                if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(qf, a.scale, scale, rest);
-                float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
-                lse = on && lse != -INFINITY ? lse : INFINITY;   // (a row that saw nothing gives nothing)
-                // keys that every row of the tile sees
-                const int clear = a.mask ? q.base : q.base + row0 / a.G + 1;
-                const int last_tok = (row0 + 15 < row_end ? row0 + 15 : row_end - 1) / a.G;
-                const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
-                const bool special = hidden || row0 + 16 > row_end || cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
-                unsigned see = there;
-                if (special) {
-                    see &= seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
-                    see = on ? see : 0;
-                }
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    f4 sc = {0, 0, 0, 0};
-                    if constexpr (TYPE == kF32) {
-                        f4 part[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) part[e] = f4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < C::NKL; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][j][e]),
-                                                                               __uint_as_float(qf[j][e]), part[e], 0, 0, 0);
-                        sc = (part[0] + part[1]) + (part[2] + part[3]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
-                        if constexpr (Q8) {
-                            unsigned y[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                y[e] = code_pair(kr[x][j][e >> 1], kr[x][j][e >> 1], e & 1 ? 0x0c030c02u : 0x0c010c00u);
-                            const f4 f = *reinterpret_cast<const f4 *>(&k_scale[wave][j][16 * x + 4 * g]);
-                            sc += f * mfma16<kF16>(u4{y[0], y[1], y[2], y[3]}, qf[j], f4{0, 0, 0, 0});
-                        } else {
-                            sc = mfma16<C::MT>(u4{kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]}, qf[j], sc);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
-                        float v = sc[i] * scale;
-                        if constexpr (Q8 && QT == kBF16) v *= rest;
-                        if (a.bias) v += bias[x][i];
-                        const float p = exp_of(v - lse);
-                        sum[x][i] += !special || (see >> (16 * x + 4 * g + i) & 1) ? p : 0.0f;
-                    }
-                }
-            }
-        }
-        // over the rows; then cell 16 x + 4 g + i is lane 16 g + 4 x + i's
-        float mine = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float v = sum[x][i];
-                for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o);
-                mine = m == 4 * x + i ? v : mine;
-            }
-        if (m < 8) add_weight(w, c, h, cell0 + 16 * (m >> 2) + 4 * g + (m & 3), mine);
-    }
-}
-
-// Few rows: 16 RT of them stay (RT = 1: in registers, more in LDS as the
-// fragments they are), and a block's waves go through a range of cells, 32 at a
-// time, the next ones' keys, biases and old weights on their way meanwhile.
-// (More rows than the launch was told of come in turns of as many; a cell's
-// weight is then added to by the lane that wrote it.)
 constexpr int kFewRows16 = 8, kFewRows32 = 4;   // row tiles of 16 that stay, of 16-bit and F32 rows
 
 // Sum over the 16 lanes of a row of v[m % 8] (lanes m and m ^ 8 alike): each
@@ -261,6 +90,191 @@ __device__ __forceinline__ float sum_of_16(float (&v)[8], int m) {
     const float x = mine + dpp(theirs, xor1{});
     return x + dpp(x, ror8{});
 }
+
+// Many rows of F32 or over Q8_0 keys, and rows of any alignment: four waves of a
+// block keep 32 cells' keys each in registers (Q8_0 ones decoded), and rows come
+// 16 RT at a time through LDS, as the fragments they are, for all four.
+template <int TYPE, int QT, int D, int RT, Columns COLS>
+__global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
+    using C = RowKernel<TYPE, QT, D, 1, COLS>;
+    constexpr bool Q8 = C::Q8;
+    __shared__ __align__(16) u4 rows_q[RT][C::NK][64];
+    __shared__ float rows_scale[Q8 ? RT : 1][2][16];
+    __shared__ float rows_lse[RT][16];
+    __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
+    const AttnArgs & a = w.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    int u = blockIdx.x;
+    const int h = u % a.H;
+    u /= a.H;
+    const int first_tile = u % w.cell_tiles, s = u / w.cell_tiles;
+    Counted c;
+    if (!counted_of(w, s, c)) return;
+    const Sequence & q = c.q;
+    const int page_mask = (1 << a.shift) - 1;
+
+    for (int tile = first_tile; tile * 128LL < q.held; tile += w.cell_tiles) {
+        const int block0 = tile * 128, cell0 = block0 + 32 * wave;
+        int t0, t1;   // the block's tokens (a wave past the sequence's end has none that see its cells)
+        tokens_of(a, c, block0, block0 + 128 < q.held ? block0 + 128 : q.held, t0, t1);
+        float sum[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] = 0.0f;
+        // keys, and the cells that rows may see (not those of bad pages or past the end)
+        unsigned kr[2][C::NKL][Q8 ? 4 : C::WK];
+        f4 ks[Q8 ? 2 : 1][Q8 ? C::NB : 1];
+        unsigned there = 0;
+        f4 bias[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int cell = cell0 + 16 * x;
+            int page = cell < q.held ? uniform_load(q.table + (cell >> a.shift)) : -1;
+            if (page >= 0 && page < a.n_pages)
+                there |= (q.held - cell >= 16 ? 0xffffu : (1u << (q.held - cell)) - 1) << (16 * x);
+            else
+                page = 0;
+            const unsigned row0 = ((unsigned)page << a.shift) + (cell & page_mask);
+            const char * p = a.k.base + h * a.k.ld_head + (unsigned long long)row0 * a.k.ld_tok;
+            const unsigned row = __umul24(m, a.k.ld_tok);
+#pragma unroll
+            for (int j = 0; j < C::NKL; j++) {
+                if constexpr (Q8) {
+                    const u2 y = COLS == FULL || 32 * j < a.dk ? *reinterpret_cast<const u2_any *>(p + (row + 34 * j + 2 + 8 * g)) : u2{0, 0};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) kr[x][j][e] = code_pair(y[e >> 1], y[e >> 1], e & 1 ? 0x0c030c02u : 0x0c010c00u);
+                } else {
+                    load_cols<C::KV, C::ES, COLS>(p, row, 4 * C::KV * j + C::KV * g, a.dk, kr[x][j]);
+                }
+            }
+            if (a.bias)
+                bias[x] = *reinterpret_cast<const f4 *>(a.bias + (((long long)page * a.H + h) << a.shift) + ((cell + 4 * g) & page_mask));
+            if constexpr (Q8) {
+                // lane g * 16 + m: blocks g, g + 4, ... of cell m, on their way to the lanes that hold its sums
+#pragma unroll
+                for (int b = 0; b < (C::NB + 3) / 4; b++) {
+                    const int at = 4 * b + g;
+                    if (at < C::NB)
+                        k_scale[wave][at][16 * x + m] =
+                            COLS == FULL || 32 * at < a.dk ? f16_value(*reinterpret_cast<const unsigned short *>(p + row + 34 * at)) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (bias[x][i] == -INFINITY) there &= ~(1u << (16 * x + 4 * g + i));
+        }
+        if constexpr (Q8) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int j = 0; j < C::NB; j++) ks[x][j] = *reinterpret_cast<const f4 *>(&k_scale[wave][j][16 * x + 4 * g]);
+        }
+        const int row_end = t1 * a.G;
+        for (int turn = t0 * a.G; turn < row_end; turn += 16 * RT) {
+            const int rows = row_end - turn < 16 * RT ? row_end - turn : 16 * RT, row_tiles = (rows + 15) >> 4;
+            __syncthreads();   // (the rows before are read)
+            for (int r = wave; r < row_tiles; r += 4) {
+                const bool on = 16 * r + m < rows;
+                const int row = turn + (on ? 16 * r + m : rows - 1), tok = row / a.G, head = row % a.G;
+                const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
+                u4 qf[C::NK];
+#pragma unroll
+                for (int j = 0; j < C::NK; j++) {
+                    const int col = 4 * C::KV * j + C::KV * g;
+                    if constexpr (Q8) {
+                        qf[j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
+                    } else {
+                        unsigned x[4];
+                        load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, x);
+                        qf[j] = u4{x[0], x[1], x[2], x[3]};
+                    }
+                }
+                float scale = a.scale, rest = 1.0f;
+                if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(qf, a.scale, scale, rest);
+#pragma unroll
+                for (int j = 0; j < C::NK; j++) rows_q[r][j][lane] = qf[j];
+                if (g == 0) {
+                    const float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
+                    rows_lse[r][m] = on && lse != -INFINITY ? lse : INFINITY;   // (a row that saw nothing gives nothing)
+                    if constexpr (Q8) {
+                        rows_scale[r][0][m] = scale;
+                        rows_scale[r][1][m] = rest;
+                    }
+                }
+            }
+            __syncthreads();
+            if (cell0 >= q.held) continue;
+            for (int r = 0; r < row_tiles; r++) {
+                const int row0 = turn + 16 * r, last_row = row0 + 15 < row_end ? row0 + 15 : row_end - 1;
+                const int first_tok = row0 / a.G, last_tok = last_row / a.G;
+                if (!a.mask && cell0 > q.base + last_tok) continue;   // (no row of the tile sees the cells)
+                u4 qf[C::NK];
+#pragma unroll
+                for (int j = 0; j < C::NK; j++) qf[j] = rows_q[r][j][lane];
+                const float lse = rows_lse[r][m], scale = Q8 ? rows_scale[r][0][m] : a.scale, rest = Q8 ? rows_scale[r][1][m] : 1.0f;
+                const int clear = a.mask ? q.base : q.base + first_tok + 1;
+                const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
+                const bool special = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
+                unsigned see = ~0u;
+                if (special) {
+                    const int tok = (row0 + m < row_end ? row0 + m : row_end - 1) / a.G;
+                    see = seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    f4 sc = {0, 0, 0, 0};
+                    if constexpr (TYPE == kF32) {
+                        f4 part[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) part[e] = f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < C::NKL; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][j][e]),
+                                                                               __uint_as_float(qf[j][e]), part[e], 0, 0, 0);
+                        sc = (part[0] + part[1]) + (part[2] + part[3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
+                        const u4 kf = {kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]};
+                        if constexpr (Q8)
+                            sc += ks[x][j] * mfma16<kF16>(kf, qf[j], f4{0, 0, 0, 0});
+                        else
+                            sc = mfma16<C::MT>(kf, qf[j], sc);
+                    }
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
+                        float v = sc[i];
+                        if constexpr (Q8 && QT == kBF16) v *= rest;
+                        p[i] = exp_of(__builtin_fmaf(v, scale, bias[x][i]) - lse);
+                    }
+                    if (special) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) p[i] = see >> (16 * x + 4 * g + i) & 1 ? p[i] : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
+        const float all = sum_of_16(sum, m);
+        if (m < 8) add_weight(w, c, h, cell0 + 16 * (m >> 2) + 4 * g + (m & 3), all);
+    }
+}
+
+// Few rows: 16 RT of them stay (RT = 1: in registers, more in LDS as the
+// fragments they are), and a block's waves go through a range of cells, 32 at a
+// time, the next ones' keys, biases and old weights on their way meanwhile.
+// (More rows than the launch was told of come in turns of as many; a cell's
+// weight is then added to by the lane that wrote it.)
 
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
@@ -988,11 +1002,12 @@ template <int TYPE> bool run_weigh_tiles(const WeighArgs & w, long long blocks, 
 }
 
 template <int TYPE, int QT, int D> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
+    constexpr int RT = TYPE == kF32 ? kFewRows32 : kFewRows16;
     const dim3 grid((unsigned)blocks), block(256);
     if constexpr (TYPE != kQ8)
-        if (careful) return launch(k_weigh_rows<TYPE, QT, D, ANY>, grid, block, st, w);
-    if (w.a.dk == D) return launch(k_weigh_rows<TYPE, QT, D, FULL>, grid, block, st, w);
-    return launch(k_weigh_rows<TYPE, QT, D, PART>, grid, block, st, w);
+        if (careful) return launch(k_weigh_rows<TYPE, QT, D, RT, ANY>, grid, block, st, w);
+    if (w.a.dk == D) return launch(k_weigh_rows<TYPE, QT, D, RT, FULL>, grid, block, st, w);
+    return launch(k_weigh_rows<TYPE, QT, D, RT, PART>, grid, block, st, w);
 }
 template <int TYPE, int QT> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
     if (w.a.dk <= 64) return run_weigh<TYPE, QT, 64>(w, careful, blocks, st);
