@@ -8,6 +8,9 @@
  *   kvc_cache_*        pages: reserve, write, fork, free, compact, read
  *   kvc_attn_cache     attention of new or drafted tokens over the cache,
  *                      with the per-head bias (beta) a compaction fits
+ *   kvc_attn_*_window  both with a sliding window and first tokens that stay
+ *   kvc_cache_weigh,   the softmax weight each cell gathers, the cells to keep
+ *     _pick, _take_weights   by it, and weights that follow a fork or compaction
  *
  * A serving step: kvc_cache_extend reserves the new tokens' cells, each layer
  * writes its K and V rows (kvc_cache_write) and attends (kvc_attn_cache).
@@ -15,6 +18,8 @@
  * kvc_compact_layers_device or kvc_compact_quantized_layers_device, and
  * kvc_cache_compact keeps the cells they select, with the refitted values
  * and beta.
+ * Without a fit: kvc_cache_weigh behind each attention, kvc_cache_pick where a
+ * sequence is past its budget, and its indices into kvc_cache_compact.
  *
  * All pointers inside the structs are device (HBM) memory of the stream's
  * device. Every call queues its work on `stream` (NULL: the default stream of

@@ -226,6 +226,11 @@ __device__ void plan_of(const PickArgs & p, int i, int & k, int & to, int & seq_
 // hundred, are then listed in LDS with their wave, and the other 21 bits and each
 // wave's counts come from the list: three passes over the cells in all. Where
 // they are too many for the list, the passes go on over all cells.
+//
+// 20 % of 16 sequences of up to 32768 cells, 32 layers, 8 heads: 98 us, 70 of them
+// the read of the weights (313 MB, 4.5 TB/s; the longest sequences' blocks), then
+// the search, in which all blocks are at once. One sequence of 5120 cells: 15 us,
+// a chain of latencies (passes over L2, barriers).
 constexpr int kList = 4096;
 
 template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArgs p) {
@@ -426,7 +431,9 @@ struct TakeArgs {
 // A block per request, layer and head. Places are filled in ascending order and
 // no cell moves down, so that a row can be moved within itself: what a step of
 // the block reads is at or behind what it writes. A step is 16 cells a thread:
-// two rounds of loads in all for most budgets.
+// two rounds of loads in all for most budgets. Bound by HBM: picking a fifth of
+// the cells touches nearly every line, so that what 16 sequences of up to 32768
+// cells keep, 32 layers of 8 heads, takes 85 us: 400 MB, 4.7 TB/s.
 __global__ __launch_bounds__(256) void k_take_weights(TakeArgs p) {
     constexpr int STEP = 4096;
     for (long long u = blockIdx.x; u < (long long)p.n * p.n_layers * p.H; u += gridDim.x) {

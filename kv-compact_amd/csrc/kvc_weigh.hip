@@ -63,6 +63,11 @@ __device__ __forceinline__ void add_weight(const WeighArgs & w, const Counted & 
     *at = (cell < c.old && w.decay != 0.0f ? w.decay * *at : 0.0f) + sum;
 }
 
+// Blocks of 128 cells below which k_weigh_rows splits rows over waves. One prompt,
+// 8 KV heads of 128, 32 heads, whole and split, us: F32 1024 tokens 401 and 165,
+// 4096 (256 blocks) 1621 and 1086, 8192 3972 and 4244; over Q8_0 1024 tokens 184
+// and 100, 4096 718 and 444, 8192 1526 and 1473, 16384 3298 and 5638.
+constexpr int kSplit = 512;
 constexpr int kFewRows16 = 8, kFewRows32 = 4;   // row tiles of 16 that stay, of 16-bit and F32 rows
 
 // Sum over the 16 lanes of a row of v[m % 8] (lanes m and m ^ 8 alike): each
@@ -93,15 +98,21 @@ __device__ __forceinline__ float sum_of_16(float (&v)[8], int m) {
 
 // Many rows of F32 or over Q8_0 keys, and rows of any alignment: four waves of a
 // block keep 32 cells' keys each in registers (Q8_0 ones decoded), and rows come
-// 16 RT at a time through LDS, as the fragments they are, for all four.
-template <int TYPE, int QT, int D, int RT, Columns COLS>
+// 16 RT at a time through LDS, as the fragments they are, for all four. SPLIT,
+// for few blocks: the four have the same 32 cells and every fourth row tile each.
+// Bound by what a row tile issues in turn (F32: 32 products in a chain of four
+// sums): 4096 tokens of 32 heads of 128, F32 1.09 ms, 64 TFLOP/s (a large product:
+// 152); over Q8_0 0.44 ms, 155 TFLOP/s, 16384 tokens 3.3 ms, 333 TFLOP/s.
+template <int TYPE, int QT, int D, int RT, Columns COLS, bool SPLIT>
 __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
+    constexpr int CELLS = SPLIT ? 32 : 128;
     using C = RowKernel<TYPE, QT, D, 1, COLS>;
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) u4 rows_q[RT][C::NK][64];
     __shared__ float rows_scale[Q8 ? RT : 1][2][16];
     __shared__ float rows_lse[RT][16];
     __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
+    __shared__ float join[SPLIT ? 4 : 1][32];
     const AttnArgs & a = w.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, g = lane >> 4;
@@ -114,10 +125,10 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
     const Sequence & q = c.q;
     const int page_mask = (1 << a.shift) - 1;
 
-    for (int tile = first_tile; tile * 128LL < q.held; tile += w.cell_tiles) {
-        const int block0 = tile * 128, cell0 = block0 + 32 * wave;
+    for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
+        const int block0 = tile * CELLS, cell0 = SPLIT ? block0 : block0 + 32 * wave;
         int t0, t1;   // the block's tokens (a wave past the sequence's end has none that see its cells)
-        tokens_of(a, c, block0, block0 + 128 < q.held ? block0 + 128 : q.held, t0, t1);
+        tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
         float sum[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] = 0.0f;
@@ -207,7 +218,7 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
             }
             __syncthreads();
             if (cell0 >= q.held) continue;
-            for (int r = 0; r < row_tiles; r++) {
+            for (int r = SPLIT ? wave : 0; r < row_tiles; r += SPLIT ? 4 : 1) {
                 const int row0 = turn + 16 * r, last_row = row0 + 15 < row_end ? row0 + 15 : row_end - 1;
                 const int first_tok = row0 / a.G, last_tok = last_row / a.G;
                 if (!a.mask && cell0 > q.base + last_tok) continue;   // (no row of the tile sees the cells)
@@ -265,7 +276,14 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
-        const float all = sum_of_16(sum, m);
+        float all = sum_of_16(sum, m);
+        if constexpr (SPLIT) {
+            const int at = 16 * (m >> 2 & 1) + 4 * g + (m & 3);
+            if (m < 8) join[wave][at] = all;
+            __syncthreads();
+            all = (join[0][at] + join[1][at]) + (join[2][at] + join[3][at]);
+            if (wave) continue;   // (a next tile's sums come behind its barriers)
+        }
         if (m < 8) add_weight(w, c, h, cell0 + 16 * (m >> 2) + 4 * g + (m & 3), all);
     }
 }
@@ -275,6 +293,10 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
 // time, the next ones' keys, biases and old weights on their way meanwhile.
 // (More rows than the launch was told of come in turns of as many; a cell's
 // weight is then added to by the lane that wrote it.)
+// The last 32 tokens of 32 heads over eight F16 caches of up to 20000 cells, 8 x
+// 128 with a bias: 71 us, 3.0 TB/s; half of a block's time is its beginning (rows
+// to LDS) and the last blocks of ragged sequences. One token of 64 sequences of
+// up to 16384 Q8_0 cells: 256 us.
 
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
@@ -549,6 +571,9 @@ __device__ __forceinline__ void load_lds4(const char * from, unsigned offset, ch
 // rows of a head; loads to registers in the products' layout take a row in four
 // pieces of 64 bytes), and no barrier. It goes through 64 cells at a time: their
 // biases and old weights are one load each, their sums one store.
+// One token of 32 heads over 64 sequences of up to 16384 bf16 cells, 8 x 128: 262
+// us, 5.0 TB/s (a plain read: 6.8; keys in registers, a group of 32 cells ahead:
+// 290 us). One sequence of 20000 cells: 12.7 us.
 template <int TYPE, int D>
 __global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
     using C = RowKernel<TYPE, TYPE, D, 1, FULL>;
@@ -731,6 +756,12 @@ template <int TYPE> bool run_weigh_ring(const WeighArgs & w, long long blocks, h
 //
 // Without a bias the scores go into the exponential by one multiply-add (scale
 // and log2 e in one factor: each rounded once, as the separate steps are).
+//
+// Bound by the exponentials: 512 of a tile's 900 cycles of vector instructions in
+// a wave, its products 512 beside them. A prompt of 16384 tokens of 32 heads of
+// 128: 1.21 to 1.24 ms, 890 to 911 TFLOP/s (a large product: 1208; with two waves a
+// SIMD, 64 cells each, 1.40 ms); 32768 tokens 963 TFLOP/s, 4096 tokens, eight
+// waves a block, 162 us (224 with four).
 template <int TYPE, int D, bool BIAS, int RW>
 __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
     constexpr int CELLS = 128, ROWS = 64 * RW, KS = D / 16, CH = D / 8, ROWB = 2 * D;
@@ -1001,18 +1032,21 @@ template <int TYPE> bool run_weigh_tiles(const WeighArgs & w, long long blocks, 
     return blocks <= 512 ? run_weigh_tiles<TYPE, 2>(w, blocks, st) : run_weigh_tiles<TYPE, 1>(w, blocks, st);
 }
 
-template <int TYPE, int QT, int D> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
+template <int TYPE, int QT, int D, bool SPLIT> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
     constexpr int RT = TYPE == kF32 ? kFewRows32 : kFewRows16;
     const dim3 grid((unsigned)blocks), block(256);
     if constexpr (TYPE != kQ8)
-        if (careful) return launch(k_weigh_rows<TYPE, QT, D, RT, ANY>, grid, block, st, w);
-    if (w.a.dk == D) return launch(k_weigh_rows<TYPE, QT, D, RT, FULL>, grid, block, st, w);
-    return launch(k_weigh_rows<TYPE, QT, D, RT, PART>, grid, block, st, w);
+        if (careful) return launch(k_weigh_rows<TYPE, QT, D, RT, ANY, SPLIT>, grid, block, st, w);
+    if (w.a.dk == D) return launch(k_weigh_rows<TYPE, QT, D, RT, FULL, SPLIT>, grid, block, st, w);
+    return launch(k_weigh_rows<TYPE, QT, D, RT, PART, SPLIT>, grid, block, st, w);
 }
-template <int TYPE, int QT> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
-    if (w.a.dk <= 64) return run_weigh<TYPE, QT, 64>(w, careful, blocks, st);
-    if (w.a.dk <= 128) return run_weigh<TYPE, QT, 128>(w, careful, blocks, st);
-    return run_weigh<TYPE, QT, 256>(w, careful, blocks, st);
+template <int TYPE, int QT, bool SPLIT> bool run_weigh(const WeighArgs & w, bool careful, long long blocks, hipStream_t st) {
+    if (w.a.dk <= 64) return run_weigh<TYPE, QT, 64, SPLIT>(w, careful, blocks, st);
+    if (w.a.dk <= 128) return run_weigh<TYPE, QT, 128, SPLIT>(w, careful, blocks, st);
+    return run_weigh<TYPE, QT, 256, SPLIT>(w, careful, blocks, st);
+}
+template <int TYPE, int QT> bool run_weigh(const WeighArgs & w, bool split, bool careful, long long blocks, hipStream_t st) {
+    return split ? run_weigh<TYPE, QT, true>(w, careful, blocks, st) : run_weigh<TYPE, QT, false>(w, careful, blocks, st);
 }
 
 }  // namespace
@@ -1069,6 +1103,8 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
         const long long enough = (fill + units - 1) / units;
         want = want < enough ? want : enough;
     }
+    const bool split = !few && !tiles && want * units < kSplit;
+    if (split) want = ((long long)x->max_len + 31) / 32;
     w.cell_tiles = (int)(want < 1 ? 1 : want < most ? want : most);
     const int group = ring ? 64 : 32;
     w.range = (int)(((long long)x->max_len + (long long)group * w.cell_tiles - 1) / ((long long)group * w.cell_tiles));
@@ -1090,10 +1126,10 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
         else ok = run_weigh_few<kQ8, kBF16>(w, rows, careful, blocks, st);
     } else if (tiles) {
         ok = c->k_type == kF16 ? run_weigh_tiles<kF16>(w, blocks, st) : run_weigh_tiles<kBF16>(w, blocks, st);
-    } else if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, careful, blocks, st);
-    else if (c->k_type == kF16) ok = run_weigh<kF16, kF16>(w, careful, blocks, st);
-    else if (c->k_type == kBF16) ok = run_weigh<kBF16, kBF16>(w, careful, blocks, st);
-    else if (x->type == kF16) ok = run_weigh<kQ8, kF16>(w, careful, blocks, st);
-    else ok = run_weigh<kQ8, kBF16>(w, careful, blocks, st);
+    } else if (c->k_type == kF32) ok = run_weigh<kF32, kF32>(w, split, careful, blocks, st);
+    else if (c->k_type == kF16) ok = run_weigh<kF16, kF16>(w, split, careful, blocks, st);
+    else if (c->k_type == kBF16) ok = run_weigh<kBF16, kBF16>(w, split, careful, blocks, st);
+    else if (x->type == kF16) ok = run_weigh<kQ8, kF16>(w, split, careful, blocks, st);
+    else ok = run_weigh<kQ8, kBF16>(w, split, careful, blocks, st);
     return ok ? 0 : KV_COMPACT_E_DEVICE;
 }
