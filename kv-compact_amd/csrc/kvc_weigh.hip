@@ -11,6 +11,7 @@
 // up the keys' weights over the row tiles; lanes are summed at the end.
 #include "kvc_attn_kernels.h"
 
+#include <type_traits>
 #pragma clang fp contract(fast)
 
 namespace kvc {
@@ -294,10 +295,10 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
 // (More rows than the launch was told of come in turns of as many; a cell's
 // weight is then added to by the lane that wrote it.)
 // The last 32 tokens of 32 heads over eight F16 caches of up to 20000 cells, 8 x
-// 128 with a bias: 71 us, 3.0 TB/s; half of a block's time is its beginning (rows
-// to LDS) and the last blocks of ragged sequences. One token of 64 sequences of
-// up to 16384 Q8_0 cells: 256 us.
-
+// 128 with a bias: 57 us, 3.8 TB/s; its reads with one row tile of eight 49 us. (Asking once a
+// group of cells, not for each 16 rows, whether some row sees less: 62 us, 71
+// before, for two divisions and a branch beside eight products.) One token of 64
+// sequences of up to 16384 Q8_0 cells: 244 us.
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     using C = RowKernel<TYPE, QT, D, 1, COLS>;
@@ -397,6 +398,10 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     for (; row_lo < all_rows; row_lo += 16 * RT) {
         rows = all_rows - row_lo < 16 * RT ? all_rows - row_lo : 16 * RT;
         const int row_tiles = (rows + 15) >> 4, t0 = g_lo + wave;
+        // cells that every row of the turn sees: those before clear, first or not before from
+        const int first_tok = c.tok_from + row_lo / a.G, last_tok = c.tok_from + (row_lo + rows - 1) / a.G;
+        const int clear = a.mask ? q.base : q.base + first_tok + 1;
+        const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
         pages_of(t0, page);
         pages_of(t0 + 4, next_page);
         if constexpr (AHEAD)
@@ -464,9 +469,8 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
             float sum[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) sum[i] = 0.0f;
-            for (int r = 0; r < (RT == 1 ? 1 : row_tiles); r++) {
-                const int row0 = 16 * r, last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
-                const int first_tok = c.tok_from + (row_lo + row0) / a.G, last_tok = c.tok_from + (row_lo + last_row) / a.G;
+            auto sixteen = [&](int r, auto hides) {   // (a constant where there are tiles)
+                const int row0 = 16 * r;
                 u4 qr[C::NK];
                 float lse = lse0, scale = scale0, rest = rest0;
                 if constexpr (RT > 1) {
@@ -482,11 +486,8 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
 #pragma unroll
                     for (int j = 0; j < C::NK; j++) qr[j] = q0[j];
                 }
-                const int clear = a.mask ? q.base : q.base + first_tok + 1;
-                const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
-                const bool special = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
                 unsigned see = ~0u;
-                if (special) {
+                if (hides) {
                     const int row = row0 + m < rows ? row0 + m : rows - 1, tok = c.tok_from + (row_lo + row) / a.G;
                     see = seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
                 }
@@ -526,13 +527,21 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
                         if constexpr (Q8 && QT == kBF16) v *= rest;
                         p[i] = exp_of(__builtin_fmaf(v, scale, bias[x][i]) - lse);
                     }
-                    if (special) {
+                    if (hides) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) p[i] = see >> (16 * x + 4 * g + i) & 1 ? p[i] : 0.0f;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
                 }
+            };
+            const bool hides = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
+            if constexpr (RT == 1) {
+                sixteen(0, hides);
+            } else if (hides) {
+                for (int r = 0; r < row_tiles; r++) sixteen(r, std::true_type{});
+            } else {
+                for (int r = 0; r < row_tiles; r++) sixteen(r, std::false_type{});
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
@@ -1093,15 +1102,19 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     // one sequence of 2000 cells 6.5, 6.6 and 8.7, of 20000 15.9, 12.7 and 12.6;
     // 16 of 2000 18.8, 13.8 and 11.4; 64 of up to 16384, 4096, 8192 and 16384
     // blocks: 278, 266 and 262. 32 tokens, ranges of 128 and 256: one of 20000
-    // 24.5 and 21.6, 4 of 4096 15.4 and 17.4; 2048 and 4096 blocks: 8 of up to
-    // 20000 63.7 and 65, 32 of up to 16384 202 and 178.
+    // 24.5 and 21.6, 4 of 4096 15.4 and 17.4. Above 16 rows, or over Q8_0, ten
+    // blocks a CU, an odd number of ranges of each sequence (an even one keeps a
+    // CU at the same range of every sequence): 2048, 2560 and 4096 blocks, 32
+    // tokens, 8 of up to 20000 55, 53 and 60, 24 of up to 16000 134, 133 and 132;
+    // Q8_0, one token, 64 of up to 16384 in 4, 5, 7 and 8 ranges 312, 246, 230 and
+    // 256, 128 of up to 8192 in 2, 3 and 4 ranges 309, 231 and 307.
     long long want = ((long long)x->max_len + 127) / 128;
     if (few) {
-        const int least = ring ? 512 : 256, fill = ring ? 16384 : 4096;
+        const int least = ring ? 512 : 256, fill = ring ? 16384 : 2560;
         want = ((long long)x->max_len + least - 1) / least;
         if (want * units < 512) want = ((long long)x->max_len + least / 2 - 1) / (least / 2);
         const long long enough = (fill + units - 1) / units;
-        want = want < enough ? want : enough;
+        want = want < enough ? want : ring ? enough : enough | 1;
     }
     const bool split = !few && !tiles && want * units < kSplit;
     if (split) want = ((long long)x->max_len + 31) / 32;
