@@ -295,10 +295,10 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
 // (More rows than the launch was told of come in turns of as many; a cell's
 // weight is then added to by the lane that wrote it.)
 // The last 32 tokens of 32 heads over eight F16 caches of up to 20000 cells, 8 x
-// 128 with a bias: 57 us, 3.8 TB/s; its reads with one row tile of eight 49 us. (Asking once a
-// group of cells, not for each 16 rows, whether some row sees less: 62 us, 71
-// before, for two divisions and a branch beside eight products.) One token of 64
-// sequences of up to 16384 Q8_0 cells: 244 us.
+// 128 with a bias: 57 to 59 us, 3.7 TB/s; its reads with one row tile of eight 49
+// us. (Asking once a group of cells, not for each 16 rows, whether some row sees
+// less: 62 us, 71 before, for two divisions and a branch beside eight products.)
+// One token of 64 sequences of up to 16384 Q8_0 cells: 244 us.
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     using C = RowKernel<TYPE, QT, D, 1, COLS>;
