@@ -234,7 +234,7 @@ __device__ void plan_of(const PickArgs & p, int i, int & k, int & to, int & seq_
 constexpr int kList = 4096;
 
 template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArgs p) {
-    __shared__ int lds[kWaves], bins[2048], found[2], above[kWaves], same[kWaves], listed;
+    __shared__ int lds[kWaves], bins[2048], found[3], above[kWaves], same[kWaves], listed;
     __shared__ unsigned list[kList];   // low 21 bits of a key, and the wave
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // (a request's blocks on different dies and CUs: requests differ in length)
@@ -271,6 +271,7 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
     unsigned top = 0;
     int left = k;   // of the keys that begin with top's bits, how many are kept
     // the place of the histogram that the left-th largest is in; how many are in it
+    // (not read from bins: a wave ahead may be clearing them)
     auto find = [&](int shift) {
         __syncthreads();
         // from the top: thread t has places 2 t and 2 t + 1
@@ -285,11 +286,12 @@ template <bool FUSED> __global__ __launch_bounds__(kPick, 8) void k_pick(PickArg
             const bool second = left > before + n0;
             found[0] = 2047 - 2 * t - second;
             found[1] = left - before - (second ? n0 : 0);
+            found[2] = second ? n1 : n0;
         }
         __syncthreads();
         top |= (unsigned)found[0] << shift;
         left = found[1];
-        return bins[found[0]];
+        return found[2];
     };
     // f(four keys, their first cell) in ascending order (all lanes), the next four on their way
     auto each = [&](auto f) {
