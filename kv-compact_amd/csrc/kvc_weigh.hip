@@ -127,6 +127,7 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
     const int page_mask = (1 << a.shift) - 1;
 
     for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
+        if constexpr (SPLIT) __syncthreads();   // (wave 0 has read the last tile's sums; this one may have no rows, and no barrier of theirs)
         const int block0 = tile * CELLS, cell0 = SPLIT ? block0 : block0 + 32 * wave;
         int t0, t1;   // the block's tokens (a wave past the sequence's end has none that see its cells)
         tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
             if (m < 8) join[wave][at] = all;
             __syncthreads();
             all = (join[0][at] + join[1][at]) + (join[2][at] + join[3][at]);
-            if (wave) continue;   // (a next tile's sums come behind its barriers)
+            if (wave) continue;
         }
         if (m < 8) add_weight(w, c, h, cell0 + 16 * (m >> 2) + 4 * g + (m & 3), all);
     }
