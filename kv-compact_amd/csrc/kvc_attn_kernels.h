@@ -377,16 +377,20 @@ struct OddTiles {
         shift = hi - lo > 64 ? 26 - __builtin_clz(hi - lo - 1) : 0;
     }
     __device__ __forceinline__ void add(int t) { bits |= 1ull << ((t - t_lo) >> shift); }
-    // f(first key, key past the last) of each stretch
+    // f(first key, key past the last) of each stretch (WINDOW: in two where it goes
+    // from the first cells' tiles to the window's, not over what lies between)
     template <bool WINDOW, int KEYS, class F>
     __device__ __forceinline__ void each(const KeyTiles<WINDOW, KEYS> & at, int held, F f) const {
 #pragma nounroll
         for (unsigned long long m = bits; m; m &= m - 1) {
             const int t0 = t_lo + ((__ffsll((long long)m) - 1) << shift);
             const int t1 = t0 + (1 << shift) < t_hi ? t0 + (1 << shift) : t_hi;
-            // (a stretch may go over tiles that no row sees: their keys are hidden)
-            const int end = WINDOW ? (at.tile(t1 - 1) + 1) * KEYS : t1 * KEYS;
-            f(at.tile(t0) * KEYS, end < held ? end : held);
+#pragma nounroll
+            for (int t = t0, stop; t < t1; t = stop) {
+                stop = WINDOW && t < at.near && at.near < t1 ? at.near : t1;
+                const int end = (at.tile(stop - 1) + 1) * KEYS;
+                f(at.tile(t) * KEYS, end < held ? end : held);
+            }
         }
     }
 };
