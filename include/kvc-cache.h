@@ -269,7 +269,7 @@ int kvc_attn_cache_window(const kvc_cache * c, const kvc_cache_attn_args * a, co
  * that does not name every token that came since the last one; decay 0 begins
  * all at 0: nothing is read then. decay is from 0 to 1. tail > 0: only the last
  * `tail` tokens of each sequence are counted. Rows whose lse is -inf give
- * nothing; cells of a bad page gather nothing. Weights at or past the
+ * nothing, whatever their queries hold; cells of a bad page gather nothing. Weights at or past the
  * sequence's end are left as they were, and so are sequences without tokens, of
  * a bad number or with more tokens than cells. No sequence is named twice.
  * Types and limits as of kvc_attn_cache. No workspace. */

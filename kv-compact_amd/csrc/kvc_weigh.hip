@@ -58,6 +58,36 @@ __device__ __forceinline__ void tokens_of(const AttnArgs & a, const Counted & c,
     if (lo >= a.first && hi - 1 - c.q.base + a.last < t1) t1 = hi - 1 - c.q.base + a.last;
 }
 
+// Rows whose log-sum-exp is -inf give nothing, whatever their queries hold: cells
+// are hidden from them as they are by a mask. With few rows a block knows whether
+// it has such ones. The kernels for many rows take a log-sum-exp of +inf for them,
+// which gives 0 but for scores that are NaN or +inf, and go through a tile of cells
+// once more, masks everywhere, where a sum is NaN. (A look at each tile of rows:
+// 4096 tokens 156 us, 151 so; over Q8_0 460 and 447.)
+// Rows behind the last repeat it, with +inf; one that saw nothing keeps its -inf.
+__device__ __forceinline__ float row_log_sum(float lse, bool on) { return on || lse == -INFINITY ? lse : INFINITY; }
+
+// (what the first of two passes derives from x is not kept in registers for the second)
+__device__ __forceinline__ int opaque(int x) {
+    x = __builtin_amdgcn_readfirstlane(x);
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// Whether a sum of the block's is NaN (seen: a word a wave; all waves call).
+template <int N, int WAVES> __device__ __forceinline__ bool any_nan(const float (&sum)[N], int (&seen)[WAVES]) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) nan |= sum[i] != sum[i];
+    nan = __ballot(nan) != 0;
+    if ((threadIdx.x & 63) == 0) seen[threadIdx.x >> 6] = nan;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) any |= seen[i];
+    return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+
 __device__ __forceinline__ void add_weight(const WeighArgs & w, const Counted & c, int h, int cell, float sum) {
     if (cell >= c.q.held) return;
     float * at = w.weight + c.seq * w.w_seq + h * w.room + cell;
@@ -102,16 +132,19 @@ __device__ __forceinline__ float sum_of_16(float (&v)[8], int m) {
 // 16 RT at a time through LDS, as the fragments they are, for all four. SPLIT,
 // for few blocks: the four have the same 32 cells and every fourth row tile each.
 // Bound by what a row tile issues in turn (F32: 32 products in a chain of four
-// sums): 4096 tokens of 32 heads of 128, F32 1.09 ms, 64 TFLOP/s (a large product:
-// 152); over Q8_0 0.44 ms, 155 TFLOP/s, 16384 tokens 3.3 ms, 333 TFLOP/s.
+// sums): 4096 tokens of 32 heads of 128, F32 1.01 ms, 68 TFLOP/s (a large product:
+// 152); over Q8_0 0.45 ms, 154 TFLOP/s, 16384 tokens 3.3 ms, 332 TFLOP/s. 128-wide
+// heads have registers for three waves a SIMD (F32 1.09 ms and Q8_0 0.49 ms with
+// the two that the compiler takes by itself), F32 heads from 65 to 127 do not.
 template <int TYPE, int QT, int D, int RT, Columns COLS, bool SPLIT>
-__global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
+__global__ __launch_bounds__(256, D == 128 && !(TYPE == kF32 && COLS == PART) ? 3 : 1) void k_weigh_rows(WeighArgs w) {
     constexpr int CELLS = SPLIT ? 32 : 128;
     using C = RowKernel<TYPE, QT, D, 1, COLS>;
     constexpr bool Q8 = C::Q8;
     __shared__ __align__(16) u4 rows_q[RT][C::NK][64];
     __shared__ float rows_scale[Q8 ? RT : 1][2][16];
-    __shared__ float rows_lse[RT][16];
+    __shared__ float rows_lse[RT][2][16];   // as subtracted, and as given
+    __shared__ int sums_nan[4];
     __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
     __shared__ float join[SPLIT ? 4 : 1][32];
     const AttnArgs & a = w.a;
@@ -127,13 +160,11 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
     const int page_mask = (1 << a.shift) - 1;
 
     for (int tile = first_tile; (long long)tile * CELLS < q.held; tile += w.cell_tiles) {
-        if constexpr (SPLIT) __syncthreads();   // (wave 0 has read the last tile's sums; this one may have no rows, and no barrier of theirs)
+        __syncthreads();   // (what waves left each other of the last tile is read; this one may have no rows, and no barrier of theirs)
         const int block0 = tile * CELLS, cell0 = SPLIT ? block0 : block0 + 32 * wave;
         int t0, t1;   // the block's tokens (a wave past the sequence's end has none that see its cells)
         tokens_of(a, c, block0, block0 + CELLS < q.held ? block0 + CELLS : q.held, t0, t1);
         float sum[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum[i] = 0.0f;
         // keys, and the cells that rows may see (not those of bad pages or past the end)
         unsigned kr[2][C::NKL][Q8 ? 4 : C::WK];
         f4 ks[Q8 ? 2 : 1][Q8 ? C::NB : 1];
@@ -186,95 +217,104 @@ __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs w) {
                 for (int j = 0; j < C::NB; j++) ks[x][j] = *reinterpret_cast<const f4 *>(&k_scale[wave][j][16 * x + 4 * g]);
         }
         const int row_end = t1 * a.G;
-        for (int turn = t0 * a.G; turn < row_end; turn += 16 * RT) {
-            const int rows = row_end - turn < 16 * RT ? row_end - turn : 16 * RT, row_tiles = (rows + 15) >> 4;
-            __syncthreads();   // (the rows before are read)
-            for (int r = wave; r < row_tiles; r += 4) {
-                const bool on = 16 * r + m < rows;
-                const int row = turn + (on ? 16 * r + m : rows - 1), tok = row / a.G, head = row % a.G;
-                const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
-                u4 qf[C::NK];
+        for (bool again = false;; again = true) {
 #pragma unroll
-                for (int j = 0; j < C::NK; j++) {
-                    const int col = 4 * C::KV * j + C::KV * g;
-                    if constexpr (Q8) {
-                        qf[j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
-                    } else {
-                        unsigned x[4];
-                        load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, x);
-                        qf[j] = u4{x[0], x[1], x[2], x[3]};
+            for (int i = 0; i < 8; i++) sum[i] = 0.0f;
+            for (int turn = opaque(t0) * a.G; turn < row_end; turn += 16 * RT) {
+                const int rows = row_end - turn < 16 * RT ? row_end - turn : 16 * RT, row_tiles = (rows + 15) >> 4;
+                __syncthreads();   // (the rows before are read)
+                for (int r = wave; r < row_tiles; r += 4) {
+                    const bool on = 16 * r + m < rows;
+                    const int row = turn + (on ? 16 * r + m : rows - 1), tok = row / a.G, head = row % a.G;
+                    const char * p = a.q + ((long long)(q.tok0 + tok) * a.q_tok + (long long)(h * a.G + head) * a.q_head) * C::ES;
+                    u4 qf[C::NK];
+#pragma unroll
+                    for (int j = 0; j < C::NK; j++) {
+                        const int col = 4 * C::KV * j + C::KV * g;
+                        if constexpr (Q8) {
+                            qf[j] = COLS == FULL || col < a.dk ? *reinterpret_cast<const u4_any *>(p + 2 * col) : u4{0, 0, 0, 0};
+                        } else {
+                            unsigned x[4];
+                            load_cols<C::KV, C::ES, COLS>(p, 0, col, a.dk, x);
+                            qf[j] = u4{x[0], x[1], x[2], x[3]};
+                        }
+                    }
+                    float scale = a.scale, rest = 1.0f;
+                    if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(qf, a.scale, scale, rest);
+#pragma unroll
+                    for (int j = 0; j < C::NK; j++) rows_q[r][j][lane] = qf[j];
+                    if (g == 0) {
+                        const float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
+                        rows_lse[r][0][m] = on && lse != -INFINITY ? lse : INFINITY;
+                        rows_lse[r][1][m] = lse;
+                        if constexpr (Q8) {
+                            rows_scale[r][0][m] = scale;
+                            rows_scale[r][1][m] = rest;
+                        }
                     }
                 }
-                float scale = a.scale, rest = 1.0f;
-                if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(qf, a.scale, scale, rest);
+                __syncthreads();
+                if (cell0 >= q.held) continue;
+                for (int r = SPLIT ? wave : 0; r < row_tiles; r += SPLIT ? 4 : 1) {
+                    const int row0 = turn + 16 * r, last_row = row0 + 15 < row_end ? row0 + 15 : row_end - 1;
+                    const int first_tok = row0 / a.G, last_tok = last_row / a.G;
+                    if (!a.mask && cell0 > q.base + last_tok) continue;   // (no row of the tile sees the cells)
+                    u4 qf[C::NK];
 #pragma unroll
-                for (int j = 0; j < C::NK; j++) rows_q[r][j][lane] = qf[j];
-                if (g == 0) {
-                    const float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
-                    rows_lse[r][m] = on && lse != -INFINITY ? lse : INFINITY;   // (a row that saw nothing gives nothing)
-                    if constexpr (Q8) {
-                        rows_scale[r][0][m] = scale;
-                        rows_scale[r][1][m] = rest;
-                    }
-                }
-            }
-            __syncthreads();
-            if (cell0 >= q.held) continue;
-            for (int r = SPLIT ? wave : 0; r < row_tiles; r += SPLIT ? 4 : 1) {
-                const int row0 = turn + 16 * r, last_row = row0 + 15 < row_end ? row0 + 15 : row_end - 1;
-                const int first_tok = row0 / a.G, last_tok = last_row / a.G;
-                if (!a.mask && cell0 > q.base + last_tok) continue;   // (no row of the tile sees the cells)
-                u4 qf[C::NK];
-#pragma unroll
-                for (int j = 0; j < C::NK; j++) qf[j] = rows_q[r][j][lane];
-                const float lse = rows_lse[r][m], scale = Q8 ? rows_scale[r][0][m] : a.scale, rest = Q8 ? rows_scale[r][1][m] : 1.0f;
-                const int clear = a.mask ? q.base : q.base + first_tok + 1;
-                const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
-                const bool special = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
-                unsigned see = ~0u;
-                if (special) {
-                    const int tok = (row0 + m < row_end ? row0 + m : row_end - 1) / a.G;
-                    see = seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
-                }
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    f4 sc = {0, 0, 0, 0};
-                    if constexpr (TYPE == kF32) {
-                        f4 part[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) part[e] = f4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < C::NKL; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][j][e]),
-                                                                               __uint_as_float(qf[j][e]), part[e], 0, 0, 0);
-                        sc = (part[0] + part[1]) + (part[2] + part[3]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
-                        const u4 kf = {kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]};
-                        if constexpr (Q8)
-                            sc += ks[x][j] * mfma16<kF16>(kf, qf[j], f4{0, 0, 0, 0});
-                        else
-                            sc = mfma16<C::MT>(kf, qf[j], sc);
-                    }
-                    float p[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
-                        float v = sc[i];
-                        if constexpr (Q8 && QT == kBF16) v *= rest;
-                        p[i] = exp_of(__builtin_fmaf(v, scale, bias[x][i]) - lse);
-                    }
+                    for (int j = 0; j < C::NK; j++) qf[j] = rows_q[r][j][lane];
+                    const float lse = rows_lse[r][0][m], scale = Q8 ? rows_scale[r][0][m] : a.scale, rest = Q8 ? rows_scale[r][1][m] : 1.0f;
+                    const int clear = a.mask ? q.base : q.base + first_tok + 1;
+                    const int from = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
+                    const bool special = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from) || again;
+                    unsigned see = ~0u;
                     if (special) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) p[i] = see >> (16 * x + 4 * g + i) & 1 ? p[i] : 0.0f;
+                        const int tok = (row0 + m < row_end ? row0 + m : row_end - 1) / a.G;
+                        see = rows_lse[r][1][m] == -INFINITY ? 0 : seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
+                    for (int x = 0; x < 2; x++) {
+                        f4 sc = {0, 0, 0, 0};
+                        if constexpr (TYPE == kF32) {
+                            f4 part[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) part[e] = f4{0, 0, 0, 0};
+#pragma unroll
+                            for (int j = 0; j < C::NKL; j++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][j][e]),
+                                                                                   __uint_as_float(qf[j][e]), part[e], 0, 0, 0);
+                            sc = (part[0] + part[1]) + (part[2] + part[3]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < (TYPE == kF32 ? 0 : C::NKL); j++) {
+                            const u4 kf = {kr[x][j][0], kr[x][j][1], kr[x][j][2], kr[x][j][3]};
+                            if constexpr (Q8)
+                                sc += ks[x][j] * mfma16<kF16>(kf, qf[j], f4{0, 0, 0, 0});
+                            else
+                                sc = mfma16<C::MT>(kf, qf[j], sc);
+                        }
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
+                            float v = sc[i];
+                            if constexpr (Q8 && QT == kBF16) v *= rest;
+                            p[i] = exp_of(__builtin_fmaf(v, scale, bias[x][i]) - lse);
+                        }
+                        if (special) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) p[i] = see >> (16 * x + 4 * g + i) & 1 ? p[i] : 0.0f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
+                    }
                 }
             }
+            if (again) break;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
+            if (!any_nan(sum, sums_nan)) break;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] = there >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1 ? sum[i] : 0.0f;
@@ -309,6 +349,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     __shared__ __align__(16) u4 rows_q[RT > 1 ? RT : 1][RT > 1 ? C::NK : 1][64];
     __shared__ float rows_scale[RT > 1 && Q8 ? RT : 1][2][16];
     __shared__ float rows_lse[RT > 1 ? RT : 1][16];
+    __shared__ int rows_nothing[4];
     __shared__ __align__(16) float k_scale[Q8 ? 4 : 1][Q8 ? C::NB : 1][32];
     const AttnArgs & a = w.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -349,7 +390,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
         rest = 1.0f;
         if constexpr (Q8 && QT == kBF16) bf16_row_to_f16(x, a.scale, scale, rest);
         lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
-        lse = on && lse != -INFINITY ? lse : INFINITY;
+        lse = row_log_sum(lse, on);
     };
 
     unsigned kr[2][C::NKL][C::WK], next_kr[AHEAD ? 2 : 1][AHEAD ? C::NKL : 1][C::WK];
@@ -409,12 +450,15 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
             if (t0 < g_hi) load_keys(t0, page, next_kr);
         u4 q0[C::NK];
         float lse0 = 0.0f, scale0 = 0.0f, rest0 = 0.0f;
+        bool nothing = false;   // a row with a log-sum-exp of -inf
         if constexpr (RT == 1) {
             load_row(m, q0, lse0, scale0, rest0);
+            nothing = __ballot(lse0 == -INFINITY) != 0;
         } else {
             if (row_lo) __syncthreads();   // (the rows before are read)
             for (int r = wave; r < row_tiles; r += 4) {
                 load_row(16 * r + m, q0, lse0, scale0, rest0);
+                nothing |= lse0 == -INFINITY;
 #pragma unroll
                 for (int j = 0; j < C::NK; j++) rows_q[r][j][lane] = q0[j];
                 if (g == 0) {
@@ -425,7 +469,10 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
                     }
                 }
             }
+            nothing = __ballot(nothing) != 0;
+            if (lane == 0) rows_nothing[wave] = nothing;
             __syncthreads();
+            nothing = __builtin_amdgcn_readfirstlane(rows_nothing[0] | rows_nothing[1] | rows_nothing[2] | rows_nothing[3]);
         }
 
         for (int t = t0; t < g_hi; t += 4) {
@@ -490,7 +537,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
                 unsigned see = ~0u;
                 if (hides) {
                     const int row = row0 + m < rows ? row0 + m : rows - 1, tok = c.tok_from + (row_lo + row) / a.G;
-                    see = seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
+                    see = lse == -INFINITY ? 0 : seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0);
                 }
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
@@ -536,7 +583,7 @@ __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
                     for (int i = 0; i < 4; i++) sum[4 * x + i] += p[i];
                 }
             };
-            const bool hides = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from);
+            const bool hides = cell0 + 32 > clear || (cell0 + 32 > a.first && cell0 < from) || nothing;
             if constexpr (RT == 1) {
                 sixteen(0, hides);
             } else if (hides) {
@@ -676,7 +723,7 @@ __global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
             }
         }
         float lse = a.lse[(long long)(q.tok0 + tok) * a.H * a.G + h * a.G + head];
-        lse = on && lse != -INFINITY ? lse : INFINITY;
+        lse = row_log_sum(lse, on);
         const int first_tok = c.tok_from + row_lo / a.G, last_tok = c.tok_from + (row_lo + rows - 1) / a.G;
         const int clear = a.mask ? q.base : q.base + first_tok + 1;
         const int cut = a.mask ? q.base - (q.n_new < a.last ? a.last - q.n_new : 0) : q.base + last_tok + 1 - a.last;
@@ -685,6 +732,7 @@ __global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
 #pragma unroll
         for (int j = 0; j < C::NK; j++) asm volatile("" : "+v"(qf[j]));
         asm volatile("" : "+v"(lse));
+        const bool nothing = __ballot(lse == -INFINITY) != 0;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) fill();
 
@@ -715,8 +763,8 @@ __global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
             // (the difference before log2 e: its rounding goes with the weight's size, not the score's)
 #pragma unroll
             for (int i = 0; i < 4; i++) p[i] = exp_of(__builtin_fmaf(sc[i], a.scale, bias[i]) - lse);
-            if (cell0 + 16 > clear || (cell0 + 16 > a.first && cell0 < cut)) {
-                const unsigned see = seen32(a, q, tok, cell0) & window32(a, from, cell0);
+            if (cell0 + 16 > clear || (cell0 + 16 > a.first && cell0 < cut) || nothing) {
+                const unsigned see = lse == -INFINITY ? 0 : seen32(a, q, tok, cell0) & window32(a, from, cell0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) p[i] = see >> (4 * g + i) & 1 ? p[i] : 0.0f;
             }
@@ -782,6 +830,7 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
     __shared__ __align__(16) char lds[BUFS][ROWS * ROWB];
     __shared__ float row_lse[BUFS][ROWS];
     __shared__ float join[RW == 2 ? 4 : 1][16][2];
+    __shared__ int sums_nan[WAVES];
 
     const AttnArgs & a = w.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -829,9 +878,8 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
         if (cell0 >= q.held) wt1 = wt0;
 
         // the next tile to load: its first token, its place, its rows and log-sum-exps
-        int load_tt = t0, load_buf = 0;
-        const char * load_q = a.q + 2 * ((long long)(q.tok0 + t0) * a.q_tok + (long long)(h * a.G) * a.q_head);
-        const char * load_l = reinterpret_cast<const char *>(a.lse + (long long)(q.tok0 + t0) * a.H * a.G + h * a.G);
+        int load_tt, load_buf;
+        const char *load_q, *load_l;
         const long long q_step = 2 * T * a.q_tok, l_step = 4LL * T * a.H * a.G;
         auto fill = [&] {
             const int most = t1 - 1 - load_tt;
@@ -891,16 +939,7 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 16; i++) sum[i] = 0.0f;
         }
-        if (t0 < t1) {
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) fill();
-        }
-        // (the keys are waited for here: a wait in the loop would be one for the rows on their way too)
-#pragma unroll
-        for (int j = 0; j < KS; j++) asm volatile("" : "+v"(kf[j]));
         auto arrive = [&] {
             wait_lds_loads<(AHEAD - 1) * LOADS>();
             __builtin_amdgcn_s_barrier();
@@ -917,11 +956,10 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
 #pragma unroll
                 for (int i = 0; i < 16; i++) sc[r][i] = 0.0f;
                 const float lse = row_lse[buf][64 * rw + 32 * r + n];
-                // (a row that saw nothing gives nothing, nor does one past the last)
                 l2[r] = lse == -INFINITY || !my_on[r] || tt + my_tok[r] >= t1 ? INFINITY : BIAS ? lse : lse * kLog2e;
                 if constexpr (!PLAIN) {
                     const int tok = tt + my_tok[r] < t1 ? tt + my_tok[r] : t1 - 1;
-                    see[r] = (seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0)) >> (4 * hf);
+                    see[r] = lse == -INFINITY ? 0 : (seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0)) >> (4 * hf);
                 }
             }
             // four of a row's scores to weights (PLAIN: exponentials side by side, with products around them)
@@ -988,25 +1026,49 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
             w_hi = cell0 + 32 > a.first && cell0 - q.base + a.last - T + 1 < t1 ? cell0 - q.base + a.last - T + 1 : t1;
         }
         if (w_hi <= w_lo) w_lo = w_hi = t1;
-        int tt = t0, buf = 0;
+        int tt, buf;
         auto next = [&] {
             tt += T;
             buf = buf + 1 < BUFS ? buf + 1 : 0;
         };
-        while (tt < t1) {
-            const int stop = tt >= w_hi ? t1 : w_lo < t1 ? w_lo : t1;
-            while (tt < stop) {
-                arrive();
-                if (tt + T > wt0 && tt < wt1) step(tt, buf, std::false_type{});
-                next();
+        for (bool again = false;; again = true) {
+            const int tok_lo = opaque(t0);
+            load_tt = tok_lo;
+            load_buf = 0;
+            load_q = a.q + 2 * ((long long)(q.tok0 + tok_lo) * a.q_tok + (long long)(h * a.G) * a.q_head);
+            load_l = reinterpret_cast<const char *>(a.lse + (long long)(q.tok0 + tok_lo) * a.H * a.G + h * a.G);
+#pragma unroll
+            for (int i = 0; i < 16; i++) sum[i] = 0.0f;
+            if (t0 < t1) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) fill();
             }
-            while (tt < w_hi && tt < t1) {
-                arrive();
-                step(tt, buf, std::true_type{});
-                next();
+            // (the keys are waited for here: a wait in the loop would be one for the rows on their way too)
+#pragma unroll
+            for (int j = 0; j < KS; j++) asm volatile("" : "+v"(kf[j]));
+            tt = tok_lo;
+            buf = 0;
+            while (tt < t1) {
+                const int stop = tt >= w_hi ? t1 : w_lo < t1 ? w_lo : t1;
+                while (tt < stop) {
+                    arrive();
+                    if (tt + T > wt0 && tt < wt1) step(tt, buf, std::false_type{});
+                    next();
+                }
+                while (tt < w_hi && tt < t1) {
+                    arrive();
+                    step(tt, buf, std::true_type{});
+                    next();
+                }
             }
+            wait_lds_loads<0>();
+            if (again) break;
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = there >> (8 * (i >> 2) + 4 * hf + (i & 3)) & 1 ? sum[i] : 0.0f;
+            if (!any_nan(v, sums_nan)) break;
+            w_lo = w_hi = t1;
         }
-        wait_lds_loads<0>();
         // over a half's 32 lanes: each step hands half of the sums to the lane across, until each holds one cell's
         float v[16];
 #pragma unroll

@@ -43,7 +43,7 @@ def exe(tmp_path_factory):
     return d / "weigh_rows"
 
 
-def run(exe, split, first, cells, tokens, window, tiles, H=1, G=4, page=16, decay=0.5, seed=0):
+def run(exe, split, first, cells, tokens, window, tiles, H=1, G=4, page=16, decay=0.5, seed=0, out=()):
     rng = np.random.default_rng(seed)
     pages = -(-cells // page)
     n_pages = pages + 1
@@ -54,6 +54,9 @@ def run(exe, split, first, cells, tokens, window, tiles, H=1, G=4, page=16, deca
     seen = window_seen(cells, tokens, window[0], window[1])
     rows = k[table].reshape(-1, H, 64)[:cells].astype(np.float64)
     lse = log_sums(q.astype(np.float64), rows, None, seen, 0.125)
+    for i, h in out:   # rows whose log-sum-exp is -inf, and whose queries are not finite
+        lse[i, h] = -np.inf
+        q[i, h, i % 5::7] = np.nan if i % 2 else np.inf
     want, tol = weights_of(q.astype(np.float64), rows, None, seen, 0.125, lse.astype(np.float64), 0)
     had = old[:, :cells].astype(np.float64)
     had[:, cells - tokens:] = 0
@@ -79,3 +82,12 @@ def test_tiles_that_no_token_sees(exe, split, first, tiles):
 def test_prompts(exe, split, first):
     run(exe, split, first, 150, 150, (0, 1 << 30), 1, H=2, G=3)
     run(exe, split, first, 150, 40, (5, 20), 2, H=2, G=3, page=32)
+
+
+@pytest.mark.parametrize("split", [True, False])
+@pytest.mark.parametrize("first", [0, 1, 2, 3, -1])
+def test_rows_left_out(exe, split, first):
+    # (their scores are NaN: tiles of cells are gone through twice, beside others that no token sees)
+    run(exe, split, first, 400, 20, (20, 30), 1, out=[(3, 0), (8, 2), (19, 3)])
+    run(exe, split, first, 300, 60, (0, 1 << 30), 1, G=2, out=[(0, 0), (33, 1), (59, 1)])
+    run(exe, split, first, 200, 40, (5, 20), 2, G=2, out=[(i, h) for i in range(40) for h in (0, 1)])
