@@ -1143,7 +1143,7 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     WeighArgs w{};
     w.room = (long long)c->max_pages * c->page_size;
     w.w_seq = w.room * c->n_head_kv;
-    w.weight = y->weight + x->layer * c->max_seqs * w.w_seq;
+    w.weight = y->weight + (long long)x->layer * c->max_seqs * w.w_seq;
     w.decay = y->decay;
     w.tail = y->tail;
     w.fresh = y->fresh;
