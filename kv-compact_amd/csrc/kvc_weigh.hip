@@ -668,8 +668,10 @@ __global__ __launch_bounds__(256) void k_weigh_ring(WeighArgs w) {
         load_off[i] = __umul24(row, a.k.ld_tok) + 16 * piece;
         load_on[i] = piece * C::KV < a.dk;
     }
-    if (a.dk < D)
+    if (a.dk < D) {
         for (int i = lane; i < BUFS * 16 * PR; i += 64) reinterpret_cast<u4 *>(ring[wave])[i] = u4{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (direct loads take another way to LDS)
+    }
 
     for (int row_lo = 0; row_lo < all_rows; row_lo += 16) {           // (more rows than the launch was told of: in turns)
         const int rows = all_rows - row_lo < 16 ? all_rows - row_lo : 16;
