@@ -540,8 +540,12 @@ int kvc_cache_pick(const kvc_cache * c, int n, const kvc_pick_args * a, void * w
     // those blocks are few and long: 32 layers, 20 % of one sequence kept and its
     // weights moved, us (own launch, picking blocks): 5120 cells 20.6 and 20.0,
     // 16384 30.6 and 36.7, 32768 48.6 and 63.9; 4 of up to 32768 79 both, 8 103
-    // both, 16 of up to 8192 62.3 and 54.1.
-    const bool fused = units >= 256 || p.max_len <= 8192;
+    // both, 16 of up to 8192 62.3 and 54.1. One list for all layers has a block a
+    // request, and a thread adds layers x heads: 32 layers of 8, 5120 cells 31.4 and
+    // 175, 16 of up to 8192 57.4 and 204, 256 of up to 2048 306 and 373; 8 layers 5120
+    // cells 21.9 and 34.2; 2 layers 2000 cells 17.8 and 17.1.
+    const bool alone = p.groups == 1 && p.n_layers > 1;
+    const bool fused = !alone && (units >= 256 || p.max_len <= 8192);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice dev(st);
     if (!dev.ok) return KV_COMPACT_E_DEVICE;

@@ -79,6 +79,20 @@ int main() {
         CHECK(to == at<float>(4ull * layer * (1 << 20) * 2 * 48));
     }
     wanted = 0;
+    // a list for each layer of one sequence: one launch; one for all layers: the keys by blocks of their own, too
+    for (int layers : {1, 8, 32}) {
+        const kvc_cache c = cache(layers, 4, 8, 128, 64, KV_TYPE_F16);
+        kvc_pick_args k{};
+        k.seqs = k.start = k.keep = at<int>(0), k.weight = at<float>(0), k.idx = k.cu = k.granted = k.status = at<int>(0);
+        k.n_idx = 1000, k.max_len = 5120;
+        int before = launches;
+        CHECK(kvc_cache_pick(&c, 1, &k, base, kvc_cache_pick_workspace(&c, 1, &k), nullptr) == 0);
+        CHECK(launches - before == (layers > 1 ? 2 : 1));
+        k.ld_idx = 1000;
+        before = launches;
+        CHECK(kvc_cache_pick(&c, 1, &k, base, kvc_cache_pick_workspace(&c, 1, &k), nullptr) == 0);
+        CHECK(launches - before == 1);
+    }
     // sizes that arguments can announce
     unsigned long long x = 88172645463325252ull;
     auto any = [&](long long most) {   // spread over the logarithm
