@@ -27,6 +27,8 @@ struct WeighArgs {
     int tail, fresh;
     int cell_tiles;        // blocks of a sequence's head
     int range;             // k_weigh_few, k_weigh_ring: groups of 32 or 64 cells of each, at least
+    float to_log2;         // k_weigh_tiles: scale times log2 e, rounded
+    float lse_log2[2];     // the same of a log-sum-exp: to_log2 / scale in two parts
 };
 
 // What a block of a call works on.
@@ -815,7 +817,11 @@ template <int TYPE> bool run_weigh_ring(const WeighArgs & w, long long blocks, h
 // rows; they join in LDS.
 //
 // Without a bias the scores go into the exponential by one multiply-add (scale
-// and log2 e in one factor: each rounded once, as the separate steps are).
+// and log2 e in one factor). What that factor's rounding does to a score is done to
+// the log-sum-exp too, by its own factor in two parts, so that it goes with their
+// difference, and one rounding, of the log-sum-exp's product, with the score's size,
+// as the score's own does in the other kernels. (With log2 e for the log-sum-exps:
+// twice the error, scores of 5600 off by 3.4e-4 where half a step is 2.4e-4.)
 //
 // Bound by the exponentials: 512 of a tile's 900 cycles of vector instructions in
 // a wave, its products 512 beside them. A prompt of 16384 tokens of 32 heads of
@@ -846,7 +852,7 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
     const Sequence & q = c.q;
     const int page_mask = (1 << a.shift) - 1;
     const int T = ROWS / a.G;                                 // tokens of a tile
-    const float to_log2 = a.scale * kLog2e;
+    const float to_log2 = w.to_log2;
     // places of a tile's rows: this lane's two, and those it loads
     int my_tok[2];
     bool my_on[2];
@@ -958,7 +964,8 @@ __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void
 #pragma unroll
                 for (int i = 0; i < 16; i++) sc[r][i] = 0.0f;
                 const float lse = row_lse[buf][64 * rw + 32 * r + n];
-                l2[r] = lse == -INFINITY || !my_on[r] || tt + my_tok[r] >= t1 ? INFINITY : BIAS ? lse : lse * kLog2e;
+                const float less = BIAS ? lse : __builtin_fmaf(lse, w.lse_log2[0], lse * w.lse_log2[1]);
+                l2[r] = fabsf(lse) == INFINITY || !my_on[r] || tt + my_tok[r] >= t1 ? INFINITY : less;
                 if constexpr (!PLAIN) {
                     const int tok = tt + my_tok[r] < t1 ? tt + my_tok[r] : t1 - 1;
                     see[r] = lse == -INFINITY ? 0 : (seen32(a, q, tok, cell0) & window32(a, window_from(a, q, tok), cell0)) >> (4 * hf);
@@ -1149,6 +1156,13 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     w.decay = y->decay;
     w.tail = y->tail;
     w.fresh = y->fresh;
+    w.to_log2 = a.scale * kLog2e;
+    {
+        // (scales that leave no whole fraction of a float: scores are 0 then, or not finite)
+        const double near = (double)w.to_log2 / a.scale, of = near > 1.4 && near < 1.5 ? near : 1.44269504088896340736;
+        w.lse_log2[0] = (float)of;
+        w.lse_log2[1] = (float)(of - w.lse_log2[0]);
+    }
     const int es = esize(x->type);
     const bool careful = c->k_type != kQ8 && (!vec_rows(x->q, es) || c->d_k * es % 16);
     const long long rows = (long long)(y->tail > 0 && y->tail < x->max_new ? y->tail : x->max_new) * a.G;
