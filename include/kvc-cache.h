@@ -269,10 +269,12 @@ int kvc_attn_cache_window(const kvc_cache * c, const kvc_cache_attn_args * a, co
  * that does not name every token that came since the last one; decay 0 begins
  * all at 0: nothing is read then. decay is from 0 to 1. tail > 0: only the last
  * `tail` tokens of each sequence are counted. Rows whose lse is -inf give
- * nothing, whatever their queries hold; cells of a bad page gather nothing. Weights at or past the
- * sequence's end are left as they were, and so are sequences without tokens, of
- * a bad number or with more tokens than cells. No sequence is named twice.
- * Types and limits as of kvc_attn_cache. No workspace. */
+ * nothing, whatever their queries hold; cells of a bad page gather nothing.
+ * Weights at or past the sequence's end are left as they were, and so are
+ * sequences without tokens, of a bad number or with more tokens than cells. No
+ * sequence is named twice. A call of few tokens (up to 128 rows of a KV head; F32
+ * 64) reads the keys of every cell, under a window too. Types and limits as of
+ * kvc_attn_cache. No workspace. */
 typedef struct kvc_weigh_args {
     float * weight;
     float decay;

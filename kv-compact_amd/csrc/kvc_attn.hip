@@ -118,7 +118,8 @@ CacheShape cache_shape(const kvc_cache * c, const kvc_cache_attn_args * a, const
     // heads: 2 sequences that see 512 cells 19, 23 and 33, 2048 23, 24 and 34,
     // 8192 47, 38 and 46; 8 sequences: 20, 25 and 35; 44, 39 and 45; 140, 94 and
     // 90; 16 and 2048: 71, 55 and 64; 32: 53, 53 and 46; 132, 108 and 91; 566, 351
-    // and 288.
+    // and 288. (The keys alone do not tell all: 32 sequences of 512 are given two,
+    // where four are faster, because 8 of 2048, as many keys, do better with two.)
     if (w && s.rt > 1 && c->k_type == kQ8) {
         const long long keys = (long long)max_len * a->n_seq * c->n_head_kv;
         s.rt = keys < 1 << 16 ? 1 : keys < 400000 || s.rt == 2 ? 2 : 4;

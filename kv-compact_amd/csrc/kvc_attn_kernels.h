@@ -17,9 +17,9 @@
 // its own (kvc_window). Key tiles that no row of a row tile sees are left out:
 // tiles are numbered without them, and one number of tiles to skip turns that
 // into the keys' (KeyTiles). Prompts of 32 heads of 128 over 8, bf16: 32768 tokens
-// under a window of 4096 2.2 ms, 930 TFLOP/s; 16384 tokens in 12 ragged prompts
-// under 1024 300 us, 640 TFLOP/s: a block has 12 tiles, and its beginning costs
-// five more. Over a cache: one token of 64 sequences that see 4112 cells 195 us,
+// under a window of 4096 2.2 to 2.4 ms, 870 to 947 TFLOP/s by the card; 16384 tokens
+// in 12 ragged prompts under 1024 299 to 319 us, 600 to 640 TFLOP/s: a block has 12
+// tiles, and its beginning costs five more. Over a cache: one token of 64 sequences that see 4112 cells 195 us,
 // 5.5 TB/s; 13 drafts over 16 Q8_0 caches that see 2065 56 us, bound by the
 // latency of a wave's next tile (one tile ahead, one wave a SIMD).
 #pragma once

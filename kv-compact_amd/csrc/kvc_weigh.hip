@@ -2,9 +2,11 @@
 // (include/kvc-cache.h, kvc_cache_weigh):
 //   w[h][j] = decay w[h][j] + sum over the tokens i that see cell j and the
 //             query heads of group h of exp(scale q_i.k_j + bias_j - lse_i).
-// With the rows' log-sum-exps at hand there is no running maximum and nothing
-// to join: a block keeps its cells' keys and goes over the rows, so that a
-// cell's sum is one wave's, in one order, and needs no atomics.
+// With the rows' log-sum-exps at hand there is no running maximum: a block keeps
+// its cells' keys and goes over the rows, so that a cell's sum is one block's, in
+// one order, and needs no atomics. It is one wave's, but in the forms for few
+// blocks, where two waves (k_weigh_tiles) or four (k_weigh_rows) share out the
+// rows and join their parts in LDS.
 //
 // The product is S^T[key][row] = K Q^T as in the attention kernels: a lane
 // holds one row of the caller's, so its log-sum-exp is one register, and adds
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(256, D == 128 && !(TYPE == kF32 && COLS == PART) ? 
 // 128 with a bias: 57 to 59 us, 3.7 TB/s; its reads with one row tile of eight 49
 // us. (Asking once a group of cells, not for each 16 rows, whether some row sees
 // less: 62 us, 71 before, for two divisions and a branch beside eight products.)
-// One token of 64 sequences of up to 16384 Q8_0 cells: 244 us.
+// One token of 64 sequences of up to 16384 Q8_0 cells: 242 us.
 template <int TYPE, int QT, int D, int RT, Columns COLS>
 __global__ __launch_bounds__(256) void k_weigh_few(WeighArgs w) {
     using C = RowKernel<TYPE, QT, D, 1, COLS>;
@@ -825,9 +827,9 @@ template <int TYPE> bool run_weigh_ring(const WeighArgs & w, long long blocks, h
 //
 // Bound by the exponentials: 512 of a tile's 900 cycles of vector instructions in
 // a wave, its products 512 beside them. A prompt of 16384 tokens of 32 heads of
-// 128: 1.21 to 1.24 ms, 890 to 911 TFLOP/s (a large product: 1208; with two waves a
-// SIMD, 64 cells each, 1.40 ms); 32768 tokens 963 TFLOP/s, 4096 tokens, eight
-// waves a block, 162 us (224 with four).
+// 128: 1.19 to 1.30 ms by the card, 847 to 922 TFLOP/s (a large product: 1170 to
+// 1240; with two waves a SIMD, 64 cells each, 1.40 ms); 32768 tokens 956 TFLOP/s,
+// 4096 tokens, eight waves a block, 151 to 162 us (224 with four).
 template <int TYPE, int D, bool BIAS, int RW>
 __global__ __launch_bounds__(256 * RW, D == 256 || BIAS || RW == 2 ? 2 : 3) void k_weigh_tiles(WeighArgs w) {
     constexpr int CELLS = 128, ROWS = 64 * RW, KS = D / 16, CH = D / 8, ROWB = 2 * D;
@@ -1186,7 +1188,9 @@ extern "C" int kvc_cache_weigh(const kvc_cache * c, const kvc_cache_attn_args * 
     // CU at the same range of every sequence): 2048, 2560 and 4096 blocks, 32
     // tokens, 8 of up to 20000 55, 53 and 60, 24 of up to 16000 134, 133 and 132;
     // Q8_0, one token, 64 of up to 16384 in 4, 5, 7 and 8 ranges 312, 246, 230 and
-    // 256, 128 of up to 8192 in 2, 3 and 4 ranges 309, 231 and 307.
+    // 256, 128 of up to 8192 in 2, 3 and 4 ranges 309, 231 and 307: the rule takes 5,
+    // where 7 would be faster, and 3. Under a window all cells' keys are read here all
+    // the same, and hidden ones multiplied for nothing.
     long long want = ((long long)x->max_len + 127) / 128;
     if (few) {
         const int least = ring ? 512 : 256, fill = ring ? 16384 : 2560;
