@@ -378,7 +378,9 @@ struct OddTiles {
     }
     __device__ __forceinline__ void add(int t) { bits |= 1ull << ((t - t_lo) >> shift); }
     // f(first key, key past the last) of each stretch (WINDOW: in two where it goes
-    // from the first cells' tiles to the window's, not over what lies between)
+    // from the first cells' tiles to the window's, not over what lies between. One
+    // token of 16 sequences of up to 131072 cells that see 4112, one infinity among
+    // the first cells of each: 148 us, 51 without.)
     template <bool WINDOW, int KEYS, class F>
     __device__ __forceinline__ void each(const KeyTiles<WINDOW, KEYS> & at, int held, F f) const {
 #pragma nounroll
